@@ -18,7 +18,8 @@ from ._capi import (AdamGroup, Camera as _CCamera, GaussianGrads as _CGrads, Gau
 from ._capi import INVALID_ARGUMENT, INVALID_STATE, NOT_SUPPORTED, OUT_OF_RANGE  # noqa: F401
 
 __all__ = ["GsxError", "Camera", "RenderContext", "Renderer", "Loss", "Adam", "ParamGroup", "l1_ssim",
-           "sort_pairs", "build", "FORWARD_INFERENCE", "FORWARD_TRAIN", "FIELDS"]
+           "sort_pairs", "build", "FORWARD_INFERENCE", "FORWARD_TRAIN", "FIELDS", "embedding_lookup",
+           "embedding_backward", "budget_accumulate", "budget_select", "budget_gather"]
 
 FORWARD_INFERENCE = 0
 FORWARD_TRAIN = 1
@@ -416,3 +417,15 @@ def sort_pairs(context: RenderContext, keys, values, begin_bit: int = 0, end_bit
         raise GsxError(INVALID_ARGUMENT, "keys and values must have the same length")
     check(lib().gsx_b200_sort_pairs(context.handle, _ptr(keys), _ptr(values), keys.numel(), begin_bit, end_bit,
                                     _stream_handle(stream)))
+
+
+def __getattr__(name):
+    # the embedding and budget calls import torch, which the rest of this module imports on use only
+    if name in ("embedding_lookup", "embedding_backward"):
+        from . import embedding as module
+    elif name in ("budget_accumulate", "budget_select", "budget_gather"):
+        from . import budget as module
+    else:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    globals()[name] = value = getattr(module, name)
+    return value

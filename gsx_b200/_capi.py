@@ -55,6 +55,12 @@ class AdamGroup(ctypes.Structure):
                 ("inv_bias_correction1", ctypes.c_double), ("inv_bias_correction2", ctypes.c_double)]
 
 
+class GatherField(ctypes.Structure):
+    _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p)] + [
+        (k, ctypes.c_uint64) for k in ("row_bytes", "src_outer_stride", "src_inner_stride", "src_row_stride",
+                                       "dst_outer_stride", "dst_inner_stride", "dst_row_stride")]
+
+
 # every exported symbol with its argument types (also the list the export test checks)
 SIGNATURES = {
     "gsx_b200_last_error": (ctypes.c_char_p, []),
@@ -115,7 +121,29 @@ SIGNATURES = {
     "gsx_b200_fill_pattern": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_uint32,
                                              ctypes.c_void_p]),
     "gsx_b200_count_nonfinite_f32": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_void_p]),
+    "gsx_b200_embedding_lookup": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_int,
+        ctypes.c_uint64, ctypes.c_float, ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64, ctypes.c_void_p,
+        ctypes.c_void_p]),
+    "gsx_b200_embedding_workspace_bytes": (ctypes.c_uint64, [ctypes.c_uint64, ctypes.c_uint64, ctypes.c_uint64]),
+    "gsx_b200_embedding_backward": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64, ctypes.c_float,
+        ctypes.c_int64, ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_int,
+        ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_void_p]),
+    "gsx_b200_budget_accumulate": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64, ctypes.c_uint64,
+        ctypes.c_uint64, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_float,
+        ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p]),
+    "gsx_b200_budget_workspace_bytes": (ctypes.c_uint64, [ctypes.c_uint64, ctypes.c_uint64]),
+    "gsx_b200_budget_select": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_uint64,
+        ctypes.c_uint64, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_void_p,
+        ctypes.c_uint64, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p]),
+    "gsx_b200_budget_gather": (ctypes.c_int, [
+        ctypes.POINTER(GatherField), ctypes.c_int32, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_uint64,
+        ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
 }
+GATHER_MAX_FIELDS = 32
 NOALLOC_SORT_MAX_PAIRS = 1 << 20
 
 _lib = None

@@ -1,0 +1,140 @@
+"""Keeping the Gaussians of a scene, or the rows of key-value caches, within a budget by accumulated weight
+(gsx_b200_budget_*).
+
+A score tensor is [length] for one set of entries (a scene) or [.., length] for several (one per batch entry and
+head); `lengths`, where given, is an int32 tensor of the leading shape with the entries in use."""
+from __future__ import annotations
+
+import torch
+
+from ._capi import GATHER_MAX_FIELDS, NOT_SUPPORTED, OUT_OF_RANGE, GatherField, GsxError, lib
+from ._tensors import FLOAT_TYPES, below_2_31, empty, group_stride, invalid, launch, on_device, type_code, word
+
+
+def _score(score, name="score"):
+    """(groups, length, stride between groups) of a score tensor."""
+    if score.dim() < 1 or score.dtype != torch.float32:
+        raise invalid(f"{name} must be a float32 tensor of at least one dimension")
+    length = score.shape[-1]
+    if length > 1 and score.stride(-1) != 1:
+        raise invalid(f"the last dimension of {name} must be contiguous")
+    groups = score.shape[:-1].numel()
+    return groups, length, group_stride(score, score.dim() - 1, name) if groups > 1 else length
+
+
+def _per_group(t, lead, name):
+    """Pointer of an int32 tensor with one value per group (None allowed)."""
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() != lead.numel():
+        raise invalid(f"{name} must be a contiguous int32 tensor with one value per group")
+    return t.data_ptr()
+
+
+def budget_accumulate(score, weights, out=None, decay: float = 1.0, lengths=None, row_lengths=None, stream=None):
+    """out[.., j] = decay * score[.., j] + sum over r of weights[.., r, j] for the entries in use; the others are
+    copied.  weights is score's leading shape + (rows, length), float32, float16 or bfloat16; row_lengths (int32,
+    one per group) leaves the rows behind it out.  out None: score is updated in place.  decay 0 starts anew."""
+    groups, length, stride = _score(score)
+    lead = score.shape[:-1]
+    if out is None:
+        out = score
+    elif out.shape != score.shape:
+        raise invalid("out must have score's shape")
+    device = score.device
+    on_device(device, weights=weights, out=out, lengths=lengths, row_lengths=row_lengths)
+    if weights.dim() != score.dim() + 1 or weights.shape[:-2] != lead or weights.shape[-1] != length:
+        raise invalid(f"weights must be {(*lead, 'rows', length)}, not {tuple(weights.shape)}")
+    rows = weights.shape[-2]
+    if length > 1 and weights.stride(-1) != 1:
+        raise invalid("the last dimension of weights must be contiguous")
+    below_2_31(groups=groups, rows=rows, length=length)
+    launch(lib().gsx_b200_budget_accumulate, device, stream, score.data_ptr(), stride, weights.data_ptr(),
+           type_code(weights, FLOAT_TYPES, "weights"), group_stride(weights, weights.dim() - 2, "weights"),
+           weights.stride(-2) if rows > 1 else length, groups, rows, length, _per_group(lengths, lead, "lengths"),
+           _per_group(row_lengths, lead, "row_lengths"), decay, out.data_ptr(), _score(out, "out")[2])
+    return out
+
+
+def budget_select(score, budget: int, lengths=None, first: int = 0, recent: int = 0, keep=None, kept=None, drop=None,
+                  stream=None):
+    """(keep, kept): per group the increasing list of the entries that stay within `budget` (the `first` first,
+    the `recent` last, and the largest scores of the others, ties to the lowest index; NaN is below every number)
+    and its length min(entries in use, budget).  keep is int32, leading shape + (at least min(budget, length),);
+    drop, where given, int32 of score's shape, receives the others.  Places behind the lists are left as they were."""
+    groups, length, stride = _score(score)
+    lead = score.shape[:-1]
+    below_2_31(groups=groups, length=length, budget=budget)
+    if first < 0 or recent < 0:
+        raise GsxError(OUT_OF_RANGE, "first and recent must not be negative")
+    if first + recent > budget:
+        raise invalid("first + recent must be at most budget")
+    device = score.device
+    on_device(device, lengths=lengths, keep=keep, kept=kept, drop=drop)
+    most = min(budget, length)
+    if keep is None:
+        keep = empty((*lead, most), torch.int32, device, stream)
+    elif keep.dtype != torch.int32 or not keep.is_contiguous() or keep.shape[:-1] != lead or keep.shape[-1] < most:
+        raise invalid(f"keep must be a contiguous int32 tensor of shape {(*lead, most)} or wider")
+    if kept is None:
+        kept = empty(lead, torch.int32, device, stream)
+    if drop is not None and (drop.dtype != torch.int32 or not drop.is_contiguous() or drop.shape != score.shape):
+        raise invalid("drop must be a contiguous int32 tensor of score's shape")
+    L = lib()
+    size = L.gsx_b200_budget_workspace_bytes(groups, length)
+    workspace = empty((size,), torch.uint8, device, stream) if size else None
+    launch(L.gsx_b200_budget_select, device, stream, score.data_ptr(), stride, groups, length,
+           _per_group(lengths, lead, "lengths"), first, recent, budget, keep.data_ptr(), keep.shape[-1],
+           _per_group(kept, lead, "kept"), None if drop is None else drop.data_ptr(), length,
+           None if workspace is None else workspace.data_ptr(), size)
+    return keep, kept
+
+
+def _field(f, t, lead, tail, side):
+    """One side of a gather field: checks the shape, gives (entries, (outer, inner, row) strides in bytes)."""
+    n = len(lead)
+    if t.dim() < n + 1 or t.shape[:n] != lead or t.shape[n + 1:] != tail:
+        raise invalid(f"{side} {f} must be {(*lead, 'entries', *tail)}, not {tuple(t.shape)}")
+    want = 1
+    for d in range(t.dim() - 1, n, -1):
+        if t.shape[d] > 1 and t.stride(d) != want:
+            raise invalid(f"the rows of {side} {f} must be contiguous")
+        want *= t.shape[d]
+    size = t.element_size()
+    return t.shape[n], [s * size for s in ([0] * (2 - n) + list(t.stride()[:n]))] + [t.stride(n) * size]
+
+
+def budget_gather(fields, keep, kept, bad=None, stream=None):
+    """Row r of dst = row keep[.., r] of src for r < kept[..], for every (src, dst) pair of `fields` (up to 32) in
+    one launch.  keep is [budget], [heads, budget] or [batch, heads, budget]; src is its leading shape + (length,) +
+    any row shape, dst the same with at least `budget` rows; both may be strided in all but the row, so a cache may
+    be a transposed view.  Rows of dst behind kept are left as they were."""
+    lead = keep.shape[:-1]
+    if keep.dim() < 1 or len(lead) > 2 or keep.dtype != torch.int32 or not keep.is_contiguous():
+        raise invalid("keep must be a contiguous int32 tensor of one to three dimensions")
+    if len(fields) > GATHER_MAX_FIELDS:
+        raise GsxError(OUT_OF_RANGE, f"at most {GATHER_MAX_FIELDS} fields")
+    device = keep.device
+    on_device(device, kept=kept, bad=bad)
+    budget = keep.shape[-1]
+    table = (GatherField * max(len(fields), 1))()
+    length = None
+    for f, (src, dst) in enumerate(fields):
+        on_device(device, src=src, dst=dst)
+        if src.dtype != dst.dtype:
+            raise GsxError(NOT_SUPPORTED, "src and dst must have the same type")
+        tail = src.shape[len(lead) + 1:]
+        entries, s = _field(f, src, lead, tail, "src")
+        room, d = _field(f, dst, lead, tail, "dst")
+        if length is None:
+            length = entries
+        if entries != length or room < budget:
+            raise invalid("every src must have the same number of entries, every dst at least keep's")
+        e = table[f]
+        e.src, e.dst = src.data_ptr(), dst.data_ptr()
+        e.row_bytes = tail.numel() * src.element_size()
+        e.src_outer_stride, e.src_inner_stride, e.src_row_stride = s
+        e.dst_outer_stride, e.dst_inner_stride, e.dst_row_stride = d
+    outer, inner = ([1] * (2 - len(lead)) + list(lead))
+    launch(lib().gsx_b200_budget_gather, device, stream, table, len(fields), outer, inner, length or 0, budget,
+           keep.data_ptr(), budget, _per_group(kept, lead, "kept"), word(bad, "bad"))

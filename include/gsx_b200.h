@@ -45,6 +45,8 @@ enum { GSX_B200_FORWARD_INFERENCE = 0, GSX_B200_FORWARD_TRAIN = 1 };
 
 /* element types (the values of gsx_data_type, gsx-core.h:8-14) */
 enum { GSX_B200_DATA_F32 = 0, GSX_B200_DATA_U8 = 8, GSX_B200_DATA_I32 = 12 };
+/* element types of the shared-row and budget calls only (GSX itself stores no such tensors) */
+enum { GSX_B200_DATA_F16 = 1, GSX_B200_DATA_BF16 = 2, GSX_B200_DATA_I64 = 13 };
 
 /* Pinhole camera: world->camera rotation (quaternion x, y, z, w) and translation, as
  * gsx_camera_pose (gsx-base.h:211-216) plus gsx_camera_intrinsics fx, fy, cx, cy, width, height. */
@@ -394,6 +396,79 @@ GSX_B200_API int gsx_b200_adc_select_keep(uint64_t n, const float *opacity, cons
                                           float opacity_threshold, float max_world_scale, float max_screen_scale,
                                           float scene_scale, uint8_t *flags, int32_t *keep, uint32_t *scratch,
                                           uint32_t *device_count, void *stream);
+
+/*
+ * Shared rows (no counterpart in the reference): a table whose rows many Gaussians share, with one row number
+ * per Gaussian, or any other embedding table.  Tables, outputs and gradients are f32, f16 or bf16 in any
+ * combination, indices i32 or i64; row strides are in elements and at least dim; rows, dim and count stay below
+ * 2^31.  An index outside [0, rows) sets *device_out_of_range to 1 (when non-NULL) and takes no part: its row of
+ * out stays untouched, its gradient is dropped.  Nothing waits, allocates or depends on values: the calls can be
+ * captured into a graph.
+ * gsx_b200_embedding_lookup: out[n] = scale * table[index[n]], computed in f32 and rounded once.
+ * gsx_b200_embedding_backward: grad_table[v] = scale * (sum of grad_out[n] over index[n] = v), written for every
+ * row (zero where no index names it), or added to it when accumulate != 0 (rows that no index names are then left
+ * as they are).  The positions are sorted by row first, so every sum runs in the order of n whatever the
+ * launch: the same inputs give the same bits.  Sums are f32, rounded once.  Indices equal to padding_row (-1: none)
+ * take no part.  workspace: gsx_b200_embedding_workspace_bytes(count, rows, dim) bytes of device memory, 16-byte
+ * aligned, of any content; calls that overlap on the GPU need one each.
+ */
+GSX_B200_API int gsx_b200_embedding_lookup(const void *table, int table_type, uint64_t rows, uint64_t dim,
+                                           uint64_t table_stride, const void *index, int index_type, uint64_t count,
+                                           float scale, void *out, int out_type, uint64_t out_stride,
+                                           uint32_t *device_out_of_range, void *stream);
+GSX_B200_API uint64_t gsx_b200_embedding_workspace_bytes(uint64_t count, uint64_t rows, uint64_t dim);
+GSX_B200_API int gsx_b200_embedding_backward(const void *grad_out, int grad_type, uint64_t grad_stride,
+                                             const void *index, int index_type, uint64_t count, float scale,
+                                             int64_t padding_row, void *grad_table, int table_type, uint64_t rows,
+                                             uint64_t dim, uint64_t table_stride, int accumulate, void *workspace,
+                                             uint64_t workspace_bytes, uint32_t *device_out_of_range, void *stream);
+
+/*
+ * Keeping entries within a budget by accumulated weight (no counterpart in the reference, whose density control
+ * prunes by opacity, scale and radius): the Gaussians of a scene by the blend weight they got over the views, or
+ * the rows of key-value caches by the attention weight they got.  `groups` independent sets of up to `length`
+ * entries (one set for a scene, one per batch entry and head for caches); lengths[g] (device, NULL: all `length`)
+ * is the number of entries of group g in use, taken as within [0, length]; entries behind it are never read.
+ * Strides are in elements; all counts stay below 2^31.  The calls can be captured into a graph.
+ * gsx_b200_budget_accumulate: out[g, j] = decay * score[g, j] + sum over r < row_lengths[g] (NULL: all `rows`) of
+ *   weights[g, r, j] for the entries in use (f32 sums in a fixed order); decay 0 does not read their scores.
+ *   Entries behind lengths[g] are copied from score.  out may be score itself, or must not overlap it; it must
+ *   not overlap weights.
+ * gsx_b200_budget_select: keep[g, 0 .. kept[g]) receives, in increasing order, the entries that stay: all of them
+ *   when the group uses at most `budget`, else the `first` first, the `recent` last, and of the others the
+ *   budget - first - recent with the largest scores, ties to the lowest index, NaN below every number, -0 equal
+ *   to +0.  kept[g] = min(entries in use, budget).  drop (may be NULL) receives the other entries, in increasing
+ *   order: those in use less kept[g].  Places of keep and drop behind the lists are left as they were.
+ *   workspace: gsx_b200_budget_workspace_bytes(groups, length) bytes of device memory, 4-byte aligned, of any
+ *   content (0 bytes for groups of up to 49152 entries); calls that overlap on the GPU need one each.
+ * gsx_b200_budget_gather: for every field and group, row r of dst = row keep[g, r] of src for r < kept[g]; later
+ *   rows of dst are left as they were.  All fields in ONE launch.  Group g is (g / inner, g % inner) in a field's
+ *   outer and inner strides (caches of [batch, head, entry] and [batch, entry, head] order alike).  A keep entry
+ *   outside [0, length) sets *device_out_of_range to 1 (when non-NULL) and leaves its row untouched.  No field's
+ *   dst may overlap any field's src.
+ */
+#define GSX_B200_GATHER_MAX_FIELDS 32
+typedef struct gsx_b200_gather_field {
+    const void *src;
+    void *dst;
+    uint64_t row_bytes; /* strides are in bytes */
+    uint64_t src_outer_stride, src_inner_stride, src_row_stride;
+    uint64_t dst_outer_stride, dst_inner_stride, dst_row_stride;
+} gsx_b200_gather_field;
+GSX_B200_API int gsx_b200_budget_accumulate(const float *score, uint64_t score_stride, const void *weights,
+                                            int weight_type, uint64_t group_stride, uint64_t row_stride,
+                                            uint64_t groups, uint64_t rows, uint64_t length, const int32_t *lengths,
+                                            const int32_t *row_lengths, float decay, float *out, uint64_t out_stride,
+                                            void *stream);
+GSX_B200_API uint64_t gsx_b200_budget_workspace_bytes(uint64_t groups, uint64_t length);
+GSX_B200_API int gsx_b200_budget_select(const float *score, uint64_t score_stride, uint64_t groups, uint64_t length,
+                                        const int32_t *lengths, uint64_t first, uint64_t recent, uint64_t budget,
+                                        int32_t *keep, uint64_t keep_stride, int32_t *kept, int32_t *drop,
+                                        uint64_t drop_stride, void *workspace, uint64_t workspace_bytes, void *stream);
+GSX_B200_API int gsx_b200_budget_gather(const gsx_b200_gather_field *fields, int32_t field_count, uint64_t outer,
+                                        uint64_t inner, uint64_t length, uint64_t budget, const int32_t *keep,
+                                        uint64_t keep_stride, const int32_t *kept, uint32_t *device_out_of_range,
+                                        void *stream);
 
 #ifdef __cplusplus
 }

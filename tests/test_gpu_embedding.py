@@ -1,0 +1,273 @@
+"""Shared-row lookup and its gradient against the formulas in 64 bits.
+
+Tolerances.  u = 2^-24 is the largest relative error of one f32 operation; a rounding to type t adds
+finfo(t).eps / 2 relative, or half a step of its smallest subnormal.  Lookup: one product, one rounding.  Gradient:
+any order of adding n terms is off by at most (n - 1) u sum|g| (to first order; 1.01 covers the rest), then one
+product, with accumulate one fused product and sum, and one rounding."""
+import pytest
+import torch
+
+import gsx_b200 as gb
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def _half_step(dtype, exact):
+    info = torch.finfo(dtype)
+    return (exact.abs() * (info.eps / 2)).clamp_min(info.tiny * info.eps / 2)
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _index(g, count, rows, dtype, skew=1.0):
+    u = torch.rand(count, generator=g, device="cuda", dtype=torch.float64).pow(skew)
+    return (u * rows).long().clamp_(max=rows - 1).to(dtype)
+
+
+def _check_lookup(out, table, index, scale):
+    want = table.double()[index.long()] * float(torch.tensor(scale, dtype=F32))
+    bound = 1.01 * (want.abs() * U + _half_step(out.dtype, want))
+    assert out.shape == want.shape
+    assert bool(((out.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("itype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("out_type", [F32, F16, BF16])
+@pytest.mark.parametrize("table_type", [F32, F16, BF16])
+def test_lookup_types(cuda_device, table_type, out_type, itype):
+    g = _gen(1)
+    for count, rows, dim in [(1, 1, 1), (1, 5, 4096), (7, 3, 8), (1000, 17, 3), (1001, 300, 45), (513, 1000, 128),
+                             (40, 2, 12)]:
+        table = torch.randn(rows, dim, generator=g, device="cuda").to(table_type)
+        index = _index(g, count, rows, itype)
+        _check_lookup(gb.embedding_lookup(table, index, out=torch.empty(count, dim, dtype=out_type, device="cuda"),
+                                          scale=1.7), table, index, 1.7)
+
+
+def test_lookup_large_takes_every_path(cuda_device):
+    g = _gen(2)
+    for count, rows, dim, dtype in [(400_003, 4096, 3, F32), (200_001, 1000, 45, BF16), (300_000, 64, 32, F16)]:
+        table = torch.randn(rows, dim, generator=g, device="cuda").to(dtype)
+        index = _index(g, count, rows, torch.int32, 2.0)
+        _check_lookup(gb.embedding_lookup(table, index, scale=0.25), table, index, 0.25)
+
+
+def test_lookup_index_shapes_and_empty_calls(cuda_device):
+    g = _gen(3)
+    table = torch.randn(11, 6, generator=g, device="cuda")
+    index = _index(g, 24, 11, torch.int64).view(2, 3, 4)
+    out = gb.embedding_lookup(table, index)
+    assert out.shape == (2, 3, 4, 6)
+    assert torch.equal(out, table[index])
+    assert gb.embedding_lookup(table, index[:0]).shape == (0, 3, 4, 6)
+    assert gb.embedding_lookup(table[:, :0], index).shape == (2, 3, 4, 0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_lookup_strided_and_unaligned(cuda_device, dtype):
+    g = _gen(4)
+    wide = torch.randn(50, 83, generator=g, device="cuda").to(dtype)
+    index = _index(g, 333, 50, torch.int32)
+    for table in (wide[:, :16], wide[:, 1:17], wide[:, 2:47], wide.view(-1)[1:1 + 48 * 8].view(48, 8)[:, :8]):
+        ix = index % table.shape[0]
+        buf = torch.full((333, 100), 9.0, dtype=dtype, device="cuda")
+        out = buf[:, 3:3 + table.shape[1]]
+        gb.embedding_lookup(table, ix, out=out, scale=2.0)
+        assert torch.equal(out, table[ix.long()] * 2.0)
+        assert bool((buf[:, :3] == 9.0).all()) and bool((buf[:, 3 + table.shape[1]:] == 9.0).all())
+
+
+@pytest.mark.parametrize("dim", [3, 8, 64])
+def test_lookup_out_of_range_rows_are_left_and_flagged(cuda_device, dim):
+    table = torch.randn(10, dim, device="cuda")
+    index = torch.tensor([3, -1, 9, 10, 2 ** 40, 0], device="cuda")
+    out = torch.full((6, dim), 5.0, device="cuda")
+    bad = torch.zeros(1, dtype=torch.int32, device="cuda")
+    gb.embedding_lookup(table, index[:1], out=out[:1], bad=bad)
+    assert int(bad) == 0
+    gb.embedding_lookup(table, index, out=out, bad=bad)
+    assert int(bad) == 1
+    assert bool((out[[1, 3, 4]] == 5.0).all())
+    assert torch.equal(out[[0, 2, 5]], table[[3, 9, 0]])
+
+
+def _check_gradient(got, grad, index, rows, scale, before=None, drop=None):
+    index = index.reshape(-1).long()
+    grad = grad.reshape(index.numel(), grad.shape[-1]).double()
+    use = (index >= 0) & (index < rows)
+    if drop is not None:
+        use &= index != drop
+    index, grad = index[use], grad[use]
+    s = float(torch.tensor(scale, dtype=F32))
+    want = torch.zeros(rows, grad.shape[1], dtype=torch.float64, device="cuda").index_add_(0, index, grad) * s
+    size = torch.zeros_like(want).index_add_(0, index, grad.abs()) * abs(s)
+    n = torch.bincount(index, minlength=rows).double()[:, None]
+    bound = size * (n + 1) * U
+    if before is not None:
+        want = want + before.double()
+        bound = bound + want.abs() * U
+    bound = 1.01 * (bound + _half_step(got.dtype, want.abs() + bound))
+    assert bool(((got.double() - want).abs() <= bound).all())
+    if before is None:
+        assert bool((got[(n == 0)[:, 0]] == 0).all())
+
+
+GRADIENT_SIZES = [(0, 5, 3), (1, 1, 1), (5, 1, 4), (100, 256, 8), (8192, 300, 7), (8193, 300, 7), (9000, 1, 3),
+                  (20_000, 4096, 3), (20_000, 4097, 4), (50_000, 70_000, 2), (33_333, 5000, 45), (300, 1000, 2048),
+                  (12_000, 3, 260), (2000, 50, 33)]
+
+
+@pytest.mark.parametrize("count,rows,dim", GRADIENT_SIZES)
+def test_gradient_sizes(cuda_device, count, rows, dim):
+    g = _gen(count + rows)
+    grad = torch.randn(count, dim, generator=g, device="cuda")
+    index = _index(g, count, rows, torch.int32, 2.0)
+    got = gb.embedding_backward(grad, index, torch.full((rows, dim), float("nan"), device="cuda"), scale=0.3)
+    _check_gradient(got, grad, index, rows, 0.3)
+    again = gb.embedding_backward(grad, index, torch.empty(rows, dim, device="cuda"), scale=0.3)
+    assert torch.equal(got, again)
+
+
+@pytest.mark.parametrize("itype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("table_type", [F32, F16, BF16])
+@pytest.mark.parametrize("grad_type", [F32, F16, BF16])
+def test_gradient_types(cuda_device, grad_type, table_type, itype):
+    g = _gen(5)
+    for count, rows, dim in [(700, 40, 64), (9001, 600, 5), (900, 30, 16)]:
+        grad = torch.randn(count, dim, generator=g, device="cuda").to(grad_type)
+        index = _index(g, count, rows, itype, 3.0)
+        got = gb.embedding_backward(grad, index, torch.empty(rows, dim, dtype=table_type, device="cuda"), scale=1.5)
+        _check_gradient(got, grad, index, rows, 1.5)
+        before = torch.randn(rows, dim, generator=g, device="cuda").to(table_type)
+        got = gb.embedding_backward(grad, index, before.clone(), scale=1.5, accumulate=True)
+        _check_gradient(got, grad, index, rows, 1.5, before=before)
+
+
+def test_gradient_three_digit_sort(cuda_device):
+    rows = 2 ** 24 + 5
+    g = _gen(6)
+    grad = torch.randn(9000, 1, generator=g, device="cuda")
+    index = _index(g, 9000, rows, torch.int64)
+    index[:4000] = index[4000:8000]
+    index[0], index[1] = rows - 1, 0
+    got = gb.embedding_backward(grad, index, torch.empty(rows, 1, device="cuda"))
+    _check_gradient(got, grad, index, rows, 1.0)
+
+
+@pytest.mark.parametrize("count", [3000, 40_000, 300_000])
+@pytest.mark.parametrize("dim", [3, 64, 300])
+def test_gradient_of_one_row_that_has_nearly_all(cuda_device, count, dim):
+    g = _gen(7)
+    grad = torch.randn(count, dim, generator=g, device="cuda")
+    index = torch.full((count,), 4, dtype=torch.int32, device="cuda")
+    index[::97] = _index(g, index[::97].numel(), 9, torch.int32)
+    got = gb.embedding_backward(grad, index, torch.empty(9, dim, device="cuda"))
+    _check_gradient(got, grad, index, 9, 1.0)
+
+
+@pytest.mark.parametrize("count,rows", [(500, 64), (500, 63), (30_000, 4096), (30_000, 9000)])
+def test_gradient_drops_padding_and_out_of_range(cuda_device, count, rows):
+    g = _gen(8)
+    grad = torch.randn(count, 6, generator=g, device="cuda")
+    index = _index(g, count, rows, torch.int64)
+    index[::5] = 7
+    index[3::11] = rows + 2
+    index[4::13] = -3
+    used = (index != 7) & (index >= 0) & (index < rows)
+    grad[~used] = float("nan")  # nothing of a dropped row may be seen
+    bad = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = gb.embedding_backward(grad, index, torch.empty(rows, 6, device="cuda"), padding_row=7, bad=bad)
+    assert int(bad) == 1
+    _check_gradient(got, grad, index, rows, 1.0, drop=7)
+    bad.zero_()
+    fine = torch.where(used, index, 7)
+    gb.embedding_backward(grad, fine, got, padding_row=7, bad=bad)
+    assert int(bad) == 0
+    _check_gradient(got, grad, fine, rows, 1.0, drop=7)
+    none = torch.full_like(index, 7)
+    assert bool((gb.embedding_backward(grad, none, got, padding_row=7) == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim", [8, 21, 600])
+def test_gradient_strided(cuda_device, dtype, dim):
+    g = _gen(9)
+    for offset in (0, 1):
+        wide = torch.randn(10_000, dim + 8, generator=g, device="cuda").to(dtype)
+        grad = wide[:, offset:offset + dim]
+        index = _index(g, 10_000, 77, torch.int32)
+        buf = torch.full((77, dim + 16), 3.0, dtype=dtype, device="cuda")
+        got = gb.embedding_backward(grad, index, buf[:, offset:offset + dim])
+        _check_gradient(got, grad, index, 77, 1.0)
+        rest = torch.cat([buf[:, :offset], buf[:, offset + dim:]], 1)
+        assert bool((rest == 3.0).all())
+
+
+def test_gradient_matches_differences_of_the_lookup(cuda_device):
+    """A loss sum(c * lookup(table)) is linear in the table: moving one element by 1 moves it by its gradient."""
+    g = _gen(10)
+    table = torch.randint(-8, 9, (13, 5), generator=g, device="cuda").float()
+    index = _index(g, 200, 13, torch.int32)
+    c = torch.randint(-4, 5, (200, 5), generator=g, device="cuda").float()  # whole numbers: every sum is exact
+    grad = gb.embedding_backward(c, index, torch.empty(13, 5, device="cuda"), scale=2.0)
+    loss = lambda t: float((c * gb.embedding_lookup(t, index, scale=2.0)).double().sum())  # noqa: E731
+    for v, k in [(0, 0), (5, 3), (12, 4)]:
+        moved = table.clone()
+        moved[v, k] += 1.0
+        assert loss(moved) - loss(table) == float(grad[v, k])
+
+
+def test_calls_on_another_stream_and_in_a_replayed_graph(cuda_device):
+    g = _gen(11)
+    table = torch.randn(500, 24, generator=g, device="cuda")
+    index = _index(g, 20_000, 500, torch.int32)
+    want_out = gb.embedding_lookup(table, index, scale=0.5)
+    want = gb.embedding_backward(want_out, index, torch.empty_like(table))
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    out = gb.embedding_lookup(table, index, scale=0.5, stream=side)
+    got = gb.embedding_backward(out, index, torch.empty_like(table), stream=side)
+    side.synchronize()
+    assert torch.equal(out, want_out) and torch.equal(got, want)
+    out, got = torch.zeros_like(out), torch.zeros_like(table)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gb.embedding_lookup(table, index, out=out, scale=0.5)
+        gb.embedding_backward(out, index, got)
+    gb.embedding_backward(want_out, index.flip(0).contiguous(), torch.empty_like(table))  # other work between
+    table.add_(1.0)
+    index.copy_(index.flip(0))
+    graph.replay()
+    torch.cuda.synchronize()
+    again = gb.embedding_lookup(table, index, scale=0.5)
+    assert torch.equal(out, again)
+    assert torch.equal(got, gb.embedding_backward(again, index, torch.empty_like(table)))
+
+
+def test_refusals(cuda_device):
+    table = torch.randn(10, 4, device="cuda")
+    index = torch.zeros(6, dtype=torch.int32, device="cuda")
+    grad = torch.zeros(6, 4, device="cuda")
+
+    def refused(code, f, *args, **kw):
+        with pytest.raises(gb.GsxError) as e:
+            f(*args, **kw)
+        assert e.value.code == code, e.value
+
+    refused(gb.INVALID_ARGUMENT, gb.embedding_lookup, table[0], index)
+    refused(gb.INVALID_ARGUMENT, gb.embedding_lookup, table, index.cpu())
+    refused(gb.INVALID_ARGUMENT, gb.embedding_lookup, table, index, out=torch.empty(6, 5, device="cuda"))
+    refused(gb.INVALID_ARGUMENT, gb.embedding_lookup, table.t(), index)
+    refused(gb.INVALID_ARGUMENT, gb.embedding_lookup, table, index.repeat(2)[::2])
+    refused(gb.NOT_SUPPORTED, gb.embedding_lookup, table.double(), index)
+    refused(gb.NOT_SUPPORTED, gb.embedding_lookup, table, index.to(torch.int16))
+    refused(gb.INVALID_ARGUMENT, gb.embedding_lookup, table, index, bad=torch.zeros(2, device="cuda"))
+    refused(gb.INVALID_ARGUMENT, gb.embedding_backward, grad[:5], index, table)
+    refused(gb.INVALID_ARGUMENT, gb.embedding_backward, grad[:1].expand(6, 4), index, table)
+    refused(gb.INVALID_ARGUMENT, gb.embedding_backward, grad, index, table[:1].expand(10, 4))
+    refused(gb.OUT_OF_RANGE, gb.embedding_backward, grad, index, table, padding_row=10)
+    refused(gb.NOT_SUPPORTED, gb.embedding_backward, grad.double(), index, table)
