@@ -30,17 +30,15 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kPiece = 512;
-constexpr int kWarpMax = 64;
 constexpr int kSmallThreads = 1024;
 constexpr int kSmallItems = 8;
-constexpr int kSmallCount = kSmallThreads * kSmallItems;
-constexpr int kSortThreads = 512;
-constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kMaxBits = 12;
+constexpr int kSmallCount = kSmallThreads * kSmallItems; /* positions that one CTA sorts */
+constexpr int kSortThreads = 1024;
+constexpr int kSortItems = 8;
+constexpr int kTile = kSortThreads * kSortItems; /* pairs that a CTA of the longer sort ranks at once */
+constexpr int kMaxBits = 8;
 constexpr int kMaxBins = 1 << kMaxBits;
-constexpr uint64_t kMaxChunk = 32768; /* a warp's counts of one digit fit 16 bits */
-constexpr int kChunks = 148;
+constexpr int kChunks = 148; /* CTAs of a pass: one an SM */
 
 /* ---- element types ---- */
 template <typename T>
@@ -194,19 +192,84 @@ void launch_lookup(const void *table_, uint64_t rows, uint64_t dim, uint64_t tab
 }
 
 /* ------------------------------------------------------------------------------------------ */
+/* rows of the gradient table */
+
+struct Table {
+    void *data;
+    uint64_t stride; /* elements */
+    uint64_t rows;
+    float scale;
+    int bytes; /* of an element */
+    bool accumulate;
+};
+
+template <typename TT, int VW>
+__device__ __forceinline__ void store_sums(const Table &t, uint64_t row, uint32_t c, const float (&sum)[VW])
+{
+    Pack<TT, VW> *to = reinterpret_cast<Pack<TT, VW> *>(static_cast<TT *>(t.data) + row * t.stride + c);
+    Pack<TT, VW> y;
+    if(t.accumulate) {
+        y = *to;
+#pragma unroll
+        for(int v = 0; v < VW; ++v) y.v[v] = from_f32<TT>(fmaf(t.scale, sum[v], to_f32(y.v[v])));
+    } else {
+#pragma unroll
+        for(int v = 0; v < VW; ++v) y.v[v] = from_f32<TT>(t.scale * sum[v]);
+    }
+    *to = y;
+}
+
+/* zeros in part `part` of `parts` of a table (16-byte stores where rows and addresses allow it) */
+__device__ __forceinline__ void zero_rows(const Table &t, uint32_t dim, uint32_t part, uint32_t parts)
+{
+    const uint64_t es = t.bytes;
+    uint64_t rows = t.rows, row = dim * es;
+    const uint64_t step = t.stride * es;
+    if(row == step) {
+        row *= rows;
+        rows = 1;
+    }
+    unsigned char *base = static_cast<unsigned char *>(t.data);
+    const uint64_t tid = (uint64_t)part * blockDim.x + threadIdx.x, threads = (uint64_t)parts * blockDim.x;
+    if(rows == 1) {
+        const uint64_t head = (16 - ((uintptr_t)base & 15)) & 15, first = head < row ? head : row;
+        const uint64_t vecs = (row - first) / 16;
+        uint4 *v = reinterpret_cast<uint4 *>(base + first);
+        for(uint64_t i = tid; i < vecs; i += threads) v[i] = make_uint4(0, 0, 0, 0);
+        uint16_t *h = reinterpret_cast<uint16_t *>(base);
+        if(tid < first / 2) h[tid] = 0;
+        const uint64_t done = first + vecs * 16;
+        if(tid < (row - done) / 2) h[done / 2 + tid] = 0;
+        return;
+    }
+    const uint64_t warp = tid / 32, warps = threads / 32;
+    const uint32_t lane = threadIdx.x & 31;
+    const bool wide = (((uintptr_t)base | row | step) & 15) == 0;
+    for(uint64_t r = warp; r < rows; r += warps) {
+        unsigned char *to = base + r * step;
+        if(wide)
+            for(uint64_t i = lane; i < row / 16; i += 32) reinterpret_cast<uint4 *>(to)[i] = make_uint4(0, 0, 0, 0);
+        else
+            for(uint64_t i = lane; i < row / 2; i += 32) reinterpret_cast<uint16_t *>(to)[i] = 0;
+    }
+}
+
+/* ------------------------------------------------------------------------------------------ */
 /* the sort of positions by row */
 
-/* row of position i, or -1 where it takes no part */
+/* Which positions take part: those whose index is a row and not the padding row (UINT32_MAX: none).  Any other index
+ * than the padding row sets *bad. */
+struct Use {
+    uint32_t rows, padding;
+    uint32_t *bad;
+};
+
 template <typename I>
-__device__ __forceinline__ int64_t row_of(const I *__restrict__ index, uint64_t i, uint64_t rows, int64_t padding,
-                                          uint32_t *bad)
+__device__ __forceinline__ bool takes_part(I s, const Use &use)
 {
-    const int64_t s = (int64_t)__ldg(index + i);
-    if(s < 0 || (uint64_t)s >= rows) {
-        if(bad != nullptr && s != padding) atomicExch(bad, 1u);
-        return -1;
-    }
-    return s == padding ? -1 : s;
+    const bool in = sizeof(I) == 4 ? (uint32_t)s < use.rows : (uint64_t)s < (uint64_t)use.rows;
+    if(!in && use.bad != nullptr) atomicExch(use.bad, 1u);
+    return in && (uint32_t)s != use.padding;
 }
 
 /* block-wide inclusive scan of one value per thread; s_warp holds one word per warp */
@@ -221,621 +284,573 @@ __device__ __forceinline__ uint32_t block_inclusive_scan(uint32_t v, uint32_t *s
     __syncthreads();
     if(lane == 31) s_warp[warp] = v;
     __syncthreads();
-    uint32_t before = 0, sum = 0;
-    for(int w = 0; w < warps; ++w) {
-        const uint32_t s = s_warp[w];
-        before += w < warp ? s : 0u;
-        sum += s;
+    const uint32_t mine = lane < warps ? s_warp[lane] : 0u;
+    uint32_t incl = mine;
+#pragma unroll
+    for(int d = 1; d < 32; d <<= 1) {
+        const uint32_t t = __shfl_up_sync(0xffffffffu, incl, d);
+        if(lane >= d) incl += t;
     }
-    if(total) *total = sum;
-    return before + v;
+    if(total) *total = __shfl_sync(0xffffffffu, incl, 31);
+    return v + __shfl_sync(0xffffffffu, incl - mine, warp);
 }
 
-/* all of a small sort in one CTA: keys (rows, ascending) and positions; *n_sorted = positions that take part */
+/* A tile of (row, position) pairs that a CTA ranks by one digit of at most 8 bits. */
+template <int THREADS, int ITEMS>
+struct SortShared {
+    uint2 pair[THREADS * ITEMS];
+    uint32_t hist[THREADS / 32][kMaxBins];
+    uint32_t before[kMaxBins]; /* of a digit: the tile's pairs with smaller ones */
+    uint32_t warp[32];
+};
+
+/* Ranks the tile's pairs (warp w holds elements 32 * items * w + 32 * it + lane) by digit, stable in element
+ * order, and leaves them in s.pair in that order.  Elements with valid[it] false are dropped.  Returns, for threads
+ * below the number of digits, how many pairs have that digit.  Lanes with equal digits find one another by one
+ * ballot per digit bit: __match_any_sync takes a step per distinct value on this GPU (a tile of 8192 ranked in 12 us
+ * with it, in 4 us with ballots). */
+template <int THREADS, int ITEMS>
+__device__ __forceinline__ uint32_t sort_tile(SortShared<THREADS, ITEMS> &s, const uint32_t (&key)[ITEMS],
+                                              const uint32_t (&pos)[ITEMS], const bool (&valid)[ITEMS], int items, int shift,
+                                              int bits)
+{
+    constexpr int WARPS = THREADS / 32;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t bins = 1u << bits, mask = bins - 1u;
+    for(uint32_t j = threadIdx.x; j < WARPS * bins; j += THREADS) s.hist[j >> bits][j & mask] = 0u;
+    __syncthreads();
+    uint32_t *wh = s.hist[warp];
+    uint32_t rank[ITEMS];
+#pragma unroll
+    for(int it = 0; it < ITEMS; ++it) {
+        if(it < items) {
+            const uint32_t d = key[it] >> shift & mask;
+            unsigned peers = __ballot_sync(0xffffffffu, valid[it]);
+#pragma unroll
+            for(int b = 0; b < kMaxBits; ++b) {
+                if(b < bits) {
+                    const int one = -(int)(d >> b & 1u); /* all ones where the bit is set */
+                    peers &= ~(__ballot_sync(0xffffffffu, one != 0) ^ (unsigned)one);
+                }
+            }
+            const unsigned lt = peers & ((1u << lane) - 1u);
+            uint32_t before = 0;
+            if(valid[it]) before = wh[d];
+            rank[it] = before + (uint32_t)__popc(lt);
+            __syncwarp();
+            if(valid[it] && lt == 0u) wh[d] = before + (uint32_t)__popc(peers);
+            __syncwarp();
+        }
+    }
+    __syncthreads();
+    uint32_t count = 0;
+    if(threadIdx.x < bins) {
+        uint32_t c[WARPS];
+#pragma unroll
+        for(int w = 0; w < WARPS; ++w) c[w] = s.hist[w][threadIdx.x];
+#pragma unroll
+        for(int w = 0; w < WARPS; ++w) {
+            s.hist[w][threadIdx.x] = count;
+            count += c[w];
+        }
+    }
+    const uint32_t upto = block_inclusive_scan(count, s.warp, nullptr);
+    if(threadIdx.x < bins) s.before[threadIdx.x] = upto - count;
+    __syncthreads();
+#pragma unroll
+    for(int it = 0; it < ITEMS; ++it)
+        if(it < items && valid[it]) {
+            const uint32_t d = key[it] >> shift & mask;
+            s.pair[s.before[d] + wh[d] + rank[it]] = make_uint2(key[it], pos[it]);
+        }
+    __syncthreads();
+    return count;
+}
+
+/* all of a small sort in one CTA */
 template <typename I>
 __global__ void __launch_bounds__(kSmallThreads) small_sort_kernel(const I *__restrict__ index, uint32_t count,
-                                                                   uint64_t rows, int64_t padding,
-                                                                   uint32_t *__restrict__ keys,
-                                                                   uint32_t *__restrict__ pos,
-                                                                   uint32_t *__restrict__ n_sorted,
-                                                                   uint32_t *__restrict__ bad)
+                                                                   const Use use, uint2 *__restrict__ pairs,
+                                                                   uint32_t *__restrict__ n_sorted)
 {
     extern __shared__ __align__(16) unsigned char smem[];
-    uint32_t *s_key = reinterpret_cast<uint32_t *>(smem);         /* kSmallCount */
-    uint32_t *s_pos = s_key + kSmallCount;                        /* kSmallCount */
-    uint32_t *s_hist = s_pos + kSmallCount;                       /* 32 warps * 256 */
-    uint32_t *s_warp = s_hist + 32 * 256;                         /* 32 */
+    auto &s = *reinterpret_cast<SortShared<kSmallThreads, kSmallItems> *>(smem);
+    gsx_pdl_trigger(); /* the zeros are written meanwhile */
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int items = (int)((count + kSmallThreads - 1) / kSmallThreads);
     const uint32_t wbase = (uint32_t)warp * 32u * (uint32_t)items + (uint32_t)lane;
-    uint32_t k[kSmallItems], p[kSmallItems], rank[kSmallItems];
-    uint32_t dropped = 0;
+    uint32_t k[kSmallItems], p[kSmallItems], used = 0;
+    bool valid[kSmallItems];
+    I raw[kSmallItems];
 #pragma unroll
     for(int it = 0; it < kSmallItems; ++it) {
-        k[it] = 0xffffffffu; /* after every row in each digit: behind the count, never written */
         p[it] = wbase + (uint32_t)it * 32u;
-        if(it < items && p[it] < count) {
-            const int64_t r = row_of(index, p[it], rows, padding, bad);
-            if(r >= 0) k[it] = (uint32_t)r;
-            else ++dropped;
-        }
-    }
-    uint32_t all_dropped;
-    block_inclusive_scan(dropped, s_warp, &all_dropped);
-    if(threadIdx.x == 0) *n_sorted = count - all_dropped;
-    /* the top digit's bits; dropped positions need a value above the last row */
-    const int bits = 32 - __clz((uint32_t)(all_dropped ? rows : rows - 1));
-    const int passes = bits == 0 ? 0 : (bits + 7) / 8;
-    for(int pass = 0; pass < passes; ++pass) {
-        const int shift = 8 * pass;
-        for(int j = threadIdx.x; j < 32 * 256; j += kSmallThreads) s_hist[j] = 0u;
-        __syncthreads();
-        uint32_t *wh = s_hist + warp * 256;
-#pragma unroll
-        for(int it = 0; it < kSmallItems; ++it) {
-            if(it < items) {
-                const uint32_t d = (k[it] >> shift) & 255u;
-                const unsigned peers = __match_any_sync(0xffffffffu, d);
-                const int leader = __ffs(peers) - 1;
-                uint32_t base = 0;
-                if(lane == leader) {
-                    base = wh[d];
-                    wh[d] = base + (uint32_t)__popc(peers);
-                }
-                base = __shfl_sync(0xffffffffu, base, leader);
-                rank[it] = base + (uint32_t)__popc(peers & ((1u << lane) - 1u));
-                __syncwarp();
-            }
-        }
-        __syncthreads();
-        uint32_t sum = 0;
-        if(threadIdx.x < 256) {
-#pragma unroll
-            for(int w = 0; w < 32; ++w) {
-                const uint32_t c = s_hist[w * 256 + threadIdx.x];
-                s_hist[w * 256 + threadIdx.x] = sum;
-                sum += c;
-            }
-        }
-        const uint32_t before = block_inclusive_scan(sum, s_warp, nullptr) - sum;
-        if(threadIdx.x < 256) {
-#pragma unroll
-            for(int w = 0; w < 32; ++w) s_hist[w * 256 + threadIdx.x] += before;
-        }
-        __syncthreads();
-#pragma unroll
-        for(int it = 0; it < kSmallItems; ++it) {
-            if(it < items) {
-                const uint32_t to = wh[(k[it] >> shift) & 255u] + rank[it];
-                s_key[to] = k[it];
-                s_pos[to] = p[it];
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for(int it = 0; it < kSmallItems; ++it) {
-            if(it < items) {
-                k[it] = s_key[wbase + (uint32_t)it * 32u];
-                p[it] = s_pos[wbase + (uint32_t)it * 32u];
-            }
-        }
-        __syncthreads();
+        raw[it] = it < items && p[it] < count ? __ldg(index + p[it]) : (I)0;
     }
 #pragma unroll
     for(int it = 0; it < kSmallItems; ++it) {
-        const uint32_t i = wbase + (uint32_t)it * 32u;
-        if(it < items && i < count - all_dropped) {
-            keys[i] = k[it];
-            pos[i] = p[it];
-        }
+        k[it] = (uint32_t)raw[it];
+        valid[it] = it < items && p[it] < count && takes_part(raw[it], use);
+        used += valid[it];
     }
+    uint32_t n;
+    block_inclusive_scan(used, s.warp, &n);
+    if(threadIdx.x == 0) *n_sorted = n;
+    const int bits = use.rows > 1 ? 32 - __clz((int)(use.rows - 1)) : 1;
+    const int passes = (bits + kMaxBits - 1) / kMaxBits;
+    for(int pass = 0, shift = 0; pass < passes; ++pass) {
+        const int width = (bits - shift + passes - 1 - pass) / (passes - pass);
+        sort_tile(s, k, p, valid, items, shift, width);
+        shift += width;
+#pragma unroll
+        for(int it = 0; it < kSmallItems; ++it) {
+            const uint32_t i = wbase + (uint32_t)it * 32u;
+            valid[it] = it < items && i < n;
+            if(valid[it]) {
+                k[it] = s.pair[i].x;
+                p[it] = s.pair[i].y;
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for(int it = 0; it < kSmallItems; ++it)
+        if(valid[it]) pairs[wbase + (uint32_t)it * 32u] = make_uint2(k[it], p[it]);
 }
 
-/* The part of a pass's input that chunk c of `chunks` covers: whole warps' shares of 32 positions. */
-__device__ __forceinline__ void chunk_range(uint64_t n, uint32_t chunks, uint32_t c, uint64_t &begin, uint64_t &end)
+/* the table's zeros, beside small_sort_kernel; the last CTA ends after that */
+__global__ void __launch_bounds__(kThreads) zero_kernel(const Table table, uint32_t dim)
 {
-    uint64_t len = (n + chunks - 1) / chunks;
-    len = (len + kSortThreads - 1) / kSortThreads * kSortThreads;
-    begin = (uint64_t)c * len < n ? (uint64_t)c * len : n;
-    end = begin + len < n ? begin + len : n;
+    gsx_pdl_trigger();
+    zero_rows(table, dim, blockIdx.x, gridDim.x);
+    if(blockIdx.x == gridDim.x - 1) gsx_pdl_wait();
 }
 
-/* One digit of element i: of the index itself in the first pass (kFirst), of the pass's input pairs else.
- * Returns the digit, or -1 where the position takes no part. */
+/* The kernels from here on are launched before the one ahead of them has ended (gsx_launch_pdl) and read what it wrote
+ * after gsx_pdl_wait: with __ldcg, since a read-only load may return what the SM's cache held before. */
+
+/* the part of a pass's input that belongs to this CTA */
+__device__ __forceinline__ void chunk_range(uint32_t n, uint32_t &begin, uint32_t &end)
+{
+    const uint32_t len = (n + gridDim.x - 1) / gridDim.x;
+    begin = len * blockIdx.x < n ? len * blockIdx.x : n;
+    end = n - begin < len ? n : begin + len;
+}
+
+/* Up to kSortItems elements of a pass's input, at first + it * step below end: of the indices themselves in the
+ * first pass (kFirst), of sorted pairs else.  All loads are issued before the first is looked at. */
 template <typename I, bool kFirst>
-__device__ __forceinline__ int digit_at(const I *__restrict__ index, const uint2 *__restrict__ pairs, uint64_t i,
-                                        uint64_t rows, int64_t padding, uint32_t *bad, int shift, uint32_t mask,
-                                        uint32_t &key, uint32_t &p)
+__device__ __forceinline__ void load_elements(const I *__restrict__ index, const uint2 *__restrict__ pairs, uint32_t first,
+                                              uint32_t step, int items, uint32_t end, const Use &use,
+                                              uint32_t (&key)[kSortItems], uint32_t (&pos)[kSortItems],
+                                              bool (&valid)[kSortItems])
 {
     if(kFirst) {
-        const int64_t r = row_of(index, i, rows, padding, bad);
-        if(r < 0) return -1;
-        key = (uint32_t)r;
-        p = (uint32_t)i;
-    } else {
-        const uint2 kp = __ldg(pairs + i);
-        key = kp.x;
-        p = kp.y;
+        I raw[kSortItems];
+#pragma unroll
+        for(int it = 0; it < kSortItems; ++it) {
+            pos[it] = first + it * step;
+            valid[it] = it < items && pos[it] < end;
+            raw[it] = valid[it] ? __ldg(index + pos[it]) : (I)0;
+        }
+#pragma unroll
+        for(int it = 0; it < kSortItems; ++it) {
+            key[it] = (uint32_t)raw[it];
+            valid[it] = valid[it] && takes_part(raw[it], use);
+        }
+        return;
     }
-    return (int)((key >> shift) & mask);
+#pragma unroll
+    for(int it = 0; it < kSortItems; ++it) {
+        const uint32_t i = first + it * step;
+        valid[it] = it < items && i < end;
+        const uint2 kp = valid[it] ? __ldcg(pairs + i) : make_uint2(0u, 0u);
+        key[it] = kp.x;
+        pos[it] = kp.y;
+    }
 }
 
-/* digit counts of every chunk, and of all (totals, cleared by the caller) */
+/* counts[c][d] = elements of chunk c with digit d; the first pass also writes the table's zeros */
 template <typename I, bool kFirst>
 __global__ void __launch_bounds__(kSortThreads) digit_count_kernel(const I *__restrict__ index,
-                                                                   const uint2 *__restrict__ pairs, uint64_t count,
-                                                                   const uint32_t *__restrict__ n_pairs, uint64_t rows,
-                                                                   int64_t padding, int shift, int bits,
-                                                                   uint32_t *__restrict__ counts,
-                                                                   uint32_t *__restrict__ totals,
-                                                                   uint32_t *__restrict__ bad)
+                                                                   const uint2 *__restrict__ pairs, uint32_t count,
+                                                                   const uint32_t *__restrict__ n_pairs, const Use use,
+                                                                   int shift, int bits, uint32_t *__restrict__ counts,
+                                                                   const Table table, uint32_t dim)
 {
     __shared__ uint32_t s_hist[kMaxBins];
-    const int bins = 1 << bits;
-    for(int j = threadIdx.x; j < bins; j += kSortThreads) s_hist[j] = 0u;
+    const uint32_t bins = 1u << bits;
+    for(uint32_t j = threadIdx.x; j < bins; j += kSortThreads) s_hist[j] = 0u;
     __syncthreads();
-    uint64_t begin, end;
-    chunk_range(kFirst ? count : (uint64_t)*n_pairs, gridDim.x, blockIdx.x, begin, end);
-    for(uint64_t i = begin + threadIdx.x; i < end; i += kSortThreads) {
-        uint32_t key, p;
-        const int d = digit_at<I, kFirst>(index, pairs, i, rows, padding, bad, shift, (uint32_t)bins - 1u, key, p);
-        if(d >= 0) atomicAdd(&s_hist[d], 1u);
-    }
-    __syncthreads();
-    for(int j = threadIdx.x; j < bins; j += kSortThreads) {
-        const uint32_t v = s_hist[j];
-        counts[(uint64_t)blockIdx.x * bins + j] = v;
-        if(v) atomicAdd(&totals[j], v);
-    }
-}
-
-/* counts[c][d] -> first output place of chunk c's digit d; starts[d] = first place of digit d (starts[bins] = all).
- * A CTA owns 32 digits: 32 x 32 threads, each adding up a 32nd of the chunks. */
-__global__ void __launch_bounds__(1024) digit_scan_kernel(uint32_t *__restrict__ counts, uint32_t chunks, int bins,
-                                                          const uint32_t *__restrict__ totals,
-                                                          uint32_t *__restrict__ starts, uint32_t *__restrict__ n_sorted)
-{
-    __shared__ uint32_t s_part[32][33];
-    __shared__ uint32_t s_warp[32];
-    __shared__ uint32_t s_base[32];
-    const int dl = threadIdx.x & 31, cl = threadIdx.x >> 5;
-    const int d0 = blockIdx.x * 32, d = d0 + dl;
-    /* everything before this CTA's digits */
-    uint32_t before = 0;
-    for(int j = threadIdx.x; j < d0; j += 1024) before += totals[j];
-    uint32_t base;
-    block_inclusive_scan(before, s_warp, &base);
-    const uint32_t per = (chunks + 31) / 32;
-    const uint32_t c0 = (uint32_t)cl * per, c1 = c0 + per < chunks ? c0 + per : chunks;
-    uint32_t sum = 0;
-    if(d < bins)
-        for(uint32_t c = c0; c < c1; ++c) sum += counts[(uint64_t)c * bins + d];
-    s_part[cl][dl] = sum;
-    if(cl == 0) {
-        const uint32_t t = d < bins ? totals[d] : 0u;
-        uint32_t v = t;
+    gsx_pdl_trigger();
+    if(!kFirst) gsx_pdl_wait();
+    uint32_t begin, end;
+    chunk_range(kFirst ? count : __ldcg(n_pairs), begin, end);
+    for(uint32_t i0 = begin; i0 < end; i0 += kTile) {
+        uint32_t key[kSortItems], pos[kSortItems];
+        bool in[kSortItems];
+        load_elements<I, kFirst>(index, pairs, i0 + threadIdx.x, kSortThreads, kSortItems, end, use, key, pos, in);
 #pragma unroll
-        for(int o = 1; o < 32; o <<= 1) {
-            const uint32_t u = __shfl_up_sync(0xffffffffu, v, o);
-            if(dl >= o) v += u;
-        }
-        s_base[dl] = base + v - t;
-        if(d < bins) starts[d] = base + v - t;
-        if(d == bins - 1) {
-            starts[bins] = base + v;
-            *n_sorted = base + v;
-        }
+        for(int it = 0; it < kSortItems; ++it)
+            if(in[it]) atomicAdd(&s_hist[key[it] >> shift & (bins - 1u)], 1u);
     }
     __syncthreads();
-    uint32_t run = s_base[dl];
-    for(int w = 0; w < cl; ++w) run += s_part[w][dl];
-    if(d < bins)
-        for(uint32_t c = c0; c < c1; ++c) {
-            const uint32_t v = counts[(uint64_t)c * bins + d];
-            counts[(uint64_t)c * bins + d] = run;
-            run += v;
-        }
+    for(uint32_t j = threadIdx.x; j < bins; j += kSortThreads) counts[blockIdx.x * bins + j] = s_hist[j];
+    if(kFirst && !table.accumulate) zero_rows(table, dim, blockIdx.x, gridDim.x);
 }
 
-/* each element to its place, in input order within a digit.  kLast writes positions (and keys, where the caller
- * needs them), the other passes write (key, position) pairs.  Shared memory: a 16-bit count of every digit for
- * each warp, which becomes the warp's next place within the chunk's run, and the chunk's first places. */
-template <typename I, bool kFirst, bool kLast>
-__global__ void __launch_bounds__(kSortThreads) digit_scatter_kernel(
-    const I *__restrict__ index, const uint2 *__restrict__ pairs, uint64_t count, const uint32_t *__restrict__ n_pairs,
-    uint64_t rows, int64_t padding, int shift, int bits, const uint32_t *__restrict__ places, uint2 *__restrict__ pairs_out,
-    uint32_t *__restrict__ keys_out, uint32_t *__restrict__ pos_out)
+/* every pair to its place, in input order within a digit.  Each CTA adds up the counts of all chunks itself. */
+template <typename I, bool kFirst>
+__global__ void __launch_bounds__(kSortThreads) digit_scatter_kernel(const I *__restrict__ index,
+                                                                        const uint2 *__restrict__ pairs, uint32_t count,
+                                                                        uint32_t *n_pairs, const Use use, int shift,
+                                                                        int bits, const uint32_t *__restrict__ counts,
+                                                                        uint2 *__restrict__ out)
 {
     extern __shared__ __align__(16) unsigned char smem[];
-    const int bins = 1 << bits;
-    const int words = bins > 1 ? bins / 2 : 1;                            /* two counts a word */
-    uint32_t *s_place = reinterpret_cast<uint32_t *>(smem);               /* bins */
-    uint32_t *s_count = s_place + bins;                                   /* kSortWarps * words */
+    auto &s = *reinterpret_cast<SortShared<kSortThreads, kSortItems> *>(smem);
+    __shared__ uint32_t s_place[kMaxBins]; /* of a digit: the next output place */
+    __shared__ uint32_t s_to[kMaxBins];    /* .. less the place of its first pair in the tile */
+    __shared__ uint32_t s_n;
+    const uint32_t bins = 1u << bits, mask = bins - 1u;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for(int j = threadIdx.x; j < kSortWarps * words; j += kSortThreads) s_count[j] = 0u;
-    for(int j = threadIdx.x; j < bins; j += kSortThreads) s_place[j] = places[(uint64_t)blockIdx.x * bins + j];
-    __syncthreads();
-    uint64_t begin, end;
-    chunk_range(kFirst ? count : (uint64_t)*n_pairs, gridDim.x, blockIdx.x, begin, end);
-    const uint64_t share = (end - begin + kSortThreads - 1) / kSortThreads * 32;
-    const uint64_t w0 = begin + share * warp < end ? begin + share * warp : end;
-    const uint64_t w1 = w0 + share < end ? w0 + share : end;
-    uint32_t *mine = s_count + warp * words;
-    uint16_t *mine16 = reinterpret_cast<uint16_t *>(mine);
-    for(uint64_t i = w0 + lane; i < w1; i += 32) {
-        uint32_t key, p;
-        const int d = digit_at<I, kFirst>(index, pairs, i, rows, padding, nullptr, shift, (uint32_t)bins - 1u, key, p);
-        if(d >= 0) atomicAdd(&mine[d >> 1], 1u << (16 * (d & 1)));
-    }
-    __syncthreads();
-    /* counts -> exclusive prefix over the warps, both halves of a word at once (no half exceeds kMaxChunk) */
-    for(int j = threadIdx.x; j < words; j += kSortThreads) {
-        uint32_t run = 0;
-#pragma unroll
-        for(int w = 0; w < kSortWarps; ++w) {
-            const uint32_t v = s_count[w * words + j];
-            s_count[w * words + j] = run;
-            run += v;
+    gsx_pdl_trigger();
+    gsx_pdl_wait();
+    {
+        const uint32_t d = threadIdx.x & mask, parts = kSortThreads >> bits;
+        uint32_t all = 0, before = 0;
+#pragma unroll 16
+        for(uint32_t c = threadIdx.x >> bits; c < gridDim.x; c += parts) {
+            const uint32_t v = __ldcg(counts + (c * bins + d));
+            all += v;
+            before += c < blockIdx.x ? v : 0u;
         }
-    }
-    __syncthreads();
-    for(uint64_t i0 = w0; i0 < w1; i0 += 32) {
-        const uint64_t i = i0 + lane;
-        uint32_t key = 0, p = 0;
-        int d = -1;
-        if(i < w1) d = digit_at<I, kFirst>(index, pairs, i, rows, padding, nullptr, shift, (uint32_t)bins - 1u, key, p);
-        const unsigned peers = __match_any_sync(0xffffffffu, d);
-        const int leader = __ffs(peers) - 1;
-        uint32_t base = 0;
-        if(lane == leader && d >= 0) {
-            base = mine16[d];
-            mine16[d] = (uint16_t)(base + (uint32_t)__popc(peers));
-        }
-        base = __shfl_sync(0xffffffffu, base, leader);
-        __syncwarp();
-        if(d >= 0) {
-            const uint32_t to = s_place[d] + base + (uint32_t)__popc(peers & ((1u << lane) - 1u));
-            if(kLast) {
-                pos_out[to] = p;
-                if(keys_out != nullptr) keys_out[to] = key;
-            } else {
-                pairs_out[to] = make_uint2(key, p);
+        uint32_t *s_all = &s.hist[0][0], *s_before = s_all + kSortThreads;
+        s_all[threadIdx.x] = all;
+        s_before[threadIdx.x] = before;
+        __syncthreads();
+        all = before = 0;
+        if(threadIdx.x < bins)
+            for(uint32_t q = 0; q < parts; ++q) {
+                all += s_all[(q << bits) + d];
+                before += s_before[(q << bits) + d];
             }
+        uint32_t n;
+        const uint32_t smaller = block_inclusive_scan(all, s.warp, &n) - all;
+        if(threadIdx.x < bins) s_place[threadIdx.x] = smaller + before;
+        if(kFirst && blockIdx.x == 0 && threadIdx.x == 0) *n_pairs = n;
+        __syncthreads();
+    }
+    uint32_t begin, end;
+    chunk_range(kFirst ? count : __ldcg(n_pairs), begin, end);
+    for(uint32_t i0 = begin; i0 < end; i0 += kTile) {
+        const int items = end - i0 >= (uint32_t)kTile ? kSortItems : (int)((end - i0 + kSortThreads - 1) / kSortThreads);
+        uint32_t k[kSortItems], p[kSortItems];
+        bool valid[kSortItems];
+        load_elements<I, kFirst>(index, pairs, i0 + (uint32_t)(warp * 32 * items + lane), 32, items, end, use, k, p, valid);
+        const uint32_t c = sort_tile(s, k, p, valid, items, shift, bits);
+        if(threadIdx.x < bins) {
+            s_to[threadIdx.x] = s_place[threadIdx.x] - s.before[threadIdx.x];
+            s_place[threadIdx.x] += c;
+            if(threadIdx.x == bins - 1) s_n = s.before[threadIdx.x] + c;
         }
+        __syncthreads();
+        const uint32_t n = s_n;
+        for(uint32_t j = threadIdx.x; j < n; j += kSortThreads) {
+            const uint2 kp = s.pair[j];
+            out[s_to[kp.x >> shift & mask] + j] = kp;
+        }
+        __syncthreads();
     }
 }
 
 /* ------------------------------------------------------------------------------------------ */
-/* sums by row */
+/* sums of sorted positions by row
+ *
+ * A CTA owns R consecutive sorted positions.  A group of 2^clog lanes, each with NR packs of VW columns, walks a run
+ * of C of them in order, with the rows of the next positions in flight, and stores a row whenever the row number
+ * changes.  A row that runs across groups is put together in shared memory (H: what a group has of a row that began
+ * before it, T: of one that goes on after it), one that runs across CTAs in row_join_kernel. */
 
-/* What the sums read: the sorted positions, and where each row's begin: starts[v] where the sort gives them
- * (tables of one pass), else the sorted keys, searched. */
-struct Sorted {
-    const uint32_t *pos;
-    const uint32_t *keys;
-    const uint32_t *starts;
+constexpr uint32_t kHead = 1, kWhole = 2, kTail = 4;
+constexpr int kMaxRun = 128;
+constexpr uint32_t kMaxPositions = 5120; /* of a CTA */
+
+struct Runs {
+    const uint2 *pairs;
     const uint32_t *n_sorted;
-    uint64_t rows;
+    float *head, *tail; /* [CTAs][dim]: sums of the CTA's first / last row where that crosses its ends */
+    uint32_t dim;
+    int clog, run; /* lanes of a group, positions of a group */
 };
 
-/* first place whose key is at least `row` */
-__device__ __forceinline__ uint32_t first_of(const Sorted &s, uint32_t n, uint64_t row)
+template <typename GT, typename TT, int VW, int NR>
+__global__ void __launch_bounds__(kThreads, NR * VW <= 8 ? 4 : 2) run_sum_kernel(const GT *__restrict__ grad, uint32_t stride_bytes, const Runs a,
+                                                              const Table table)
 {
-    if(row >= s.rows) return n;
-    if(s.starts != nullptr) return __ldg(s.starts + row);
-    uint32_t lo = 0, len = n;
-    while(len > 0) {
-        const uint32_t half = len / 2;
-        if((uint64_t)__ldg(s.keys + lo + half) < row) {
-            lo += half + 1;
-            len -= half + 1;
-        } else {
-            len = half;
-        }
+    constexpr int kRegs = NR * VW * (int)sizeof(GT) / 4 > 0 ? NR * VW * (int)sizeof(GT) / 4 : 1;
+    constexpr int U = kRegs <= 3 ? 8 : kRegs <= 8 ? 4 : 2; /* a divisor of 8, as runs are multiples of 8 */
+    extern __shared__ __align__(16) unsigned char smem[];
+    float *s_head = reinterpret_cast<float *>(smem);      /* groups * (NR * VW << clog) */
+    float *s_tail = s_head + kThreads * NR * VW;
+    /* each group's run and the pair behind it: an odd number of pairs, so that the groups of a warp read other banks */
+    uint2 *s_pair = reinterpret_cast<uint2 *>(s_tail + kThreads * NR * VW);
+    __shared__ uint32_t s_flags[kThreads / 4];
+    __shared__ uint8_t s_ends[kMaxPositions / 8]; /* bit j: position j is the last of its row */
+    gsx_pdl_trigger();
+    gsx_pdl_wait();
+    const uint32_t n = __ldcg(a.n_sorted);
+    const int cl = 1 << a.clog, groups = kThreads >> a.clog, run = a.run;
+    const uint32_t b0 = blockIdx.x * (uint32_t)(groups * run);
+    if(b0 >= n) return;
+    const uint32_t len = n - b0 < (uint32_t)(groups * run) ? n - b0 : (uint32_t)(groups * run);
+    for(int j = threadIdx.x; j < groups * (run + 1); j += kThreads) {
+        const uint32_t at = b0 + (uint32_t)(j - j / (run + 1));
+        s_pair[j] = at < n ? __ldcg(a.pairs + at) : make_uint2(0xffffffffu, 0u); /* no row */
     }
-    return lo;
-}
-
-/* How a warp covers columns and positions: 2^clog lanes side by side take VW columns each (NR times, side by side),
- * the 32 >> clog groups of such lanes take every so-manieth position. */
-template <typename GT, int VW, int NR>
-__device__ __forceinline__ void add_positions(float (&acc)[NR * VW], const GT *__restrict__ grad, uint64_t stride,
-                                              const uint32_t *__restrict__ pos, uint32_t s, uint32_t e, int lane,
-                                              int clog, uint32_t col0, uint32_t dim)
-{
-    constexpr int U = NR * VW >= 16 ? 2 : 4;
-    const int cl = 1 << clog, pl = 32 >> clog;
-    const int cg = lane & (cl - 1), pg = lane >> clog;
-    for(uint32_t base = s; base < e; base += 32) {
-        const int m = e - base < 32u ? (int)(e - base) : 32;
-        const uint32_t mine = lane < m ? __ldg(pos + base + lane) : 0u;
-        for(int k = 0; k < m; k += pl * U) {
+    __syncthreads();
+    for(int j = threadIdx.x; j < groups * run / 8; j += kThreads) {
+        const uint2 *eight = s_pair + 8 * j + 8 * j / run;
+        uint32_t key = eight[0].x, m = 0;
+#pragma unroll
+        for(int k = 0; k < 8; ++k) {
+            const uint32_t next = eight[k + 1].x;
+            m |= key != next ? 1u << k : 0u;
+            key = next;
+        }
+        s_ends[j] = (uint8_t)m;
+    }
+    __syncthreads();
+    const int group = (int)threadIdx.x >> a.clog, cg = (int)threadIdx.x & (cl - 1);
+    const uint32_t col0 = blockIdx.y * (uint32_t)(NR * VW << a.clog);
+    const int left = (int)len - group * run, r1 = left < run ? left : run; /* the group's positions */
+    uint32_t flags = 0;
+    if(r1 > 0) {
+        const uint2 *mine = s_pair + group * (run + 1);
+        const uint8_t *my_ends = s_ends + group * run / 8;
+        float acc[NR][VW] = {};
+        /* the current row began before the run */
+        bool first = group > 0 ? mine[-2].x == mine[0].x : b0 > 0 && __ldcg(&a.pairs[b0 - 1].x) == mine[0].x;
+        const unsigned char *base[NR];
+        bool in[NR]; /* which of the lane's packs lie in the row */
+#pragma unroll
+        for(int r = 0; r < NR; ++r) {
+            const uint32_t c = col0 + (uint32_t)((r * cl + cg) * VW);
+            in[r] = c < a.dim;
+            base[r] = reinterpret_cast<const unsigned char *>(grad + c);
+        }
+        auto load = [&](Pack<GT, VW> (&x)[NR], int i) {
+            const uint32_t p = mine[i].y;
+#pragma unroll
+            for(int r = 0; r < NR; ++r)
+                if(in[r]) x[r] = *reinterpret_cast<const Pack<GT, VW> *>(base[r] + (uint64_t)p * stride_bytes);
+        };
+        auto add = [&](const Pack<GT, VW> (&x)[NR]) {
+#pragma unroll
+            for(int r = 0; r < NR; ++r)
+#pragma unroll
+                for(int v = 0; v < VW; ++v) acc[r][v] += to_f32(x[r].v[v]);
+        };
+        /* the sums so far are all that the run has of `row`; `next` is the row behind them */
+        auto finish = [&](uint32_t row, uint32_t next) {
+            const bool open = next == row; /* the row goes on behind the run */
+            if(first || open) {
+                float *to = first ? s_head : s_tail;
+                flags |= !first ? kTail : open ? kHead | kWhole : kHead;
+#pragma unroll
+                for(int r = 0; r < NR; ++r)
+#pragma unroll
+                    for(int v = 0; v < VW; ++v) to[(group * NR * cl + r * cl + cg) * VW + v] = acc[r][v];
+            } else {
+#pragma unroll
+                for(int r = 0; r < NR; ++r)
+                    if(in[r]) store_sums<TT, VW>(table, row, col0 + (uint32_t)((r * cl + cg) * VW), acc[r]);
+            }
+            first = false;
+#pragma unroll
+            for(int r = 0; r < NR; ++r)
+#pragma unroll
+                for(int v = 0; v < VW; ++v) acc[r][v] = 0.0f;
+        };
+        for(int i = 0; i < r1; i += U) {
             Pack<GT, VW> x[U][NR];
-            bool in[U];
+            uint32_t ends = (uint32_t)my_ends[i >> 3] >> (i & 7) & ((1u << U) - 1u);
+            if(i + U >= r1) ends |= 1u << (r1 - 1 - i);
+            if(ends == 0u) { /* all of one row, which goes on */
 #pragma unroll
-            for(int u = 0; u < U; ++u) {
-                const int at = k + u * pl + pg;
-                const uint32_t q = __shfl_sync(0xffffffffu, mine, at & 31);
-                in[u] = at < m;
+                for(int u = 0; u < U; ++u) load(x[u], i + u);
 #pragma unroll
-                for(int r = 0; r < NR; ++r) {
-                    const uint32_t c = col0 + (uint32_t)((r * cl + cg) * VW);
-                    if(in[u] && c < dim)
-                        x[u][r] = *reinterpret_cast<const Pack<GT, VW> *>(grad + (uint64_t)q * stride + c);
-                }
+                for(int u = 0; u < U; ++u) add(x[u]);
+                continue;
             }
 #pragma unroll
             for(int u = 0; u < U; ++u)
+                if(i + u < r1) load(x[u], i + u);
 #pragma unroll
-                for(int r = 0; r < NR; ++r) {
-                    const uint32_t c = col0 + (uint32_t)((r * cl + cg) * VW);
-                    if(in[u] && c < dim)
-#pragma unroll
-                        for(int v = 0; v < VW; ++v) acc[r * VW + v] += to_f32(x[u][r].v[v]);
-                }
-        }
-    }
-}
-
-/* the groups' sums of a warp, added up (every lane of a column group gets the sum) */
-template <int N>
-__device__ __forceinline__ void join_groups(float (&acc)[N], int clog)
-{
-    for(int o = 1 << clog; o < 32; o <<= 1)
-#pragma unroll
-        for(int v = 0; v < N; ++v) acc[v] += __shfl_xor_sync(0xffffffffu, acc[v], o);
-}
-
-/* every warp's sums -> warp 0's, through shared memory, in the order of the warps */
-template <int N>
-__device__ __forceinline__ void join_warps(float (&acc)[N], float *s_join, int clog)
-{
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    __syncthreads();
-    if(lane < (1 << clog))
-#pragma unroll
-        for(int v = 0; v < N; ++v) s_join[(warp * N + v) * 32 + lane] = acc[v];
-    __syncthreads();
-    if(warp == 0 && lane < (1 << clog))
-        for(int w = 1; w < kWarps; ++w)
-#pragma unroll
-            for(int v = 0; v < N; ++v) acc[v] += s_join[(w * N + v) * 32 + lane];
-}
-
-/* partial[p] = sum of piece p, where the piece lies in one row */
-template <typename GT, int VW, int NR>
-__global__ void __launch_bounds__(kThreads) piece_sum_kernel(const GT *__restrict__ grad, uint64_t stride, Sorted sorted,
-                                                             float *__restrict__ partial, uint32_t partial_stride,
-                                                             uint32_t dim, int clog)
-{
-    __shared__ float s_join[kWarps * 32 * NR * VW];
-    __shared__ int s_in_one;
-    const uint32_t n = *sorted.n_sorted;
-    const uint64_t b = (uint64_t)blockIdx.x * kPiece;
-    if(b + kPiece > n) return;
-    if(threadIdx.x == 0) {
-        if(sorted.starts != nullptr) {
-            /* last row that starts at or before b */
-            uint64_t lo = 0, len = sorted.rows;
-            while(len > 0) {
-                const uint64_t half = len / 2;
-                if((uint64_t)__ldg(sorted.starts + lo + half) <= b) {
-                    lo += half + 1;
-                    len -= half + 1;
-                } else {
-                    len = half;
-                }
-            }
-            s_in_one = (lo < sorted.rows ? __ldg(sorted.starts + lo) : n) >= b + kPiece;
-        } else {
-            s_in_one = __ldg(sorted.keys + b) == __ldg(sorted.keys + b + kPiece - 1);
-        }
-    }
-    __syncthreads();
-    if(!s_in_one) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t col0 = blockIdx.y * (uint32_t)(NR * VW << clog);
-    float acc[NR * VW] = {};
-    constexpr uint32_t share = kPiece / kWarps;
-    const uint32_t s = (uint32_t)b + share * (uint32_t)warp;
-    add_positions<GT, VW, NR>(acc, grad, stride, sorted.pos, s, s + share, lane, clog, col0, dim);
-    join_groups(acc, clog);
-    join_warps(acc, s_join, clog);
-    if(warp == 0 && lane < (1 << clog)) {
-#pragma unroll
-        for(int r = 0; r < NR; ++r) {
-            const uint32_t c = col0 + (uint32_t)(((r << clog) + lane) * VW);
-            if(c < dim)
-#pragma unroll
-                for(int v = 0; v < VW; ++v)
-                    if(c + v < dim) partial[(uint64_t)blockIdx.x * partial_stride + c + v] = acc[r * VW + v];
-        }
-    }
-}
-
-template <typename TT, int VW, int NR>
-__device__ __forceinline__ void store_row(const float (&acc)[NR * VW], TT *__restrict__ row, float scale, bool accumulate,
-                                          int lane, int clog, uint32_t col0, uint32_t dim)
-{
-    if(lane >= (1 << clog)) return;
-#pragma unroll
-    for(int r = 0; r < NR; ++r) {
-        const uint32_t c = col0 + (uint32_t)(((r << clog) + lane) * VW);
-        if(c >= dim) continue;
-        Pack<TT, VW> y;
-        if(accumulate) y = *reinterpret_cast<const Pack<TT, VW> *>(row + c);
-#pragma unroll
-        for(int v = 0; v < VW; ++v)
-            y.v[v] = from_f32<TT>(accumulate ? fmaf(scale, acc[r * VW + v], to_f32(y.v[v])) : scale * acc[r * VW + v]);
-        *reinterpret_cast<Pack<TT, VW> *>(row + c) = y;
-    }
-}
-
-/* grad_table[v] for the rows of this CTA (rows_per_cta from blockIdx.x on) and its columns (blockIdx.y) */
-constexpr int kMaxRowsPerCta = 64;
-template <typename GT, typename TT, int VW, int NR>
-__global__ void __launch_bounds__(kThreads) row_sum_kernel(const GT *__restrict__ grad, uint64_t stride, Sorted sorted,
-                                                           const float *__restrict__ partial, uint32_t partial_stride,
-                                                           float scale, TT *__restrict__ table, uint64_t table_stride,
-                                                           uint32_t dim, int clog, int rows_per_cta, bool accumulate)
-{
-    __shared__ uint32_t s_start[kMaxRowsPerCta + 1];
-    __shared__ float s_join[kWarps * 32 * NR * VW];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t n = *sorted.n_sorted;
-    const uint64_t row0 = (uint64_t)blockIdx.x * rows_per_cta;
-    if((int)threadIdx.x <= rows_per_cta) s_start[threadIdx.x] = first_of(sorted, n, row0 + threadIdx.x);
-    __syncthreads();
-    const uint32_t col0 = blockIdx.y * (uint32_t)(NR * VW << clog);
-    bool any_long = false;
-    for(int r = 0; r < rows_per_cta; ++r) {
-        const uint64_t v = row0 + r;
-        if(v >= sorted.rows) break;
-        const uint32_t s = s_start[r], e = s_start[r + 1];
-        if(e - s > (uint32_t)kWarpMax) {
-            any_long = true;
-            continue;
-        }
-        if((r % kWarps) != warp || (accumulate && s == e)) continue;
-        float acc[NR * VW] = {};
-        add_positions<GT, VW, NR>(acc, grad, stride, sorted.pos, s, e, lane, clog, col0, dim);
-        if(s != e) join_groups(acc, clog);
-        store_row<TT, VW, NR>(acc, table + v * table_stride, scale, accumulate, lane, clog, col0, dim);
-    }
-    if(!any_long) return;
-    for(int r = 0; r < rows_per_cta; ++r) {
-        const uint64_t v = row0 + r;
-        if(v >= sorted.rows) break;
-        const uint32_t s = s_start[r], e = s_start[r + 1];
-        if(e - s <= (uint32_t)kWarpMax) continue;
-        float acc[NR * VW] = {};
-        /* whole pieces inside the row were summed by piece_sum_kernel */
-        const uint32_t p0 = (s + kPiece - 1) / kPiece, p1 = e / kPiece;
-        const uint32_t head_end = p0 < p1 ? p0 * kPiece : e, tail = p0 < p1 ? p1 * kPiece : e;
-        const uint32_t hshare = (head_end - s + kWarps - 1) / kWarps, tshare = (e - tail + kWarps - 1) / kWarps;
-        const uint32_t h0 = s + hshare * warp < head_end ? s + hshare * warp : head_end;
-        const uint32_t h1 = h0 + hshare < head_end ? h0 + hshare : head_end;
-        add_positions<GT, VW, NR>(acc, grad, stride, sorted.pos, h0, h1, lane, clog, col0, dim);
-        const int pg = lane >> clog, pl = 32 >> clog;
-        for(uint32_t p = p0 + (uint32_t)(warp * pl + pg); p < p1; p += (uint32_t)(kWarps * pl)) {
-#pragma unroll
-            for(int k = 0; k < NR; ++k) {
-                const uint32_t c = col0 + (uint32_t)(((k << clog) + (lane & ((1 << clog) - 1))) * VW);
-#pragma unroll
-                for(int w = 0; w < VW; ++w)
-                    if(c + w < dim) acc[k * VW + w] += __ldg(partial + (uint64_t)p * partial_stride + c + w);
+            for(int u = 0; u < U; ++u) {
+                if(i + u < r1) add(x[u]);
+                if(ends >> u & 1u) finish(mine[i + u].x, mine[i + u + 1].x);
             }
         }
-        const uint32_t t0 = tail + tshare * warp < e ? tail + tshare * warp : e;
-        const uint32_t t1 = t0 + tshare < e ? t0 + tshare : e;
-        add_positions<GT, VW, NR>(acc, grad, stride, sorted.pos, t0, t1, lane, clog, col0, dim);
-        join_groups(acc, clog);
-        join_warps(acc, s_join, clog);
-        if(warp == 0) store_row<TT, VW, NR>(acc, table + v * table_stride, scale, accumulate, lane, clog, col0, dim);
+    }
+    if(cg == 0) s_flags[group] = flags;
+    __syncthreads();
+    /* rows across groups, one thread a column */
+    const uint32_t cols = (uint32_t)(NR * VW << a.clog);
+    const uint2 *last = s_pair + groups * (run + 1) - 2;
+    const bool cta_tail = last[0].x == last[1].x && len == (uint32_t)(groups * run);
+    for(uint32_t c = threadIdx.x; c < cols && col0 + c < a.dim; c += kThreads) {
+        float cur = 0.0f;
+        bool outside = true;
+        for(int g = 0; g < groups; ++g) {
+            const uint32_t f = s_flags[g];
+            if(f & kHead) {
+                cur += s_head[g * cols + c];
+                if(!(f & kWhole)) {
+                    if(outside) {
+                        a.head[(uint64_t)blockIdx.x * a.dim + col0 + c] = cur;
+                    } else {
+                        const float one[1] = { cur };
+                        store_sums<TT, 1>(table, s_pair[g * (run + 1)].x, col0 + c, one);
+                    }
+                    outside = false;
+                }
+            }
+            if(f & kTail) {
+                cur = s_tail[g * cols + c];
+                outside = false;
+            }
+        }
+        if(cta_tail) (outside ? a.head : a.tail)[(uint64_t)blockIdx.x * a.dim + col0 + c] = cur;
     }
 }
 
-template <typename GT, typename TT, int VW, int NR>
-void launch_sums(const GT *grad, uint64_t grad_stride, const Sorted &sorted, uint64_t count, float *partial,
-                 float scale, TT *table, uint64_t table_stride, uint64_t dim, bool accumulate, cudaStream_t stream)
+/* Rows across CTAs of run_sum_kernel: the CTA (x) in which such a row begins adds up its parts.  Columns: 256 to a
+ * CTA (y), a thread each, while the row has few parts; else 32 at a time, the parts dealt to the eight warps. */
+constexpr uint32_t kFewParts = 16;
+template <typename TT>
+__global__ void __launch_bounds__(kThreads) row_join_kernel(const Runs a, const Table table)
 {
-    int clog = 0;
-    while(clog < 5 && ((uint64_t)(NR * VW) << clog) < dim) ++clog;
-    const uint64_t cols = (uint64_t)(NR * VW) << clog;
-    const unsigned tiles = (unsigned)((dim + cols - 1) / cols);
-    if(count >= (uint64_t)kPiece)
-        piece_sum_kernel<GT, VW, NR><<<dim3((unsigned)(count / kPiece), tiles), kThreads, 0, stream>>>(
-            grad, grad_stride, sorted, partial, (uint32_t)dim, (uint32_t)dim, clog);
-    /* few rows: one to a warp, so that they spread over the GPU; many: 64 share a CTA's searches */
-    int rows_per_cta = kWarps;
-    while(rows_per_cta < kMaxRowsPerCta && (sorted.rows / (uint64_t)rows_per_cta) * tiles > 148 * 16) rows_per_cta *= 2;
-    const unsigned ctas = (unsigned)((sorted.rows + rows_per_cta - 1) / rows_per_cta);
-    row_sum_kernel<GT, TT, VW, NR><<<dim3(ctas, tiles), kThreads, 0, stream>>>(
-        grad, grad_stride, sorted, partial, (uint32_t)dim, scale, table, table_stride, (uint32_t)dim, clog, rows_per_cta,
-        accumulate);
-}
-
-template <typename GT, typename TT>
-void launch_sums_typed(const void *grad_, uint64_t grad_stride, const Sorted &sorted, uint64_t count, float *partial,
-                       float scale, void *table_, uint64_t table_stride, uint64_t dim, bool accumulate,
-                       cudaStream_t stream)
-{
-    const GT *grad = static_cast<const GT *>(grad_);
-    TT *table = static_cast<TT *>(table_);
-    constexpr int VW = 16 / sizeof(GT);
-    constexpr uint64_t TA = VW * sizeof(TT) < 16 ? VW * sizeof(TT) : 16;
-    if(dim % VW == 0 && grad_stride % VW == 0 && (uintptr_t)grad % 16 == 0 && (uintptr_t)table % TA == 0 &&
-       (table_stride * sizeof(TT)) % TA == 0) {
-        if(dim > 32 * VW) launch_sums<GT, TT, VW, 2>(grad, grad_stride, sorted, count, partial, scale, table, table_stride, dim, accumulate, stream);
-        else launch_sums<GT, TT, VW, 1>(grad, grad_stride, sorted, count, partial, scale, table, table_stride, dim, accumulate, stream);
-    } else {
-        if(dim > 32) launch_sums<GT, TT, 1, 2>(grad, grad_stride, sorted, count, partial, scale, table, table_stride, dim, accumulate, stream);
-        else launch_sums<GT, TT, 1, 1>(grad, grad_stride, sorted, count, partial, scale, table, table_stride, dim, accumulate, stream);
+    __shared__ float s_part[kWarps][32];
+    gsx_pdl_wait();
+    const uint32_t n = __ldcg(a.n_sorted);
+    const uint32_t R = (uint32_t)(kThreads >> a.clog) * (uint32_t)a.run;
+    const uint32_t b = blockIdx.x, b0 = b * R, b1 = b0 + R;
+    if(b1 >= n) return;
+    const uint32_t row = __ldcg(&a.pairs[b1 - 1].x);
+    if(__ldcg(&a.pairs[b1].x) != row) return;
+    if(b0 > 0 && __ldcg(&a.pairs[b0].x) == row && __ldcg(&a.pairs[b0 - 1].x) == row) return; /* began before */
+    /* the last CTA whose first position has the row */
+    uint32_t lo = b + 1, hi = (n - 1) / R;
+    while(lo < hi) {
+        const uint32_t mid = (lo + hi + 1) / 2;
+        if(__ldcg(&a.pairs[(uint64_t)mid * R].x) == row) lo = mid;
+        else hi = mid - 1;
+    }
+    const uint32_t parts = lo - b;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t c0 = blockIdx.y * 256u;
+    if(parts <= kFewParts) {
+        const uint32_t c = c0 + threadIdx.x;
+        if(c >= a.dim) return;
+        float sum[1] = { __ldcg(a.tail + (uint64_t)b * a.dim + c) };
+        for(uint32_t k = 1; k <= parts; ++k) sum[0] += __ldcg(a.head + (uint64_t)(b + k) * a.dim + c);
+        store_sums<TT, 1>(table, row, c, sum);
+        return;
+    }
+    for(uint32_t c1 = c0; c1 < a.dim && c1 < c0 + 256u; c1 += 32) {
+        const uint32_t c = c1 + lane;
+        float sum[1] = { 0.0f };
+        if(c < a.dim) {
+            if(warp == 0) sum[0] = __ldcg(a.tail + (uint64_t)b * a.dim + c);
+#pragma unroll 8
+            for(uint32_t k = 1 + warp; k <= parts; k += kWarps) sum[0] += __ldcg(a.head + (uint64_t)(b + k) * a.dim + c);
+        }
+        __syncthreads();
+        s_part[warp][lane] = sum[0];
+        __syncthreads();
+        if(warp == 0 && c < a.dim) {
+#pragma unroll
+            for(int w = 1; w < kWarps; ++w) sum[0] += s_part[w][lane];
+            store_sums<TT, 1>(table, row, c, sum);
+        }
     }
 }
 
 /* ------------------------------------------------------------------------------------------ */
-/* workspace: n_sorted | totals, starts | counts | pairs, keys, positions | partial sums */
+/* workspace: n_sorted | counts | pairs, pairs | sums of rows across CTAs */
 
 struct Plan {
     int passes = 0; /* 0: the one-CTA sort */
     int bits[4] = {};
     uint32_t chunks = 0;
-    size_t o_words = 0, o_starts = 0, o_counts = 0, o_pairs = 0, o_pairs2 = 0, o_keys = 0, o_pos = 0, o_partial = 0, bytes = 0;
+    /* the sums */
+    int clog = 0, nr = 1, run = 8;
+    uint32_t ctas = 0, tiles = 1;
+    size_t o_counts = 0, o_pairs[2] = {}, o_head = 0, o_tail = 0, bytes = 0;
 };
 
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
-Plan make_plan(uint64_t count, uint64_t rows, uint64_t dim)
+/* How the sums lay lanes over columns: packs of a row over 2^clog lanes and NR packs a lane, as few idle ones as
+ * possible (fewer packs a lane where that is equal); rows of more than 32 lanes take several CTAs side by side. */
+void plan_sums(Plan &p, uint64_t count, uint64_t packs)
+{
+    uint64_t best = UINT64_MAX;
+    for(int nr = 1; nr <= 3; ++nr)
+        for(int clog = 2; clog <= 5; ++clog) {
+            const uint64_t slots = (uint64_t)nr << clog;
+            const uint64_t tiles = (packs + slots - 1) / slots;
+            if(tiles > 1 && (clog < 5 || nr > 2)) continue;
+            const uint64_t cost = tiles * slots * 16 + (uint64_t)nr;
+            if(cost < best) {
+                best = cost;
+                p.nr = nr;
+                p.clog = clog;
+                p.tiles = (uint32_t)tiles;
+            }
+        }
+    const uint64_t groups = kThreads >> p.clog;
+    /* one wave of CTAs with equal work (four an SM): a second, partly filled wave costs more than the longer runs */
+    uint64_t run = (count * p.tiles + groups * 592 - 1) / (groups * 592);
+    run = (run + 7) / 8 * 8;
+    if(run < 8) run = 8;
+    if(run > (uint64_t)kMaxRun) run = kMaxRun;
+    if(run > kMaxPositions / groups) run = kMaxPositions / groups;
+    p.run = (int)run;
+    p.ctas = (uint32_t)((count + groups * run - 1) / (groups * run));
+}
+
+/* The layout of one call.  `vec`: elements of a pack.  The sizes do not depend on it or on the pointers, which
+ * gsx_b200_embedding_workspace_bytes does not know: they are those of the larger choice. */
+Plan make_plan(uint64_t count, uint64_t rows, uint64_t dim, uint64_t vec)
 {
     Plan p;
     size_t o = 256;
     if(count > (uint64_t)kSmallCount) {
-        int bits = 0;
+        int bits = 1;
         while(bits < 32 && (rows - 1) >> bits) ++bits;
-        if(bits == 0) bits = 1;
         p.passes = (bits + kMaxBits - 1) / kMaxBits;
         for(int i = 0; i < p.passes; ++i) {
             p.bits[i] = (bits + p.passes - 1 - i) / (p.passes - i);
             bits -= p.bits[i];
         }
-        uint64_t chunks = (count + 4095) / 4096;
-        if(chunks > (uint64_t)kChunks) chunks = kChunks;
-        const uint64_t least = (count + kMaxChunk - kSortThreads - 1) / (kMaxChunk - kSortThreads);
-        if(chunks < least) chunks = least;
-        p.chunks = (uint32_t)chunks;
-        p.o_words = o;
-        o += align256(sizeof(uint32_t) * kMaxBins) * p.passes; /* totals of every pass */
-        p.o_starts = o;
-        o += align256(sizeof(uint32_t) * (kMaxBins + 1));
+        const uint64_t chunks = (count + kTile - 1) / kTile;
+        p.chunks = (uint32_t)(chunks < (uint64_t)kChunks ? chunks : kChunks);
         p.o_counts = o;
-        o += align256(sizeof(uint32_t) * chunks << p.bits[0]);
-        if(p.passes > 1) {
-            p.o_pairs = o;
-            o += align256(sizeof(uint2) * count);
-        }
-        if(p.passes > 2) {
-            p.o_pairs2 = o;
-            o += align256(sizeof(uint2) * count);
-        }
+        o += align256(sizeof(uint32_t) * p.chunks * kMaxBins);
     }
-    if(p.passes != 1) {
-        p.o_keys = o;
-        o += align256(sizeof(uint32_t) * count);
-    }
-    p.o_pos = o;
-    o += align256(sizeof(uint32_t) * count);
-    p.o_partial = o;
-    o += align256(sizeof(float) * (count / kPiece) * dim);
-    p.bytes = o;
+    p.o_pairs[0] = o;
+    o += align256(sizeof(uint2) * count);
+    p.o_pairs[1] = o;
+    if(p.passes > 1) o += align256(sizeof(uint2) * count);
+    /* every CTA of the sums has at least 64 positions (8 groups of 8) */
+    const size_t ends = align256(sizeof(float) * ((count + 63) / 64) * dim);
+    p.o_head = o;
+    p.o_tail = o + ends;
+    p.bytes = o + 2 * ends;
+    plan_sums(p, count, (dim + vec - 1) / vec);
     return p;
-}
-
-size_t small_smem() { return sizeof(uint32_t) * (2 * kSmallCount + 32 * 256 + 32); }
-size_t scatter_smem(int bits)
-{
-    const size_t bins = (size_t)1 << bits;
-    return sizeof(uint32_t) * (bins + kSortWarps * (bins > 1 ? bins / 2 : 1));
 }
 
 template <typename K>
@@ -844,66 +859,93 @@ cudaError_t allow_smem(K kernel, size_t bytes)
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
 }
 
-template <typename I, bool kFirst, bool kLast>
-cudaError_t launch_pass(const I *index, const uint2 *pairs, uint64_t count, uint32_t *n_sorted, uint64_t rows,
-                        int64_t padding, int shift, int bits, uint32_t chunks, uint32_t *totals, uint32_t *starts,
-                        uint32_t *counts, uint2 *pairs_out, uint32_t *keys_out, uint32_t *pos_out, uint32_t *bad,
+template <typename I, bool kFirst>
+cudaError_t launch_pass(const I *index, const uint2 *pairs, uint32_t count, uint32_t *n_sorted, const Use &use, int shift,
+                        int bits, uint32_t chunks, uint32_t *counts, uint2 *out, const Table &table, uint32_t dim,
                         cudaStream_t stream)
 {
-    const cudaError_t e = allow_smem(digit_scatter_kernel<I, kFirst, kLast>, scatter_smem(kMaxBits));
+    constexpr size_t smem = sizeof(SortShared<kSortThreads, kSortItems>);
+    cudaError_t e = allow_smem(digit_scatter_kernel<I, kFirst>, smem);
     if(e != cudaSuccess) return e;
-    const int bins = 1 << bits;
-    digit_count_kernel<I, kFirst><<<chunks, kSortThreads, 0, stream>>>(index, pairs, count, n_sorted, rows, padding,
-                                                                       shift, bits, counts, totals, bad);
-    digit_scan_kernel<<<(bins + 31) / 32, 1024, 0, stream>>>(counts, chunks, bins, totals, starts, n_sorted);
-    digit_scatter_kernel<I, kFirst, kLast><<<chunks, kSortThreads, scatter_smem(bits), stream>>>(
-        index, pairs, count, n_sorted, rows, padding, shift, bits, counts, pairs_out, keys_out, pos_out);
-    return cudaSuccess;
+    if(kFirst)
+        digit_count_kernel<I, true><<<chunks, kSortThreads, 0, stream>>>(index, pairs, count, n_sorted, use, shift, bits,
+                                                                         counts, table, dim);
+    else
+        e = gsx_launch_pdl(digit_count_kernel<I, false>, dim3(chunks), dim3(kSortThreads), 0, stream, index, pairs, count,
+                           n_sorted, use, shift, bits, counts, table, dim);
+    Use quiet = use; /* indices are reported once, by the count */
+    quiet.bad = nullptr;
+    if(e == cudaSuccess)
+        e = gsx_launch_pdl(digit_scatter_kernel<I, kFirst>, dim3(chunks), dim3(kSortThreads), smem, stream, index, pairs, count,
+                           n_sorted, quiet, shift, bits, counts, out);
+    return e;
 }
 
+/* sorted pairs end up in *out_pairs; the table's rows are zero afterwards (unless it accumulates) */
 template <typename I>
-cudaError_t launch_sort(const Plan &plan, unsigned char *ws, const void *index_, uint64_t count, uint64_t rows,
-                        int64_t padding, uint32_t *bad, cudaStream_t stream)
+cudaError_t launch_sort(const Plan &plan, unsigned char *ws, const void *index_, uint32_t count, const Use &use,
+                        const Table &table, uint32_t dim, const uint2 **out_pairs, cudaStream_t stream)
 {
     const I *index = static_cast<const I *>(index_);
     uint32_t *n_sorted = reinterpret_cast<uint32_t *>(ws);
-    uint32_t *keys = plan.passes != 1 ? reinterpret_cast<uint32_t *>(ws + plan.o_keys) : nullptr;
-    uint32_t *pos = reinterpret_cast<uint32_t *>(ws + plan.o_pos);
+    uint2 *pairs[2] = { reinterpret_cast<uint2 *>(ws + plan.o_pairs[0]), reinterpret_cast<uint2 *>(ws + plan.o_pairs[1]) };
     if(plan.passes == 0) {
-        const cudaError_t e = allow_smem(small_sort_kernel<I>, small_smem());
+        *out_pairs = pairs[0];
+        constexpr size_t smem = sizeof(SortShared<kSmallThreads, kSmallItems>);
+        cudaError_t e = allow_smem(small_sort_kernel<I>, smem);
         if(e != cudaSuccess) return e;
-        small_sort_kernel<I><<<1, kSmallThreads, small_smem(), stream>>>(index, (uint32_t)count, rows, padding, keys,
-                                                                         pos, n_sorted, bad);
-        return cudaSuccess;
+        small_sort_kernel<I><<<1, kSmallThreads, smem, stream>>>(index, count, use, pairs[0], n_sorted);
+        if(!table.accumulate) {
+            /* 16 KB of zeros a CTA: many short CTAs write 15% faster than one wave of long ones (6.9 against 6.0 TB/s) */
+            const uint64_t ctas = (table.rows * dim * table.bytes + 16383) / 16384;
+            e = gsx_launch_pdl(zero_kernel, dim3((unsigned)(ctas < (1u << 30) ? ctas : 1u << 30)), dim3(kThreads), 0, stream,
+                               table, dim);
+        }
+        return e;
     }
-    const size_t each = align256(sizeof(uint32_t) * kMaxBins);
-    cudaError_t e = cudaMemsetAsync(ws + plan.o_words, 0, each * plan.passes, stream);
-    if(e != cudaSuccess) return e;
-    uint32_t *starts = reinterpret_cast<uint32_t *>(ws + plan.o_starts);
     uint32_t *counts = reinterpret_cast<uint32_t *>(ws + plan.o_counts);
-    uint2 *from = nullptr, *to = reinterpret_cast<uint2 *>(ws + plan.o_pairs);
-    int shift = 0;
-    for(int p = 0; p < plan.passes; ++p) {
-        uint32_t *totals = reinterpret_cast<uint32_t *>(ws + plan.o_words + each * p);
-        const bool first = p == 0, last = p == plan.passes - 1;
-        if(first && last)
-            e = launch_pass<I, true, true>(index, nullptr, count, n_sorted, rows, padding, shift, plan.bits[p], plan.chunks,
-                                           totals, starts, counts, nullptr, keys, pos, bad, stream);
-        else if(first)
-            e = launch_pass<I, true, false>(index, nullptr, count, n_sorted, rows, padding, shift, plan.bits[p],
-                                            plan.chunks, totals, starts, counts, to, nullptr, nullptr, bad, stream);
-        else if(!last)
-            e = launch_pass<I, false, false>(index, from, count, n_sorted, rows, padding, shift, plan.bits[p],
-                                             plan.chunks, totals, starts, counts, to, nullptr, nullptr, bad, stream);
-        else
-            e = launch_pass<I, false, true>(index, from, count, n_sorted, rows, padding, shift, plan.bits[p],
-                                            plan.chunks, totals, starts, counts, nullptr, keys, pos, bad, stream);
+    for(int p = 0, shift = 0; p < plan.passes; shift += plan.bits[p], ++p) {
+        uint2 *to = pairs[p & 1];
+        const cudaError_t e = p == 0 ? launch_pass<I, true>(index, nullptr, count, n_sorted, use, shift, plan.bits[p],
+                                                            plan.chunks, counts, to, table, dim, stream)
+                                     : launch_pass<I, false>(index, pairs[(p - 1) & 1], count, n_sorted, use, shift, plan.bits[p],
+                                                             plan.chunks, counts, to, table, dim, stream);
         if(e != cudaSuccess) return e;
-        shift += plan.bits[p];
-        from = to;
-        to = reinterpret_cast<uint2 *>(ws + (p % 2 == 0 && plan.passes > 2 ? plan.o_pairs2 : plan.o_pairs));
+        *out_pairs = to;
     }
     return cudaSuccess;
+}
+
+template <typename GT, typename TT, int VW, int NR>
+cudaError_t launch_runs(const GT *grad, uint64_t stride, const Plan &plan, const Runs &runs, const Table &table,
+                        cudaStream_t stream)
+{
+    const size_t fixed = sizeof(float) * 2 * kThreads * NR * VW;
+    const cudaError_t e = allow_smem(run_sum_kernel<GT, TT, VW, NR>, fixed + sizeof(uint2) * (kMaxPositions + kThreads / 4));
+    if(e != cudaSuccess) return e;
+    return gsx_launch_pdl(run_sum_kernel<GT, TT, VW, NR>, dim3(plan.ctas, plan.tiles), dim3(kThreads),
+                          fixed + sizeof(uint2) * (size_t)(kThreads >> plan.clog) * (plan.run + 1), stream, grad,
+                          (uint32_t)(stride * sizeof(GT)), runs, table);
+}
+
+template <typename GT, typename TT>
+cudaError_t launch_sums(const void *grad_, uint64_t stride, uint64_t vec, const Plan &plan, const Runs &runs,
+                        const Table &table, cudaStream_t stream)
+{
+    const GT *grad = static_cast<const GT *>(grad_);
+    constexpr int VW = 16 / sizeof(GT);
+    cudaError_t e;
+    if(vec == (uint64_t)VW)
+        e = plan.nr == 1 ? launch_runs<GT, TT, VW, 1>(grad, stride, plan, runs, table, stream)
+            : plan.nr == 2 ? launch_runs<GT, TT, VW, 2>(grad, stride, plan, runs, table, stream)
+                           : launch_runs<GT, TT, VW, 3>(grad, stride, plan, runs, table, stream);
+    else
+        e = plan.nr == 1 ? launch_runs<GT, TT, 1, 1>(grad, stride, plan, runs, table, stream)
+            : plan.nr == 2 ? launch_runs<GT, TT, 1, 2>(grad, stride, plan, runs, table, stream)
+                           : launch_runs<GT, TT, 1, 3>(grad, stride, plan, runs, table, stream);
+    if(e == cudaSuccess && plan.ctas > 1)
+        e = gsx_launch_pdl(row_join_kernel<TT>, dim3(plan.ctas - 1, (runs.dim + 255) / 256), dim3(kThreads), 0, stream, runs, table);
+    return e;
 }
 
 bool float_type(int t) { return t == GSX_B200_DATA_F32 || t == GSX_B200_DATA_F16 || t == GSX_B200_DATA_BF16; }
@@ -970,7 +1012,7 @@ extern "C" int gsx_b200_embedding_lookup(const void *table, int table_type, uint
 extern "C" uint64_t gsx_b200_embedding_workspace_bytes(uint64_t count, uint64_t rows, uint64_t dim)
 {
     if(count > (uint64_t)INT32_MAX || rows > (uint64_t)INT32_MAX || dim > (uint64_t)INT32_MAX || rows == 0) return 0;
-    return make_plan(count, rows, dim).bytes;
+    return make_plan(count, rows, dim, 1).bytes;
 }
 
 extern "C" int gsx_b200_embedding_backward(const void *grad_out, int grad_type, uint64_t grad_stride, const void *index,
@@ -985,6 +1027,8 @@ extern "C" int gsx_b200_embedding_backward(const void *grad_out, int grad_type, 
         return gsx_internal_fail(GSX_B200_NOT_SUPPORTED, "embedding indices are i32 or i64");
     if(int rc = check_shape(rows, dim, grad_stride, table_stride, count)) return rc;
     if(dim > 65535ull * 32) return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "dim must be at most 2097120");
+    if(grad_stride * float_bytes(grad_type) > 0xffffffffull)
+        return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "grad_stride must be below 4 GiB");
     if(padding_row >= (int64_t)rows) return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "padding_row must be below rows");
     if(dim == 0 || (rows == 0 && count == 0)) return GSX_B200_SUCCESS;
     if(rows == 0) return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "rows must be positive");
@@ -994,26 +1038,39 @@ extern "C" int gsx_b200_embedding_backward(const void *grad_out, int grad_type, 
        (uintptr_t)index % (index_type == GSX_B200_DATA_I32 ? 4 : 8) || (uintptr_t)workspace % 16)
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT,
                                  "pointers must be aligned to their element type, the workspace to 16 bytes");
-    const Plan plan = make_plan(count, rows, dim);
+    Table table;
+    table.data = grad_table;
+    table.stride = table_stride;
+    table.rows = rows;
+    table.scale = scale;
+    table.bytes = (int)float_bytes(table_type);
+    table.accumulate = accumulate != 0;
+    const uint64_t gb = float_bytes(grad_type), pack = 16 / gb;
+    const uint64_t tb = float_bytes(table_type) * pack < 16 ? float_bytes(table_type) * pack : 16;
+    const bool packs = dim % pack == 0 && grad_stride % pack == 0 && (uintptr_t)grad_out % 16 == 0 &&
+                       (uintptr_t)grad_table % tb == 0 && table_stride * float_bytes(table_type) % tb == 0;
+    const uint64_t vec = packs ? pack : 1;
+    const Plan plan = make_plan(count, rows, dim, vec);
     if(workspace_bytes < plan.bytes)
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT,
                                  "workspace is smaller than gsx_b200_embedding_workspace_bytes");
     cudaStream_t stream = (cudaStream_t)stream_;
     unsigned char *ws = static_cast<unsigned char *>(workspace);
-    const cudaError_t e = index_type == GSX_B200_DATA_I32
-                              ? launch_sort<int32_t>(plan, ws, index, count, rows, padding_row, device_out_of_range, stream)
-                              : launch_sort<int64_t>(plan, ws, index, count, rows, padding_row, device_out_of_range, stream);
-    if(e != cudaSuccess) return launch_status(e);
-    Sorted sorted;
-    sorted.pos = reinterpret_cast<const uint32_t *>(ws + plan.o_pos);
-    sorted.keys = plan.passes != 1 ? reinterpret_cast<const uint32_t *>(ws + plan.o_keys) : nullptr;
-    sorted.starts = plan.passes == 1 ? reinterpret_cast<const uint32_t *>(ws + plan.o_starts) : nullptr;
-    sorted.n_sorted = reinterpret_cast<const uint32_t *>(ws);
-    sorted.rows = rows;
-    float *partial = reinterpret_cast<float *>(ws + plan.o_partial);
+    const Use use = { (uint32_t)rows, padding_row < 0 ? UINT32_MAX : (uint32_t)padding_row, device_out_of_range };
+    cudaError_t e = cudaSuccess;
+    Runs runs;
+    e = index_type == GSX_B200_DATA_I32
+            ? launch_sort<int32_t>(plan, ws, index, (uint32_t)count, use, table, (uint32_t)dim, &runs.pairs, stream)
+            : launch_sort<int64_t>(plan, ws, index, (uint32_t)count, use, table, (uint32_t)dim, &runs.pairs, stream);
+    if(e != cudaSuccess || count == 0) return launch_status(e);
+    runs.n_sorted = reinterpret_cast<const uint32_t *>(ws);
+    runs.head = reinterpret_cast<float *>(ws + plan.o_head);
+    runs.tail = reinterpret_cast<float *>(ws + plan.o_tail);
+    runs.dim = (uint32_t)dim;
+    runs.clog = plan.clog;
+    runs.run = plan.run;
     GSX_WITH_FLOAT_TYPE(grad_type, GT, GSX_WITH_FLOAT_TYPE(table_type, TT, {
-        launch_sums_typed<GT, TT>(grad_out, grad_stride, sorted, count, partial, scale, grad_table, table_stride, dim,
-                                  accumulate != 0, stream);
+        e = launch_sums<GT, TT>(grad_out, grad_stride, vec, plan, runs, table, stream);
     }));
-    return launch_status(cudaSuccess);
+    return launch_status(e);
 }

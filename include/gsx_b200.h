@@ -400,8 +400,8 @@ GSX_B200_API int gsx_b200_adc_select_keep(uint64_t n, const float *opacity, cons
 /*
  * Shared rows (no counterpart in the reference): a table whose rows many Gaussians share, with one row number
  * per Gaussian, or any other embedding table.  Tables, outputs and gradients are f32, f16 or bf16 in any
- * combination, indices i32 or i64; row strides are in elements and at least dim; rows, dim and count stay below
- * 2^31.  An index outside [0, rows) sets *device_out_of_range to 1 (when non-NULL) and takes no part: its row of
+ * combination, indices i32 or i64; row strides are in elements and at least dim (that of grad_out is below
+ * 4 GiB); rows, dim and count stay below 2^31.  An index outside [0, rows) sets *device_out_of_range to 1 (when non-NULL) and takes no part: its row of
  * out stays untouched, its gradient is dropped.  Nothing waits, allocates or depends on values: the calls can be
  * captured into a graph.
  * gsx_b200_embedding_lookup: out[n] = scale * table[index[n]], computed in f32 and rounded once.

@@ -50,7 +50,7 @@ CASES = [
                                     dict(table=P + 2), dict(out=P + 1, otype=F16), dict(index=P + 4, itype=I64)]),
     (_capi.SUCCESS, _lookup, [dict(count=0), dict(dim=0)]),
     (gb.NOT_SUPPORTED, _backward, [dict(gtype=U8), dict(ttype=I32), dict(itype=U8)]),
-    (gb.OUT_OF_RANGE, _backward, [dict(rows=2 ** 31), dict(padding=4),
+    (gb.OUT_OF_RANGE, _backward, [dict(rows=2 ** 31), dict(padding=4), dict(gstride=2 ** 30),
                                   dict(dim=2 ** 22, gstride=2 ** 22, tstride=2 ** 22)]),
     (gb.INVALID_ARGUMENT, _backward, [dict(grad=None), dict(index=None), dict(table=None), dict(ws=None), dict(gstride=7),
                                       dict(tstride=7), dict(size=100), dict(ws=P + 8), dict(grad=P + 2),
@@ -92,10 +92,10 @@ def test_workspace_sizes():
     assert L.gsx_b200_embedding_workspace_bytes(10, 0, 4) == 0
     small = L.gsx_b200_embedding_workspace_bytes(100, 50, 4)
     assert 800 <= small < 1 << 20
-    # one-pass sort: positions, chunk counts, pieces; two passes: also pairs and keys
-    one = L.gsx_b200_embedding_workspace_bytes(1_000_000, 4096, 3)
-    two = L.gsx_b200_embedding_workspace_bytes(1_000_000, 4097, 3)
-    assert 4_000_000 < one < 8_000_000 < 16_000_000 < two < 24_000_000
+    # (row, position) pairs: once for a sort of one pass (up to 256 rows), twice for more
+    one = L.gsx_b200_embedding_workspace_bytes(1_000_000, 256, 8)
+    two = L.gsx_b200_embedding_workspace_bytes(1_000_000, 257, 8)
+    assert 8_000_000 < one < 16_000_000 <= two < 24_000_000
     assert L.gsx_b200_budget_workspace_bytes(32, 49_152) == 0
     assert 0 < L.gsx_b200_budget_workspace_bytes(32, 49_153) < 4 << 20
 

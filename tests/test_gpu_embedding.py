@@ -118,7 +118,8 @@ def _check_gradient(got, grad, index, rows, scale, before=None, drop=None):
 
 GRADIENT_SIZES = [(0, 5, 3), (1, 1, 1), (5, 1, 4), (100, 256, 8), (8192, 300, 7), (8193, 300, 7), (9000, 1, 3),
                   (20_000, 4096, 3), (20_000, 4097, 4), (50_000, 70_000, 2), (33_333, 5000, 45), (300, 1000, 2048),
-                  (12_000, 3, 260), (2000, 50, 33)]
+                  (12_000, 3, 260), (2000, 50, 33), (200_001, 100, 1), (300_000, 1000, 2), (700_000, 4096, 3),
+                  (150_000, 777, 4), (60_000, 1, 3)]
 
 
 @pytest.mark.parametrize("count,rows,dim", GRADIENT_SIZES)
@@ -137,7 +138,7 @@ def test_gradient_sizes(cuda_device, count, rows, dim):
 @pytest.mark.parametrize("grad_type", [F32, F16, BF16])
 def test_gradient_types(cuda_device, grad_type, table_type, itype):
     g = _gen(5)
-    for count, rows, dim in [(700, 40, 64), (9001, 600, 5), (900, 30, 16)]:
+    for count, rows, dim in [(700, 40, 64), (9001, 600, 5), (900, 30, 16), (90_000, 300, 3), (80_000, 9, 1)]:
         grad = torch.randn(count, dim, generator=g, device="cuda").to(grad_type)
         index = _index(g, count, rows, itype, 3.0)
         got = gb.embedding_backward(grad, index, torch.empty(rows, dim, dtype=table_type, device="cuda"), scale=1.5)
@@ -169,10 +170,11 @@ def test_gradient_of_one_row_that_has_nearly_all(cuda_device, count, dim):
     _check_gradient(got, grad, index, 9, 1.0)
 
 
-@pytest.mark.parametrize("count,rows", [(500, 64), (500, 63), (30_000, 4096), (30_000, 9000)])
-def test_gradient_drops_padding_and_out_of_range(cuda_device, count, rows):
+@pytest.mark.parametrize("dim", [3, 6])
+@pytest.mark.parametrize("count,rows", [(500, 64), (500, 63), (30_000, 4096), (30_000, 9000), (90_000, 500)])
+def test_gradient_drops_padding_and_out_of_range(cuda_device, count, rows, dim):
     g = _gen(8)
-    grad = torch.randn(count, 6, generator=g, device="cuda")
+    grad = torch.randn(count, dim, generator=g, device="cuda")
     index = _index(g, count, rows, torch.int64)
     index[::5] = 7
     index[3::11] = rows + 2
@@ -180,7 +182,7 @@ def test_gradient_drops_padding_and_out_of_range(cuda_device, count, rows):
     used = (index != 7) & (index >= 0) & (index < rows)
     grad[~used] = float("nan")  # nothing of a dropped row may be seen
     bad = torch.zeros(1, dtype=torch.int32, device="cuda")
-    got = gb.embedding_backward(grad, index, torch.empty(rows, 6, device="cuda"), padding_row=7, bad=bad)
+    got = gb.embedding_backward(grad, index, torch.empty(rows, dim, device="cuda"), padding_row=7, bad=bad)
     assert int(bad) == 1
     _check_gradient(got, grad, index, rows, 1.0, drop=7)
     bad.zero_()
@@ -193,13 +195,13 @@ def test_gradient_drops_padding_and_out_of_range(cuda_device, count, rows):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("dim", [8, 21, 600])
-def test_gradient_strided(cuda_device, dtype, dim):
+@pytest.mark.parametrize("dim,count", [(8, 10_000), (21, 10_000), (600, 10_000), (3, 100_000)])
+def test_gradient_strided(cuda_device, dtype, dim, count):
     g = _gen(9)
     for offset in (0, 1):
-        wide = torch.randn(10_000, dim + 8, generator=g, device="cuda").to(dtype)
+        wide = torch.randn(count, dim + 8, generator=g, device="cuda").to(dtype)
         grad = wide[:, offset:offset + dim]
-        index = _index(g, 10_000, 77, torch.int32)
+        index = _index(g, count, 77, torch.int32)
         buf = torch.full((77, dim + 16), 3.0, dtype=dtype, device="cuda")
         got = gb.embedding_backward(grad, index, buf[:, offset:offset + dim])
         _check_gradient(got, grad, index, 77, 1.0)
