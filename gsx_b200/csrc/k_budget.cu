@@ -14,11 +14,14 @@
  */
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <cooperative_groups.h>
 
 #include "../../include/gsx_b200.h"
 #include "gsx_b200_kernels.cuh"
 
 int gsx_internal_fail(int code, const char *msg);
+
+namespace cg = cooperative_groups;
 
 namespace {
 
@@ -49,10 +52,26 @@ __device__ __forceinline__ uint32_t length_of(const int32_t *__restrict__ length
 /* ------------------------------------------------------------------------------------------ */
 /* accumulate */
 
-/* A CTA owns kThreads / RG * VW columns of one group; RG threads share a column's rows (row r goes to thread
- * r mod RG) and are joined in shared memory in their order. */
+constexpr int kAccumulateCtas = 4; /* an SM */
+
+/* U rows, hop elements apart, all in flight before the first is added */
+template <typename T, int VW, int U>
+__device__ __forceinline__ void add_rows(float (&acc)[VW], const T *__restrict__ w, uint64_t hop)
+{
+    Pack<T, VW> x[U];
+#pragma unroll
+    for(int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const Pack<T, VW> *>(w + u * hop);
+#pragma unroll
+    for(int u = 0; u < U; ++u)
+#pragma unroll
+        for(int v = 0; v < VW; ++v) acc[v] += to_f32(x[u].v[v]);
+}
+
+/* A cluster of CTAs owns kThreads / RG * VW columns of one group and deals their rows out: row r goes to CTA
+ * (r / RG) mod clusters, thread row r mod RG.  A thread keeps U rows in flight; the RG threads of a column are joined in
+ * shared memory, the CTAs in distributed shared memory, each in a fixed order. */
 template <typename T, int VW, int RG>
-__global__ void __launch_bounds__(kThreads) accumulate_kernel(const float *score, uint64_t score_stride,
+__global__ void __launch_bounds__(kThreads, kAccumulateCtas) accumulate_kernel(const float *score, uint64_t score_stride,
                                                               const T *__restrict__ weights, uint64_t group_stride,
                                                               uint64_t row_stride, uint32_t groups, uint32_t rows,
                                                               uint32_t length, const int32_t *__restrict__ lengths,
@@ -60,44 +79,64 @@ __global__ void __launch_bounds__(kThreads) accumulate_kernel(const float *score
                                                               float *out, uint64_t out_stride)
 {
     constexpr int CT = kThreads / RG;
-    constexpr int U = VW >= 8 ? 4 : 8;
-    __shared__ float s_part[RG > 1 ? RG * CT * VW : 1];
+    constexpr int U = VW == 1 && sizeof(T) == 2 ? 16 : 8;
+    __shared__ float s_part[RG * CT * VW];
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t splits = cluster.num_blocks(), split = cluster.block_rank();
     const int ct = threadIdx.x % CT, rg = threadIdx.x / CT;
+    const uint32_t step = RG * splits, j = (blockIdx.x / splits * (uint32_t)CT + (uint32_t)ct) * VW;
     for(uint32_t g = blockIdx.y; g < groups; g += gridDim.y) {
         const uint32_t n = length_of(lengths, g, length);
         const uint32_t nr = length_of(row_lengths, g, rows);
-        const uint32_t j = (blockIdx.x * (uint32_t)CT + (uint32_t)ct) * VW;
         float acc[VW] = {};
         if(j < n) {
-            const T *w = weights + (uint64_t)g * group_stride + j;
-            uint32_t r = (uint32_t)rg;
-            for(; r + (U - 1) * RG < nr; r += U * RG) {
-                Pack<T, VW> x[U];
-#pragma unroll
-                for(int u = 0; u < U; ++u)
-                    x[u] = *reinterpret_cast<const Pack<T, VW> *>(w + (uint64_t)(r + u * RG) * row_stride);
-#pragma unroll
-                for(int u = 0; u < U; ++u)
-#pragma unroll
-                    for(int v = 0; v < VW; ++v) acc[v] += to_f32(x[u].v[v]);
+            const T *w = weights + (uint64_t)g * group_stride + j + (uint64_t)(split * RG + (uint32_t)rg) * row_stride;
+            const uint64_t hop = (uint64_t)step * row_stride;
+            /* rows of this thread */
+            int left = nr > split * RG + (uint32_t)rg ? (int)((nr - split * RG - (uint32_t)rg + step - 1) / step) : 0;
+            for(; left >= U; left -= U, w += U * hop) add_rows<T, VW, U>(acc, w, hop);
+            if(U > 8 && left >= 8) {
+                add_rows<T, VW, 8>(acc, w, hop);
+                left -= 8;
+                w += 8 * hop;
             }
-            for(; r < nr; r += RG) {
-                const Pack<T, VW> x = *reinterpret_cast<const Pack<T, VW> *>(w + (uint64_t)r * row_stride);
-#pragma unroll
-                for(int v = 0; v < VW; ++v) acc[v] += to_f32(x.v[v]);
+            if(left >= 4) {
+                add_rows<T, VW, 4>(acc, w, hop);
+                left -= 4;
+                w += 4 * hop;
             }
+            if(left >= 2) {
+                add_rows<T, VW, 2>(acc, w, hop);
+                left -= 2;
+                w += 2 * hop;
+            }
+            if(left) add_rows<T, VW, 1>(acc, w, hop);
         }
-        if(RG > 1) {
+        if(RG > 1 || splits > 1) {
             __syncthreads();
 #pragma unroll
             for(int v = 0; v < VW; ++v) s_part[(rg * VW + v) * CT + ct] = acc[v];
             __syncthreads();
-            if(rg == 0)
+            if(rg == 0) {
                 for(int k = 1; k < RG; ++k)
 #pragma unroll
                     for(int v = 0; v < VW; ++v) acc[v] += s_part[(k * VW + v) * CT + ct];
+                if(splits > 1)
+#pragma unroll
+                    for(int v = 0; v < VW; ++v) s_part[v * CT + ct] = acc[v];
+            }
         }
-        if(rg != 0) continue;
+        if(splits > 1) {
+            cluster.sync();
+            if(split == 0 && rg == 0)
+                for(uint32_t k = 1; k < splits; ++k) {
+                    const float *other = cluster.map_shared_rank(s_part, k);
+#pragma unroll
+                    for(int v = 0; v < VW; ++v) acc[v] += other[v * CT + ct];
+                }
+            cluster.sync();
+        }
+        if(split != 0 || rg != 0) continue;
         const float *in = score + (uint64_t)g * score_stride;
         float *to = out + (uint64_t)g * out_stride;
 #pragma unroll
@@ -109,27 +148,53 @@ __global__ void __launch_bounds__(kThreads) accumulate_kernel(const float *score
     }
 }
 
+template <typename T, int VW, int RG>
+cudaError_t launch_accumulate_rg(const float *score, uint64_t score_stride, const T *weights, uint64_t group_stride,
+                                 uint64_t row_stride, uint32_t groups, uint32_t rows, uint32_t length,
+                                 const int32_t *lengths, const int32_t *row_lengths, float decay, float *out,
+                                 uint64_t out_stride, cudaStream_t stream)
+{
+    constexpr uint32_t cols = kThreads / RG * VW;
+    const uint32_t blocks = (length + cols - 1) / cols, gy = groups < 65535u ? groups : 65535u;
+    /* split the rows further while the GPU is not full and a split keeps at least two rows a thread */
+    uint32_t splits = 1;
+    while(splits < 8 && (uint64_t)blocks * gy * splits * 2 <= 148 * kAccumulateCtas && rows >= splits * 2 * RG * 2) splits *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks * splits, gy);
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = splits;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, accumulate_kernel<T, VW, RG>, score, score_stride, weights, group_stride, row_stride, groups,
+                              rows, length, lengths, row_lengths, decay, out, out_stride);
+}
+
 template <typename T, int VW>
-void launch_accumulate(const float *score, uint64_t score_stride, const void *weights, uint64_t group_stride,
-                       uint64_t row_stride, uint32_t groups, uint32_t rows, uint32_t length, const int32_t *lengths,
-                       const int32_t *row_lengths, float decay, float *out, uint64_t out_stride, cudaStream_t stream)
+cudaError_t launch_accumulate(const float *score, uint64_t score_stride, const void *weights, uint64_t group_stride,
+                              uint64_t row_stride, uint32_t groups, uint32_t rows, uint32_t length, const int32_t *lengths,
+                              const int32_t *row_lengths, float decay, float *out, uint64_t out_stride, cudaStream_t stream)
 {
     const T *w = static_cast<const T *>(weights);
-    const unsigned gy = groups < 65535u ? groups : 65535u;
-    auto blocks = [&](int rg) { return dim3((length + (kThreads / rg) * VW - 1) / ((kThreads / rg) * VW), gy); };
-    if(rows >= 64)
-        accumulate_kernel<T, VW, 8><<<blocks(8), kThreads, 0, stream>>>(score, score_stride, w, group_stride, row_stride, groups, rows,
-                                                                        length, lengths, row_lengths, decay, out, out_stride);
-    else
-        accumulate_kernel<T, VW, 1><<<blocks(1), kThreads, 0, stream>>>(score, score_stride, w, group_stride, row_stride, groups, rows,
-                                                                        length, lengths, row_lengths, decay, out, out_stride);
+    /* many rows: fewer columns to a CTA, whose threads share them (512 bytes of a row a CTA where it reads packs) */
+    constexpr int RG = VW > 1 ? 8 : 2;
+    if(rows >= 32)
+        return launch_accumulate_rg<T, VW, RG>(score, score_stride, w, group_stride, row_stride, groups, rows, length, lengths,
+                                               row_lengths, decay, out, out_stride, stream);
+    return launch_accumulate_rg<T, VW, 1>(score, score_stride, w, group_stride, row_stride, groups, rows, length, lengths,
+                                          row_lengths, decay, out, out_stride, stream);
 }
 
 /* ------------------------------------------------------------------------------------------ */
 /* select */
 
 constexpr int kCtaThreads = 1024;
-constexpr uint32_t kCtaKeys = 49152; /* 192 KB of keys */
+constexpr uint32_t kCtaKeys = 49152;             /* 192 KB of keys */
+constexpr uint32_t kClusterKeys = 8 * kCtaKeys; /* of the eight CTAs of a cluster */
 constexpr int kBins = 2048;
 constexpr int kPasses = 3;
 __device__ constexpr int kShift[kPasses] = { 21, 10, 0 };
@@ -166,7 +231,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *s_warp, uin
 }
 
 /* The bin, from the top, in which the need-th largest element lies: s_out[0] = bin, s_out[1] = how many of the
- * bin's elements are still needed.  need >= 1 and at most the sum of the bins.  A block of kBins / PER threads. */
+ * bin's elements are still needed, s_out[2] = whether that is all of them.  need >= 1 and at most the sum of the bins.  A block of kBins / PER threads. */
 template <int PER, typename H>
 __device__ __forceinline__ void find_bin(const H &hist, uint32_t need, uint32_t *s_warp, uint32_t *s_out)
 {
@@ -183,6 +248,7 @@ __device__ __forceinline__ void find_bin(const H &hist, uint32_t need, uint32_t 
         if(above < need && above + c[k] >= need) {
             s_out[0] = (uint32_t)(top - k);
             s_out[1] = need - above;
+            s_out[2] = need - above == c[k];
         }
         above += c[k];
     }
@@ -206,107 +272,160 @@ __device__ __forceinline__ bool is_protected(const Select &a, uint32_t n, uint32
     return j < a.first || j >= n - a.recent;
 }
 
-/* Ordered compaction of [begin, end): entries above the threshold (or protected) and the first `need` equal ones go
- * to keep, the others to drop.  gt0 / eq0: entries above / equal before `begin`.  get(j) gives 1 for above, 0 for
- * equal, -1 for below.  Each warp takes a contiguous share. */
-template <typename Get>
-__device__ __forceinline__ void compact(const Select &a, uint32_t g, uint32_t begin, uint32_t end, uint32_t gt0,
-                                        uint32_t eq0, uint32_t need, const Get &get, uint32_t *s_warp)
+/* 1 for an entry that stays, 0 for one equal to the threshold, -1 for one below */
+__device__ __forceinline__ int place_of(const Select &a, uint32_t n, uint32_t j, uint32_t key, uint32_t t)
 {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const uint32_t span = end - begin;
-    const uint32_t share = ((span + warps - 1) / warps + 31) / 32 * 32;
-    const uint32_t w0 = begin + (share * warp < span ? share * warp : span);
-    const uint32_t w1 = end - w0 < share ? end : w0 + share;
-    uint32_t gt = 0, eq = 0;
-    for(uint32_t j0 = w0; j0 < w1; j0 += 32) {
-        const int t = j0 + lane < w1 ? get(j0 + lane) : -1;
-        gt += __popc(__ballot_sync(0xffffffffu, t > 0));
-        eq += __popc(__ballot_sync(0xffffffffu, t == 0));
-    }
-    __syncthreads();
-    if(lane == 0) {
-        s_warp[warp] = gt;
-        s_warp[32 + warp] = eq;
-    }
-    __syncthreads();
-    gt = gt0;
-    eq = eq0;
-    for(int w = 0; w < warp; ++w) {
-        gt += s_warp[w];
-        eq += s_warp[32 + w];
-    }
+    return is_protected(a, n, j) || key > t ? 1 : key == t ? 0 : -1;
+}
+
+/* Ordered compaction of [begin, end): entries above the threshold (or protected) and the first `need` equal ones go
+ * to keep, the others to drop.  gt0 / eq0: entries above / equal before `begin`.  load(j, key) gives the keys of four
+ * consecutive entries, of which those behind `end` are not looked at. */
+template <typename Load>
+__device__ __forceinline__ void compact(const Select &a, uint32_t g, uint32_t n, uint32_t begin, uint32_t end, uint32_t gt0,
+                                        uint32_t eq0, uint32_t t, uint32_t need, const Load &load, uint32_t *s_warp)
+{
     int32_t *keep = a.keep + (uint64_t)g * a.keep_stride;
     int32_t *drop = a.drop != nullptr ? a.drop + (uint64_t)g * a.drop_stride : nullptr;
-    const unsigned lt = (1u << lane) - 1u;
-    for(uint32_t j0 = w0; j0 < w1; j0 += 32) {
-        const uint32_t j = j0 + lane;
-        const int t = j < w1 ? get(j) : -1;
-        const unsigned bg = __ballot_sync(0xffffffffu, t > 0), be = __ballot_sync(0xffffffffu, t == 0);
-        const uint32_t g_before = gt + __popc(bg & lt), e_before = eq + __popc(be & lt);
-        const uint32_t kept_before = g_before + (e_before < need ? e_before : need);
-        if(j < w1) {
-            if(t > 0 || (t == 0 && e_before < need)) keep[kept_before] = (int32_t)j;
-            else if(drop != nullptr) drop[j - kept_before] = (int32_t)j;
+    for(uint32_t base = begin; base < end; base += blockDim.x * 4) {
+        const uint32_t j0 = base + threadIdx.x * 4;
+        uint32_t key[4];
+        int at[4];
+        uint32_t sum = 0; /* above | equal << 16 */
+        load(j0, key);
+#pragma unroll
+        for(int k = 0; k < 4; ++k) {
+            at[k] = j0 + k < end ? place_of(a, n, j0 + k, key[k], t) : -1;
+            sum += at[k] > 0 ? 1u : at[k] == 0 ? 0x10000u : 0u;
         }
-        gt += __popc(bg);
-        eq += __popc(be);
+        uint32_t all;
+        const uint32_t before = block_scan(sum, s_warp, &all) - sum;
+        uint32_t gt = gt0 + (before & 0xffffu), eq = eq0 + (before >> 16);
+#pragma unroll
+        for(int k = 0; k < 4; ++k)
+            if(j0 + k < end) {
+                const uint32_t kept_before = gt + (eq < need ? eq : need);
+                if(at[k] > 0 || (at[k] == 0 && eq < need)) keep[kept_before] = (int32_t)(j0 + k);
+                else if(drop != nullptr) drop[j0 + k - kept_before] = (int32_t)(j0 + k);
+                gt += at[k] > 0;
+                eq += at[k] == 0;
+            }
+        gt0 += all & 0xffffu;
+        eq0 += all >> 16;
     }
 }
 
-/* one CTA per group, keys in shared memory */
-__global__ void __launch_bounds__(kCtaThreads) select_cta_kernel(const Select a)
+/* Groups of up to kClusterKeys entries: a cluster of CTAs a group, each with its part of the keys in shared memory.
+ * The first CTA adds up the histograms (integer atomics on distributed shared memory) and finds the bins. */
+__global__ void __launch_bounds__(kCtaThreads) select_cluster_kernel(const Select a)
 {
     extern __shared__ __align__(16) uint32_t s_keys[];
     __shared__ uint32_t s_hist[kBins];
-    __shared__ uint32_t s_warp[64];
-    __shared__ uint32_t s_found[2];
-    for(uint32_t g = blockIdx.x; g < a.groups; g += gridDim.x) {
-        const uint32_t n = length_of(a.lengths, g, a.length);
-        const float *score = a.score + (uint64_t)g * a.score_stride;
-        if(threadIdx.x == 0) a.kept[g] = (int32_t)(n < a.budget ? n : a.budget);
-        if(n <= a.budget) {
-            for(uint32_t j = threadIdx.x; j < n; j += kCtaThreads) a.keep[(uint64_t)g * a.keep_stride + j] = (int32_t)j;
-            continue;
-        }
-        __syncthreads(); /* the previous group's readers of s_keys are done */
-        for(uint32_t j = threadIdx.x; j < n; j += kCtaThreads) s_keys[j] = key_of(score[j]);
-        uint32_t need = a.budget - a.first - a.recent, prefix = 0;
-        for(int p = 0; p < kPasses && need > 0; ++p) {
-            for(int b = threadIdx.x; b < kBins; b += kCtaThreads) s_hist[b] = 0u;
-            __syncthreads();
-            const int shift = kShift[p], bits = kPassBits[p];
-            for(uint32_t j = a.first + threadIdx.x; j < n - a.recent; j += kCtaThreads) {
-                const uint32_t k = s_keys[j];
-                if(p == 0 || k >> (shift + bits) == prefix) atomicAdd(&s_hist[k >> shift & ((1u << bits) - 1u)], 1u);
-            }
-            __syncthreads();
-            find_bin<kBins / kCtaThreads>([&](int b) { return s_hist[b]; }, need, s_warp, s_found);
-            prefix = prefix << bits | s_found[0];
-            need = s_found[1];
-            __syncthreads();
-        }
-        const uint32_t t = need > 0 ? prefix : 0xffffffffu; /* no key reaches 0xffffffff */
-        __syncthreads();
-        compact(a, g, 0u, n, 0u, 0u, need,
-                [&](uint32_t j) {
-                    const uint32_t k = s_keys[j];
-                    return is_protected(a, n, j) || k > t ? 1 : k == t ? 0 : -1;
-                },
-                s_warp);
+    __shared__ uint32_t s_warp[32];
+    __shared__ uint32_t s_found[3]; /* bin, how many of it are needed, whether that is all of them */
+    __shared__ uint32_t s_counts;   /* this CTA's entries above | equal << 16 */
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t ctas = cluster.num_blocks(), rank = cluster.block_rank(), g = blockIdx.x / ctas;
+    const uint32_t n = length_of(a.lengths, g, a.length);
+    const uint32_t seg = ((n + ctas - 1) / ctas + 3u) / 4u * 4u;
+    const uint32_t begin = seg * rank < n ? seg * rank : n, end = n - begin < seg ? n : begin + seg;
+    const float *score = a.score + (uint64_t)g * a.score_stride;
+    if(rank == 0 && threadIdx.x == 0) a.kept[g] = (int32_t)(n < a.budget ? n : a.budget);
+    if(n <= a.budget) {
+        for(uint32_t j = begin + threadIdx.x; j < end; j += kCtaThreads) a.keep[(uint64_t)g * a.keep_stride + j] = (int32_t)j;
+        return;
     }
+    for(uint32_t j0 = begin + threadIdx.x; j0 < end; j0 += kCtaThreads * 4) {
+        float x[4];
+#pragma unroll
+        for(int k = 0; k < 4; ++k)
+            if(j0 + k * kCtaThreads < end) x[k] = __ldg(score + j0 + k * kCtaThreads);
+#pragma unroll
+        for(int k = 0; k < 4; ++k)
+            if(j0 + k * kCtaThreads < end) s_keys[j0 + k * kCtaThreads - begin] = key_of(x[k]);
+    }
+    uint32_t need = a.budget - a.first - a.recent, prefix = 0;
+    uint32_t t = 0xffffffffu; /* no key reaches 0xffffffff */
+    const uint32_t from = begin > a.first ? begin : a.first, to = end < n - a.recent ? end : n - a.recent;
+    for(int p = 0; p < kPasses && need > 0; ++p) {
+        for(int b = threadIdx.x; b < kBins; b += kCtaThreads) s_hist[b] = 0u;
+        __syncthreads();
+        const int shift = kShift[p], bits = kPassBits[p];
+        for(uint32_t j = from + threadIdx.x; j < to; j += kCtaThreads) {
+            const uint32_t k = s_keys[j - begin];
+            if(p == 0 || k >> (shift + bits) == prefix) atomicAdd(&s_hist[k >> shift & ((1u << bits) - 1u)], 1u);
+        }
+        __syncthreads();
+        if(ctas > 1) {
+            cluster.sync();
+            if(rank != 0) {
+                uint32_t *hist0 = cluster.map_shared_rank(s_hist, 0);
+                for(int b = threadIdx.x; b < kBins; b += kCtaThreads)
+                    if(s_hist[b]) atomicAdd(hist0 + b, s_hist[b]);
+            }
+            cluster.sync();
+        }
+        if(rank == 0) {
+            find_bin<kBins / kCtaThreads>([&](int b) { return s_hist[b]; }, need, s_warp, s_found);
+            if(ctas > 1 && threadIdx.x > 0 && threadIdx.x < ctas) {
+                uint32_t *other = cluster.map_shared_rank(s_found, threadIdx.x);
+                other[0] = s_found[0];
+                other[1] = s_found[1];
+                other[2] = s_found[2];
+            }
+        }
+        if(ctas > 1) cluster.sync();
+        prefix = prefix << bits | s_found[0];
+        need = s_found[1];
+        t = prefix << shift;
+        if(s_found[2] && t > 0) { /* all of the bin stay: the rest of its bits does not matter */
+            --t;
+            need = 0;
+        }
+        __syncthreads();
+    }
+    __syncthreads();
+    uint32_t gt0 = 0, eq0 = 0;
+    if(ctas > 1) {
+        uint32_t gt = 0, eq = 0;
+        for(uint32_t j = begin + threadIdx.x; j < end; j += kCtaThreads) {
+            const int at = place_of(a, n, j, s_keys[j - begin], t);
+            gt += at > 0;
+            eq += at == 0;
+        }
+        uint32_t all;
+        block_scan(gt | eq << 16, s_warp, &all);
+        if(threadIdx.x == 0) s_counts = all; /* each at most kCtaKeys < 65536 */
+        cluster.sync();
+        for(uint32_t k = 0; k < rank; ++k) {
+            const uint32_t c = *cluster.map_shared_rank(&s_counts, k);
+            gt0 += c & 0xffffu;
+            eq0 += c >> 16;
+        }
+        cluster.sync(); /* nobody leaves while its counts are read */
+    }
+    compact(a, g, n, begin, end, gt0, eq0, t, need,
+            [&](uint32_t j, uint32_t (&key)[4]) {
+                if(j >= end) return;
+                const uint4 v = *reinterpret_cast<const uint4 *>(s_keys + (j - begin));
+                key[0] = v.x;
+                key[1] = v.y;
+                key[2] = v.z;
+                key[3] = v.w;
+            },
+            s_warp);
 }
 
 /* Long groups.  Workspace of one group: kState words of state, kPasses * kBins of histogram (both cleared by the
  * caller), then two counts for each of the group's blocks. */
-constexpr int kState = 32; /* [0] prefix, [1] need, [8..11] tickets */
+constexpr int kState = 32; /* [0] threshold so far, [1] equals needed, [2] bits still open, [8..11] tickets */
 constexpr int kSegThreads = 512;
-constexpr uint32_t kSegLeast = 8192;
+constexpr uint32_t kSegLeast = 4096;
 
 uint32_t long_blocks(uint32_t groups, uint32_t length)
 {
     const uint32_t most = (length + kSegLeast - 1) / kSegLeast;
-    uint32_t nb = groups < 148u * 2u ? 148u * 2u / groups : 1u;
+    uint32_t nb = groups < 148u * 4u ? 148u * 4u / groups : 1u;
     if(nb > most) nb = most;
     return nb ? nb : 1u;
 }
@@ -342,29 +461,46 @@ __device__ __forceinline__ bool last_block(uint32_t *ticket)
     return s_last;
 }
 
+/* f(entry, key) for the entries [begin, end) of a group, dealt to the threads, eight loads in flight */
+template <typename F>
+__device__ __forceinline__ void for_keys(const float *__restrict__ score, uint32_t begin, uint32_t end, const F &f)
+{
+    for(uint32_t j0 = begin + threadIdx.x; j0 < end; j0 += kSegThreads * 8) {
+        float x[8];
+#pragma unroll
+        for(int k = 0; k < 8; ++k)
+            if(j0 + k * kSegThreads < end) x[k] = __ldg(score + j0 + k * kSegThreads);
+#pragma unroll
+        for(int k = 0; k < 8; ++k)
+            if(j0 + k * kSegThreads < end) f(j0 + k * kSegThreads, key_of(x[k]));
+    }
+}
+
 template <int P>
 __global__ void __launch_bounds__(kSegThreads) select_hist_kernel(const Select a, const Long w)
 {
     __shared__ uint32_t s_hist[kBins];
     __shared__ uint32_t s_warp[32];
-    __shared__ uint32_t s_found[2];
+    __shared__ uint32_t s_found[3];
     const uint32_t g = blockIdx.y;
     const uint32_t n = length_of(a.lengths, g, a.length);
     const uint32_t most = a.budget - a.first - a.recent;
-    if(n <= a.budget || most == 0) return;
-    uint32_t *state = w.state + (uint64_t)g * kState;
-    const uint32_t prefix = P > 0 ? state[0] : 0u, need = P > 0 ? state[1] : most;
     for(int b = threadIdx.x; b < kBins; b += kSegThreads) s_hist[b] = 0u;
     __syncthreads();
-    const float *score = a.score + (uint64_t)g * a.score_stride;
+    gsx_pdl_trigger();
+    gsx_pdl_wait();
+    if(n <= a.budget || most == 0) return;
+    uint32_t *state = w.state + (uint64_t)g * kState;
+    const uint32_t prefix = P > 0 ? __ldcg(state) : 0u, need = P > 0 ? __ldcg(state + 1) : most;
+    if(need == 0) return; /* the earlier bits decided */
     constexpr int shift = kShift[P], bits = kPassBits[P];
     uint32_t begin, end;
     segment(n, begin, end);
-    for(uint32_t j = begin + threadIdx.x; j < end; j += kSegThreads) {
-        if(is_protected(a, n, j)) continue;
-        const uint32_t k = key_of(__ldg(score + j));
-        if(P == 0 || k >> ((shift + bits) & 31) == prefix) atomicAdd(&s_hist[k >> shift & ((1u << bits) - 1u)], 1u);
-    }
+    if(begin < a.first) begin = a.first < end ? a.first : end;
+    if(end > n - a.recent) end = n - a.recent > begin ? n - a.recent : begin;
+    for_keys(a.score + (uint64_t)g * a.score_stride, begin, end, [&](uint32_t, uint32_t k) {
+        if(P == 0 || (k ^ prefix) >> ((shift + bits) & 31) == 0) atomicAdd(&s_hist[k >> shift & ((1u << bits) - 1u)], 1u);
+    });
     __syncthreads();
     uint32_t *hist = w.hist + ((uint64_t)g * kPasses + P) * kBins;
     for(int b = threadIdx.x; b < kBins; b += kSegThreads)
@@ -372,8 +508,13 @@ __global__ void __launch_bounds__(kSegThreads) select_hist_kernel(const Select a
     if(!last_block(&state[8 + P])) return;
     find_bin<kBins / kSegThreads>([&](int b) { return __ldcg(hist + b); }, need, s_warp, s_found);
     if(threadIdx.x == 0) {
-        state[0] = prefix << bits | s_found[0];
-        state[1] = s_found[1];
+        uint32_t t = prefix | s_found[0] << shift, left = s_found[1];
+        if(s_found[2] && t > 0) { /* all of the bin stay: the rest of its bits does not matter */
+            --t;
+            left = 0;
+        }
+        state[0] = t;
+        state[1] = left;
     }
 }
 
@@ -381,28 +522,29 @@ __global__ void __launch_bounds__(kSegThreads) select_hist_kernel(const Select a
 __device__ __forceinline__ void threshold(const Select &a, const uint32_t *state, uint32_t &t, uint32_t &need)
 {
     const bool any = a.budget > a.first + a.recent;
-    t = any ? state[0] : 0xffffffffu;
-    need = any ? state[1] : 0u;
+    t = any ? __ldcg(state) : 0xffffffffu;
+    need = any ? __ldcg(state + 1) : 0u;
 }
 
 /* per block: entries above and equal; the last block turns them into counts before each block */
 __global__ void __launch_bounds__(kSegThreads) select_count_kernel(const Select a, const Long w)
 {
     __shared__ uint32_t s_warp[32];
+    gsx_pdl_trigger();
+    gsx_pdl_wait();
     const uint32_t g = blockIdx.y;
     const uint32_t n = length_of(a.lengths, g, a.length);
     if(n <= a.budget) return;
     uint32_t *state = w.state + (uint64_t)g * kState;
     uint32_t t, need;
     threshold(a, state, t, need);
-    const float *score = a.score + (uint64_t)g * a.score_stride;
     uint32_t begin, end, gt = 0, eq = 0;
     segment(n, begin, end);
-    for(uint32_t j = begin + threadIdx.x; j < end; j += kSegThreads) {
-        const uint32_t k = key_of(__ldg(score + j));
-        if(is_protected(a, n, j) || k > t) ++gt;
-        else if(k == t) ++eq;
-    }
+    for_keys(a.score + (uint64_t)g * a.score_stride, begin, end, [&](uint32_t j, uint32_t k) {
+        const int at = place_of(a, n, j, k, t);
+        gt += at > 0;
+        eq += at == 0;
+    });
     uint32_t gts, eqs;
     block_scan(gt, s_warp, &gts);
     block_scan(eq, s_warp, &eqs);
@@ -429,7 +571,8 @@ __global__ void __launch_bounds__(kSegThreads) select_count_kernel(const Select 
 
 __global__ void __launch_bounds__(kSegThreads) select_write_kernel(const Select a, const Long w)
 {
-    __shared__ uint32_t s_warp[64];
+    __shared__ uint32_t s_warp[32];
+    gsx_pdl_wait();
     const uint32_t g = blockIdx.y;
     const uint32_t n = length_of(a.lengths, g, a.length);
     uint32_t begin, end;
@@ -443,10 +586,15 @@ __global__ void __launch_bounds__(kSegThreads) select_write_kernel(const Select 
     threshold(a, w.state + (uint64_t)g * kState, t, need);
     const uint32_t *counts = w.counts + ((uint64_t)g * gridDim.x + blockIdx.x) * 2;
     const float *score = a.score + (uint64_t)g * a.score_stride;
-    compact(a, g, begin, end, counts[0], counts[1], need,
-            [&](uint32_t j) {
-                const uint32_t k = key_of(__ldg(score + j));
-                return is_protected(a, n, j) || k > t ? 1 : k == t ? 0 : -1;
+    compact(a, g, n, begin, end, __ldcg(counts), __ldcg(counts + 1), t, need,
+            [&](uint32_t j, uint32_t (&key)[4]) {
+                float x[4];
+#pragma unroll
+                for(int k = 0; k < 4; ++k)
+                    if(j + k < end) x[k] = __ldg(score + j + k);
+#pragma unroll
+                for(int k = 0; k < 4; ++k)
+                    if(j + k < end) key[k] = key_of(x[k]);
             },
             s_warp);
 }
@@ -457,65 +605,184 @@ __global__ void __launch_bounds__(kSegThreads) select_write_kernel(const Select 
 struct Field {
     const unsigned char *src;
     unsigned char *dst;
-    uint64_t src_outer, src_inner, src_row, dst_outer, dst_inner, dst_row; /* bytes */
-    uint32_t row_bytes, unit, rows_per_block, first_block;
+    uint64_t src_outer, src_inner, dst_outer, dst_inner; /* bytes */
+    uint32_t src_row, dst_row, row_bytes;
+    uint32_t unit; /* bytes of an access, or 100 + the words of a short row */
+    uint32_t first_block;
+    uint32_t div_mul, div_shift; /* of the division by row_bytes / unit */
 };
 struct Fields {
     Field f[GSX_B200_GATHER_MAX_FIELDS];
     int count;
 };
-constexpr uint32_t kGatherBytes = 16384; /* of output per CTA */
 
-template <typename W>
-__device__ __forceinline__ void gather_tile(const Field &f, const unsigned char *src, unsigned char *dst,
-                                            const int32_t *__restrict__ keep, uint32_t r0, uint32_t rows, uint32_t length,
-                                            uint32_t *bad)
+/* i / per_row for i < 2^31 by one multiplication (division by an invariant, Granlund and Montgomery 1994):
+ * with 2^s >= d and m = floor(2^(31 + s) / d) + 1, i / d = i * m >> (31 + s) */
+__device__ __forceinline__ uint32_t divide(uint32_t i, uint32_t mul, uint32_t shift)
 {
-    const uint32_t per_row = f.row_bytes / (uint32_t)sizeof(W);
-    const uint32_t total = rows * per_row;
-    for(uint32_t i = threadIdx.x; i < total; i += kThreads) {
-        const uint32_t r = i / per_row, k = i - r * per_row;
-        const int32_t s = __ldg(keep + r0 + r);
-        if(s < 0 || (uint32_t)s >= length) {
-            if(bad != nullptr && k == 0) atomicExch(bad, 1u);
-            continue;
-        }
-        reinterpret_cast<W *>(dst + (uint64_t)(r0 + r) * f.dst_row)[k] =
-            __ldg(reinterpret_cast<const W *>(src + (uint64_t)s * f.src_row) + k);
-    }
+    return shift ? __umulhi(i, mul) >> (shift - 1) : i;
 }
 
-__global__ void __launch_bounds__(kThreads) budget_gather_kernel(const __grid_constant__ Fields fields, uint32_t groups,
-                                                                 uint32_t inner, uint32_t length, uint32_t budget,
-                                                                 const int32_t *__restrict__ keep, uint64_t keep_stride,
-                                                                 const int32_t *__restrict__ kept,
-                                                                 uint32_t *__restrict__ bad)
+/* What a CTA needs of a field and group.  The gathers below are functions of their own (not inlined), so that the widest
+ * does not take registers from the others. */
+struct Part {
+    const unsigned char *src;
+    unsigned char *dst;
+    uint32_t src_row, dst_row, row_bytes, div_mul, div_shift;
+};
+
+/* A row that is not there is read in the place of row 0 and not stored: a load under a condition becomes a branch. */
+
+/* row (of a list of n) that the list names, or UINT32_MAX for none; a name outside [0, length) sets outside */
+__device__ __forceinline__ uint32_t named(uint32_t s, uint32_t r, uint32_t n, uint32_t length, bool &outside)
 {
+    if(r >= n) return UINT32_MAX;
+    outside |= s >= length;
+    return s < length ? s : UINT32_MAX;
+}
+
+/* A CTA's part of one field: accesses [first, first + kThreads * U) of a W each, all of a thread's in flight at once.
+ * The list is read before its length is known (its places behind the length are not used). */
+template <typename W, int U>
+__device__ __noinline__ bool gather_part(const Part a, uint32_t part, const int32_t *__restrict__ keep,
+                                         const int32_t *__restrict__ kept, uint32_t budget, uint32_t length)
+{
+    const unsigned char *__restrict__ src = a.src;
+    unsigned char *__restrict__ dst = a.dst;
+    const uint32_t per_row = a.row_bytes / (uint32_t)sizeof(W), src_row = a.src_row, dst_row = a.dst_row;
+    const uint64_t first = (uint64_t)part * (kThreads * U);
+    /* the part's first row, and accesses counted from the start of that */
+    const uint32_t row0 = (uint32_t)(first / per_row), i0 = (uint32_t)(first - (uint64_t)row0 * per_row) + threadIdx.x;
+    const uint32_t r0 = row0 + divide(i0, a.div_mul, a.div_shift), c0 = i0 - (r0 - row0) * per_row;
+    const uint32_t dr = divide(kThreads, a.div_mul, a.div_shift), dc = kThreads - dr * per_row;
+    auto next = [&](uint32_t &r, uint32_t &c) { /* the access kThreads further on */
+        r += dr;
+        c += dc;
+        if(c >= per_row) {
+            c -= per_row;
+            ++r;
+        }
+    };
+    uint32_t s[U], r = r0, c = c0;
+    W x[U];
+#pragma unroll
+    for(int u = 0; u < U; ++u, next(r, c)) s[u] = r < budget ? (uint32_t)__ldg(keep + r) : UINT32_MAX;
+    const uint32_t n = length_of(kept, 0, budget);
+    if(row0 >= n) return false;
+    bool outside = false;
+    r = r0;
+    c = c0;
+#pragma unroll
+    for(int u = 0; u < U; ++u, next(r, c)) {
+        s[u] = named(s[u], r, n, length, outside);
+        x[u] = __ldg(reinterpret_cast<const W *>(src + (uint64_t)(s[u] != UINT32_MAX ? s[u] : 0u) * src_row) + c);
+    }
+    r = r0;
+    c = c0;
+#pragma unroll
+    for(int u = 0; u < U; ++u, next(r, c))
+        if(s[u] != UINT32_MAX) reinterpret_cast<W *>(dst + (uint64_t)r * dst_row)[c] = x[u];
+    return outside;
+}
+
+/* Short rows of WORDS 4-byte words into a contiguous, 16-byte aligned dst: a thread reads whole rows, shared memory
+ * turns them into 16-byte stores (a word an access took 59 instructions a word, this takes about six). */
+constexpr int kShortRows = 1024; /* rows of a CTA */
+constexpr uint32_t kShortWords = 8;
+template <int WORDS>
+__device__ __noinline__ bool gather_short(const Part a, uint32_t part, const int32_t *__restrict__ keep,
+                                          const int32_t *__restrict__ kept, uint32_t budget, uint32_t length,
+                                          uint32_t *s_tile)
+{
+    constexpr int U = kShortRows / kThreads;
+    const unsigned char *__restrict__ src = a.src;
+    const uint32_t row0 = part * kShortRows;
+    uint32_t s[U], x[U][WORDS];
+#pragma unroll
+    for(int u = 0; u < U; ++u) {
+        const uint32_t r = row0 + threadIdx.x + u * kThreads;
+        s[u] = r < budget ? (uint32_t)__ldg(keep + r) : UINT32_MAX;
+    }
+    const uint32_t n = length_of(kept, 0, budget), src_row = a.src_row;
+    if(row0 >= n) return false;
+    bool outside = false;
+#pragma unroll
+    for(int u = 0; u < U; ++u) {
+        s[u] = named(s[u], row0 + threadIdx.x + u * kThreads, n, length, outside);
+        const uint32_t *from = reinterpret_cast<const uint32_t *>(src + (uint64_t)(s[u] != UINT32_MAX ? s[u] : 0u) * src_row);
+#pragma unroll
+        for(int w = 0; w < WORDS; ++w) x[u][w] = __ldg(from + w);
+    }
+    uint32_t *to = reinterpret_cast<uint32_t *>(a.dst) + (uint64_t)row0 * WORDS;
+    if(__syncthreads_or(outside)) { /* some rows stay as they were */
+#pragma unroll
+        for(int u = 0; u < U; ++u)
+            if(s[u] != UINT32_MAX)
+#pragma unroll
+                for(int w = 0; w < WORDS; ++w) to[(threadIdx.x + u * kThreads) * WORDS + w] = x[u][w];
+        return outside;
+    }
+#pragma unroll
+    for(int u = 0; u < U; ++u)
+#pragma unroll
+        for(int w = 0; w < WORDS; ++w) s_tile[(threadIdx.x + u * kThreads) * WORDS + w] = x[u][w];
+    __syncthreads();
+    const uint32_t words = (n - row0 < (uint32_t)kShortRows ? n - row0 : (uint32_t)kShortRows) * WORDS;
+    for(uint32_t i = threadIdx.x; i < words / 4; i += kThreads)
+        reinterpret_cast<uint4 *>(to)[i] = reinterpret_cast<const uint4 *>(s_tile)[i];
+    if(threadIdx.x < words % 4) to[words / 4 * 4 + threadIdx.x] = s_tile[words / 4 * 4 + threadIdx.x];
+    __syncthreads();
+    return false;
+}
+
+/* accesses of a thread by their size: 16 KB of output a CTA in whole packs, less where rows need narrower accesses */
+__host__ __device__ constexpr uint32_t gather_accesses(uint32_t unit) { return unit == 16 ? 4u : 8u; }
+
+__global__ void __launch_bounds__(kThreads, 4) budget_gather_kernel(const __grid_constant__ Fields fields, uint32_t groups,
+                                                                    uint32_t inner, uint32_t length, uint32_t budget,
+                                                                    const int32_t *__restrict__ keep, uint64_t keep_stride,
+                                                                    const int32_t *__restrict__ kept,
+                                                                    uint32_t *__restrict__ bad)
+{
+    __shared__ __align__(16) uint32_t s_tile[kShortRows * kShortWords];
+    if(length == 0) { /* no row to name */
+        for(uint32_t g = blockIdx.y; g < groups; g += gridDim.y)
+            if(bad != nullptr && threadIdx.x == 0 && length_of(kept, g, budget) > 0) atomicExch(bad, 1u);
+        return;
+    }
     int k = 0;
     while(k + 1 < fields.count && blockIdx.x >= fields.f[k + 1].first_block) ++k;
     const Field &f = fields.f[k];
-    const uint32_t r0 = (blockIdx.x - f.first_block) * f.rows_per_block;
+    const uint32_t part = blockIdx.x - f.first_block;
     for(uint32_t g = blockIdx.y; g < groups; g += gridDim.y) {
-        const uint32_t n = length_of(kept, g, budget);
-        if(r0 >= n) continue;
-        const uint32_t rows = n - r0 < f.rows_per_block ? n - r0 : f.rows_per_block;
-        const uint64_t o = g / inner, i = g - (uint32_t)o * inner;
-        const unsigned char *src = f.src + o * f.src_outer + i * f.src_inner;
-        unsigned char *dst = f.dst + o * f.dst_outer + i * f.dst_inner;
+        const uint32_t o = g / inner, i = g - o * inner;
+        const Part a = { f.src + o * f.src_outer + i * f.src_inner, f.dst + o * f.dst_outer + i * f.dst_inner, f.src_row,
+                         f.dst_row, f.row_bytes, f.div_mul, f.div_shift };
         const int32_t *list = keep + (uint64_t)g * keep_stride;
+        bool outside;
         switch(f.unit) {
-        case 16: gather_tile<uint4>(f, src, dst, list, r0, rows, length, bad); break;
-        case 8: gather_tile<uint2>(f, src, dst, list, r0, rows, length, bad); break;
-        case 4: gather_tile<uint32_t>(f, src, dst, list, r0, rows, length, bad); break;
-        case 2: gather_tile<uint16_t>(f, src, dst, list, r0, rows, length, bad); break;
-        default: gather_tile<uint8_t>(f, src, dst, list, r0, rows, length, bad); break;
+        case 101: outside = gather_short<1>(a, part, list, kept + g, budget, length, s_tile); break;
+        case 102: outside = gather_short<2>(a, part, list, kept + g, budget, length, s_tile); break;
+        case 103: outside = gather_short<3>(a, part, list, kept + g, budget, length, s_tile); break;
+        case 104: outside = gather_short<4>(a, part, list, kept + g, budget, length, s_tile); break;
+        case 105: outside = gather_short<5>(a, part, list, kept + g, budget, length, s_tile); break;
+        case 106: outside = gather_short<6>(a, part, list, kept + g, budget, length, s_tile); break;
+        case 107: outside = gather_short<7>(a, part, list, kept + g, budget, length, s_tile); break;
+        case 108: outside = gather_short<8>(a, part, list, kept + g, budget, length, s_tile); break;
+        case 16: outside = gather_part<uint4, gather_accesses(16)>(a, part, list, kept + g, budget, length); break;
+        case 8: outside = gather_part<uint2, gather_accesses(8)>(a, part, list, kept + g, budget, length); break;
+        case 4: outside = gather_part<uint32_t, gather_accesses(4)>(a, part, list, kept + g, budget, length); break;
+        case 2: outside = gather_part<uint16_t, gather_accesses(2)>(a, part, list, kept + g, budget, length); break;
+        default: outside = gather_part<uint8_t, gather_accesses(1)>(a, part, list, kept + g, budget, length); break;
         }
+        if(outside && bad != nullptr) atomicExch(bad, 1u);
     }
 }
 
-int launch_status()
+int launch_status(cudaError_t e = cudaSuccess)
 {
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t last = cudaGetLastError();
+    if(e == cudaSuccess) e = last;
     return e == cudaSuccess ? GSX_B200_SUCCESS : gsx_internal_fail(GSX_B200_UNKNOWN, cudaGetErrorString(e));
 }
 
@@ -554,9 +821,10 @@ extern "C" int gsx_b200_budget_accumulate(const float *score, uint64_t score_str
     cudaStream_t stream = (cudaStream_t)stream_;
     const bool vec = (uintptr_t)weights % 16 == 0 && (groups == 1 || group_stride * es % 16 == 0) &&
                      (rows <= 1 || row_stride * es % 16 == 0) && length * es % 16 == 0;
-#define GSX_ACCUMULATE(T, VW)                                                                                          \
-    launch_accumulate<T, VW>(score, score_stride, weights, group_stride, row_stride, (uint32_t)groups, (uint32_t)rows, \
-                             (uint32_t)length, lengths, row_lengths, decay, out, out_stride, stream)
+#define GSX_ACCUMULATE(T, VW)                                                                                              \
+    e = launch_accumulate<T, VW>(score, score_stride, weights, group_stride, row_stride, (uint32_t)groups, (uint32_t)rows, \
+                                 (uint32_t)length, lengths, row_lengths, decay, out, out_stride, stream)
+    cudaError_t e;
     if(weight_type == GSX_B200_DATA_F32) {
         if(vec) GSX_ACCUMULATE(float, 4);
         else GSX_ACCUMULATE(float, 1);
@@ -568,12 +836,12 @@ extern "C" int gsx_b200_budget_accumulate(const float *score, uint64_t score_str
         else GSX_ACCUMULATE(__nv_bfloat16, 1);
     }
 #undef GSX_ACCUMULATE
-    return launch_status();
+    return launch_status(e);
 }
 
 extern "C" uint64_t gsx_b200_budget_workspace_bytes(uint64_t groups, uint64_t length)
 {
-    if(groups == 0 || length <= kCtaKeys || groups > 65535 || length > (uint64_t)INT32_MAX) return 0;
+    if(groups == 0 || length <= kClusterKeys || groups > 65535 || length > (uint64_t)INT32_MAX) return 0;
     return 4 * long_words((uint32_t)groups, (uint32_t)length);
 }
 
@@ -584,8 +852,8 @@ extern "C" int gsx_b200_budget_select(const float *score, uint64_t score_stride,
 {
     if(groups > (uint64_t)INT32_MAX || length > (uint64_t)INT32_MAX || budget > (uint64_t)INT32_MAX)
         return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "groups, length and budget must be below 2^31");
-    if(length > kCtaKeys && groups > 65535)
-        return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "at most 65535 groups of more than 49152 entries");
+    if(groups > (length > kClusterKeys ? 65535u : 1u << 27))
+        return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "at most 65535 groups of more than 393216 entries, 2^27 of fewer");
     if(first > budget || recent > budget - first)
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "first + recent must be at most budget");
     if(groups == 0) return GSX_B200_SUCCESS;
@@ -611,11 +879,27 @@ extern "C" int gsx_b200_budget_select(const float *score, uint64_t score_stride,
     a.kept = kept;
     a.drop = drop;
     a.drop_stride = drop_stride;
-    if(length <= kCtaKeys) {
-        const cudaError_t e = cudaFuncSetAttribute(select_cta_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kCtaKeys * 4));
-        if(e != cudaSuccess) return gsx_internal_fail(GSX_B200_UNKNOWN, cudaGetErrorString(e));
-        select_cta_kernel<<<(unsigned)groups, kCtaThreads, (size_t)length * 4, stream>>>(a);
-        return launch_status();
+    if(length <= kClusterKeys) {
+        /* as many CTAs as the keys need, and more while the GPU is not full (two an SM) and a part keeps 2048 entries */
+        uint32_t ctas = 1;
+        while(ctas < 8 && (length > (uint64_t)ctas * kCtaKeys || (groups * ctas * 2 <= 148 * 2 && length >= (uint64_t)ctas * 2 * 2048)))
+            ctas *= 2;
+        const size_t part = ((length + ctas - 1) / ctas + 3) / 4 * 4;
+        cudaError_t e = cudaFuncSetAttribute(select_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kCtaKeys * 4));
+        if(e != cudaSuccess) return launch_status(e);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(groups * ctas));
+        cfg.blockDim = dim3(kCtaThreads);
+        cfg.dynamicSmemBytes = part * 4;
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = ctas;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        return launch_status(cudaLaunchKernelEx(&cfg, select_cluster_kernel, a));
     }
     const uint64_t need = gsx_b200_budget_workspace_bytes(groups, length);
     if(workspace == nullptr || (uintptr_t)workspace % 4 || workspace_bytes < need)
@@ -624,19 +908,22 @@ extern "C" int gsx_b200_budget_select(const float *score, uint64_t score_stride,
     w.state = static_cast<uint32_t *>(workspace);
     w.hist = w.state + (size_t)groups * kState;
     w.counts = w.state + long_clear_words(a.groups);
-    const cudaError_t e = cudaMemsetAsync(workspace, 0, 4 * long_clear_words(a.groups), stream);
-    if(e != cudaSuccess) return gsx_internal_fail(GSX_B200_UNKNOWN, cudaGetErrorString(e));
-    const dim3 grid(long_blocks(a.groups, a.length), a.groups);
-    if(length > budget) {
-        if(budget > first + recent) {
-            select_hist_kernel<0><<<grid, kSegThreads, 0, stream>>>(a, w);
-            select_hist_kernel<1><<<grid, kSegThreads, 0, stream>>>(a, w);
-            select_hist_kernel<2><<<grid, kSegThreads, 0, stream>>>(a, w);
-        }
-        select_count_kernel<<<grid, kSegThreads, 0, stream>>>(a, w);
+    const dim3 grid(long_blocks(a.groups, a.length), a.groups), block(kSegThreads);
+    if(length <= budget) { /* every group keeps all */
+        select_write_kernel<<<grid, block, 0, stream>>>(a, w);
+        return launch_status();
     }
-    select_write_kernel<<<grid, kSegThreads, 0, stream>>>(a, w);
-    return launch_status();
+    cudaError_t e = cudaMemsetAsync(workspace, 0, 4 * long_clear_words(a.groups), stream);
+    if(e == cudaSuccess && budget > first + recent) {
+        select_hist_kernel<0><<<grid, block, 0, stream>>>(a, w);
+        e = gsx_launch_pdl(select_hist_kernel<1>, grid, block, 0, stream, a, w);
+        if(e == cudaSuccess) e = gsx_launch_pdl(select_hist_kernel<2>, grid, block, 0, stream, a, w);
+        if(e == cudaSuccess) e = gsx_launch_pdl(select_count_kernel, grid, block, 0, stream, a, w);
+    } else if(e == cudaSuccess) {
+        select_count_kernel<<<grid, block, 0, stream>>>(a, w);
+    }
+    if(e == cudaSuccess) e = gsx_launch_pdl(select_write_kernel, grid, block, 0, stream, a, w);
+    return launch_status(e);
 }
 
 extern "C" int gsx_b200_budget_gather(const gsx_b200_gather_field *fields, int32_t field_count, uint64_t outer,
@@ -664,13 +951,13 @@ extern "C" int gsx_b200_budget_gather(const gsx_b200_gather_field *fields, int32
     for(int i = 0; i < field_count; ++i) {
         const gsx_b200_gather_field &in = fields[i];
         if(in.row_bytes == 0) continue;
-        if(in.row_bytes > (1ull << 31)) return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "rows of at most 2^31 bytes");
+        if(in.row_bytes > (1ull << 30)) return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "rows of at most 2^30 bytes");
         if(in.dst == nullptr || (length > 0 && in.src == nullptr))
             return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "field pointers must be non-null");
         const uint64_t limit = 1ull << 42;
-        if(in.src_outer_stride > limit || in.src_inner_stride > limit || in.src_row_stride > limit ||
-           in.dst_outer_stride > limit || in.dst_inner_stride > limit || in.dst_row_stride > limit)
-            return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "strides must be at most 2^42 bytes");
+        if(in.src_outer_stride > limit || in.src_inner_stride > limit || in.dst_outer_stride > limit || in.dst_inner_stride > limit ||
+           in.src_row_stride > UINT32_MAX || in.dst_row_stride > UINT32_MAX)
+            return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "group strides of at most 2^42 bytes, row strides below 2^32");
         if(budget > 1 && in.dst_row_stride < in.row_bytes)
             return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "dst_row_stride must be at least row_bytes");
         Field &f = t.f[t.count];
@@ -678,20 +965,31 @@ extern "C" int gsx_b200_budget_gather(const gsx_b200_gather_field *fields, int32
         f.dst = static_cast<unsigned char *>(in.dst);
         f.src_outer = in.src_outer_stride;
         f.src_inner = in.src_inner_stride;
-        f.src_row = in.src_row_stride;
+        f.src_row = (uint32_t)in.src_row_stride;
         f.dst_outer = in.dst_outer_stride;
         f.dst_inner = in.dst_inner_stride;
-        f.dst_row = in.dst_row_stride;
+        f.dst_row = (uint32_t)in.dst_row_stride;
         f.row_bytes = (uint32_t)in.row_bytes;
         const uint64_t all = (uint64_t)(uintptr_t)in.src | (uint64_t)(uintptr_t)in.dst | in.row_bytes | (outer > 1 ? in.src_outer_stride | in.dst_outer_stride : 0) |
                              (inner > 1 ? in.src_inner_stride | in.dst_inner_stride : 0) | in.src_row_stride | in.dst_row_stride;
         f.unit = 16;
         while(all % f.unit) f.unit /= 2;
-        f.rows_per_block = f.row_bytes >= kGatherBytes ? 1u : kGatherBytes / f.row_bytes;
+        const uint64_t per_row = f.row_bytes / f.unit;
+        f.div_shift = 0;
+        while((1ull << f.div_shift) < per_row) ++f.div_shift;
+        f.div_mul = f.div_shift ? (uint32_t)((1ull << (31 + f.div_shift)) / per_row + 1) : 0u;
         f.first_block = (uint32_t)blocks;
-        blocks += (budget + f.rows_per_block - 1) / f.rows_per_block;
-        src_span[t.count] = { in.src, length == 0 ? 0 : (outer - 1) * f.src_outer + (inner - 1) * f.src_inner + (length - 1) * f.src_row + f.row_bytes };
-        dst_span[t.count] = { in.dst, (outer - 1) * f.dst_outer + (inner - 1) * f.dst_inner + (budget - 1) * f.dst_row + f.row_bytes };
+        const uint64_t dst_all = (uint64_t)(uintptr_t)in.dst | (outer > 1 ? in.dst_outer_stride : 0) | (inner > 1 ? in.dst_inner_stride : 0);
+        uint64_t part = kThreads * gather_accesses(f.unit), accesses = budget * per_row;
+        if(f.unit < 16 && f.unit >= 4 && f.row_bytes <= kShortWords * 4 && f.dst_row == f.row_bytes && dst_all % 16 == 0) {
+            f.unit = 100 + f.row_bytes / 4;
+            part = kShortRows;
+            accesses = budget;
+        }
+        blocks += (accesses + part - 1) / part;
+        if(blocks > (uint64_t)INT32_MAX) return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "too many rows in one call");
+        src_span[t.count] = { in.src, length == 0 ? 0 : (outer - 1) * f.src_outer + (inner - 1) * f.src_inner + (length - 1) * (uint64_t)f.src_row + f.row_bytes };
+        dst_span[t.count] = { in.dst, (outer - 1) * f.dst_outer + (inner - 1) * f.dst_inner + (budget - 1) * (uint64_t)f.dst_row + f.row_bytes };
         ++t.count;
     }
     for(int i = 0; i < t.count; ++i)
@@ -700,7 +998,6 @@ extern "C" int gsx_b200_budget_gather(const gsx_b200_gather_field *fields, int32
                 return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "a field's dst must not overlap any field's src");
         }
     if(t.count == 0) return GSX_B200_SUCCESS;
-    if(blocks > (uint64_t)INT32_MAX) return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "too many rows in one call");
     const uint64_t groups = outer * inner;
     budget_gather_kernel<<<dim3((unsigned)blocks, (unsigned)(groups < 65535 ? groups : 65535)), kThreads, 0, (cudaStream_t)stream_>>>(
         t, (uint32_t)groups, (uint32_t)inner, (uint32_t)length, (uint32_t)budget, keep, keep_stride, kept, device_out_of_range);

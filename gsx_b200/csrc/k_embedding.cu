@@ -87,14 +87,19 @@ __global__ void __launch_bounds__(kThreads) lookup_pack_kernel(const T *__restri
         c[u] = (uint32_t)(w - n[u] * packs);
         s[u] = w < total ? __ldg(index + n[u]) : (I)-1;
     }
+    if(rows == 0) {
+        if(w0 < total && bad != nullptr) atomicExch(bad, 1u);
+        return;
+    }
 #pragma unroll
-    for(int u = 0; u < U; ++u)
-        if(s[u] >= 0 && (uint64_t)s[u] < rows)
-            x[u] = *reinterpret_cast<const Pack<T, VW> *>(table + (uint64_t)s[u] * table_stride + (uint64_t)c[u] * VW);
+    for(int u = 0; u < U; ++u) {
+        const uint64_t row = (uint64_t)s[u] < rows ? (uint64_t)s[u] : 0; /* a negative index is a large one here */
+        x[u] = *reinterpret_cast<const Pack<T, VW> *>(table + row * table_stride + (uint64_t)c[u] * VW);
+    }
 #pragma unroll
     for(int u = 0; u < U; ++u) {
         if(w0 + (uint64_t)u * kThreads >= total) continue;
-        if(s[u] < 0 || (uint64_t)s[u] >= rows) {
+        if((uint64_t)s[u] >= rows) {
             if(bad != nullptr && c[u] == 0) atomicExch(bad, 1u);
             continue;
         }
@@ -105,61 +110,158 @@ __global__ void __launch_bounds__(kThreads) lookup_pack_kernel(const T *__restri
     }
 }
 
-/* any row: each thread makes OV consecutive elements of a contiguous out, across row borders */
-template <typename T, typename O, typename I, int OV>
-__global__ void __launch_bounds__(kThreads) lookup_flat_kernel(const T *__restrict__ table, uint64_t rows, uint32_t dim,
-                                                               uint64_t table_stride, const I *__restrict__ index,
-                                                               uint64_t total, float scale, O *__restrict__ out,
-                                                               uint64_t out_stride, uint32_t *__restrict__ bad)
+/* an index as a row number, or a number no table has */
+template <typename I>
+__device__ __forceinline__ uint32_t row_number(I v)
 {
-    const uint64_t e0 = ((uint64_t)blockIdx.x * kThreads + threadIdx.x) * OV;
-    if(e0 >= total) return;
-    uint64_t n = total <= 0xffffffffull ? (uint64_t)((uint32_t)e0 / dim) : e0 / dim;
-    uint32_t c = (uint32_t)(e0 - n * dim);
-    const int m = total - e0 < (uint64_t)OV ? (int)(total - e0) : OV;
-    I s = __ldg(index + n);
-    bool whole = m == OV;
-    Pack<O, OV> y;
-    uint32_t ok = 0;
-    uint64_t n_k = n;
-    uint32_t c_k = c;
+    return sizeof(I) == 8 && ((uint64_t)v >> 32) != 0 ? UINT32_MAX : (uint32_t)v;
+}
+
+/* Rows of DIM <= 4 elements into an out without gaps: a thread makes R of them, whole 16-byte stores.  A lane an element
+ * spends 30 instructions on each (place, index, row, element), this about 3.  kTable: the scaled table lies in shared
+ * memory, where the rows of 32 lanes cost a few bank conflicts instead of a cache line each. */
+constexpr size_t kShortTable = 100 * 1024;
+
+template <typename T, typename O, typename I, int DIM, bool kTable>
+__global__ void __launch_bounds__(kTable ? 1024 : kThreads) lookup_short_kernel(const T *__restrict__ table, uint32_t rows,
+                                                                                uint32_t stride_bytes,
+                                                                                const I *__restrict__ index, uint64_t count,
+                                                                                float scale, O *__restrict__ out,
+                                                                                uint32_t *__restrict__ bad)
+{
+    constexpr int R = 16 / sizeof(O);
+    constexpr uint32_t kBlock = kTable ? 1024 : kThreads;
+    extern __shared__ __align__(16) unsigned char smem[];
+    O *s_table = reinterpret_cast<O *>(smem);
+    const unsigned char *bytes = reinterpret_cast<const unsigned char *>(table);
+    if(kTable) {
+        for(uint32_t j = threadIdx.x; j < rows * DIM; j += kBlock)
+            s_table[j] = from_f32<O>(scale * to_f32(reinterpret_cast<const T *>(bytes + (uint64_t)(j / DIM) * stride_bytes)[j % DIM]));
+        __syncthreads();
+    }
+    const bool wide = (uintptr_t)index % 16 == 0;
+    for(uint64_t t = (uint64_t)blockIdx.x * kBlock + threadIdx.x; t * R < count; t += (uint64_t)gridDim.x * kBlock) {
+        const I *ix = index + t * R;
+        uint32_t s[R];
+        if(wide && t * R + R <= count) {
+            constexpr int V = 16 / sizeof(I);
 #pragma unroll
-    for(int k = 0; k < OV; ++k) {
-        if(k < m) {
-            if(c_k == dim) {
-                c_k = 0;
-                s = __ldg(index + ++n_k);
+            for(int r = 0; r < R; r += V) {
+                const Pack<I, V> v = *reinterpret_cast<const Pack<I, V> *>(ix + r);
+#pragma unroll
+                for(int k = 0; k < V; ++k) s[r + k] = row_number(v.v[k]);
             }
-            if(s >= 0 && (uint64_t)s < rows) {
-                y.v[k] = from_f32<O>(scale * to_f32(table[(uint64_t)s * table_stride + c_k]));
-                ok |= 1u << k;
-            } else {
-                whole = false;
-                if(bad != nullptr && c_k == 0) atomicExch(bad, 1u);
-            }
-            ++c_k;
+        } else {
+#pragma unroll
+            for(int r = 0; r < R; ++r) s[r] = t * R + r < count ? row_number(__ldg(ix + r)) : UINT32_MAX;
         }
-    }
-    if(whole && OV > 1) {
-        *reinterpret_cast<Pack<O, OV> *>(out + e0) = y; /* out_stride == dim */
-        return;
-    }
+        Pack<O, R> y[DIM]; /* R * DIM elements in order */
+        bool all = true;
 #pragma unroll
-    for(int k = 0; k < OV; ++k) {
-        if(k < m) {
-            if(c == dim) {
-                c = 0;
-                ++n;
+        for(int r = 0; r < R; ++r) {
+            all &= s[r] < rows;
+            if(s[r] < rows)
+#pragma unroll
+                for(int k = 0; k < DIM; ++k) {
+                    const int e = r * DIM + k;
+                    y[e / R].v[e % R] = kTable ? s_table[s[r] * DIM + k]
+                                               : from_f32<O>(scale * to_f32(reinterpret_cast<const T *>(bytes + (uint64_t)s[r] * stride_bytes)[k]));
+                }
+        }
+        O *to = out + t * R * DIM;
+        if(all) {
+#pragma unroll
+            for(int k = 0; k < DIM; ++k) reinterpret_cast<Pack<O, R> *>(to)[k] = y[k];
+            continue;
+        }
+#pragma unroll
+        for(int r = 0; r < R; ++r) {
+            if(s[r] < rows) {
+#pragma unroll
+                for(int k = 0; k < DIM; ++k) to[r * DIM + k] = y[(r * DIM + k) / R].v[(r * DIM + k) % R];
+            } else if(bad != nullptr && t * R + r < count) {
+                atomicExch(bad, 1u);
             }
-            if(ok >> k & 1u) out[n * out_stride + c] = y.v[k];
-            ++c;
         }
     }
 }
 
+/* Any row: 2^CLOG lanes take a row's elements side by side (NC of them each, 2^CLOG apart), a warp 32 consecutive rows,
+ * whose indices it loads at once and hands round; U steps of rows in flight.  Longer rows than 32 * NC take several
+ * turns. */
+template <typename T, typename O, typename I, int NC, int CLOG>
+__global__ void __launch_bounds__(kThreads) lookup_warp_kernel(const T *__restrict__ table, uint32_t rows, uint32_t dim,
+                                                               uint32_t stride_bytes, const I *__restrict__ index,
+                                                               uint64_t count, float scale, O *__restrict__ out,
+                                                               uint64_t out_stride, uint32_t *__restrict__ bad)
+{
+    constexpr int U = 8 / NC, cl = 1 << CLOG, per = 32 >> CLOG; /* rows a step */
+    const int lane = threadIdx.x & 31;
+    const uint64_t n0 = ((uint64_t)blockIdx.x * kWarps + (threadIdx.x >> 5)) * 32;
+    if(n0 >= count) return;
+    const int left = count - n0 < 32 ? (int)(count - n0) : 32;
+    const uint32_t mine = lane < left ? row_number(__ldg(index + n0 + lane)) : UINT32_MAX;
+    if(bad != nullptr && lane < left && mine >= rows) atomicExch(bad, 1u);
+    if(rows == 0) return;
+    const unsigned char *bytes = reinterpret_cast<const unsigned char *>(table);
+    const uint64_t hop = out_stride * per;
+    for(uint32_t c0 = lane & (cl - 1); c0 - (lane & (cl - 1)) < dim; c0 += NC << CLOG) {
+        /* elements and rows that are not there are read in the place of ones that are (a load under a condition becomes a
+         * branch of some ten instructions) and not stored */
+        const unsigned char *from[NC];
+        bool in[NC];
+#pragma unroll
+        for(int k = 0; k < NC; ++k) {
+            const uint32_t c = c0 + (k << CLOG);
+            in[k] = c < dim;
+            from[k] = bytes + (uint64_t)(in[k] ? c : 0u) * sizeof(T);
+        }
+        O *to = out + (n0 + (lane >> CLOG)) * out_stride + c0;
+#pragma unroll 1
+        for(int j = 0; j < cl; j += U) { /* cl steps of `per` rows are the warp's 32 */
+            uint32_t s[U];
+            T x[U][NC];
+#pragma unroll
+            for(int u = 0; u < U; ++u) {
+                s[u] = __shfl_sync(0xffffffffu, mine, (j + u) * per + (lane >> CLOG));
+                const uint32_t row = s[u] < rows ? s[u] : 0u;
+#pragma unroll
+                for(int k = 0; k < NC; ++k) x[u][k] = *reinterpret_cast<const T *>(from[k] + (uint64_t)row * stride_bytes);
+            }
+#pragma unroll
+            for(int u = 0; u < U; ++u) {
+#pragma unroll
+                for(int k = 0; k < NC; ++k)
+                    if(s[u] < rows && in[k]) to[k << CLOG] = from_f32<O>(scale * to_f32(x[u][k]));
+                to += hop;
+            }
+        }
+    }
+}
+
+template <typename T, typename O, typename I, int DIM>
+cudaError_t launch_short(const T *table, uint32_t rows, uint32_t stride_bytes, const I *index, uint64_t count, float scale, O *out,
+                         uint32_t *bad, cudaStream_t stream)
+{
+    constexpr uint64_t R = 16 / sizeof(O);
+    const size_t bytes = (size_t)rows * DIM * sizeof(O);
+    /* a small table that is read many times over: each of two CTAs an SM copies it to shared memory once */
+    if(bytes <= kShortTable && count >= (uint64_t)rows * 64 && count >= (1u << 18)) {
+        const cudaError_t e = cudaFuncSetAttribute(lookup_short_kernel<T, O, I, DIM, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   (int)kShortTable);
+        if(e != cudaSuccess) return e;
+        lookup_short_kernel<T, O, I, DIM, true><<<148 * 2, 1024, bytes, stream>>>(table, rows, stride_bytes, index, count, scale, out, bad);
+        return cudaSuccess;
+    }
+    const uint64_t threads = (count + R - 1) / R;
+    lookup_short_kernel<T, O, I, DIM, false><<<(unsigned)((threads + kThreads - 1) / kThreads), kThreads, 0, stream>>>(
+        table, rows, stride_bytes, index, count, scale, out, bad);
+    return cudaSuccess;
+}
+
 template <typename T, typename O, typename I>
-void launch_lookup(const void *table_, uint64_t rows, uint64_t dim, uint64_t table_stride, const void *index_,
-                   uint64_t count, float scale, void *out_, uint64_t out_stride, uint32_t *bad, cudaStream_t stream)
+cudaError_t launch_lookup(const void *table_, uint64_t rows, uint64_t dim, uint64_t table_stride, const void *index_,
+                          uint64_t count, float scale, void *out_, uint64_t out_stride, uint32_t *bad, cudaStream_t stream)
 {
     const T *table = static_cast<const T *>(table_);
     const I *index = static_cast<const I *>(index_);
@@ -168,27 +270,38 @@ void launch_lookup(const void *table_, uint64_t rows, uint64_t dim, uint64_t tab
     constexpr int OV = 16 / sizeof(O);
     const bool packs = dim % VW == 0 && table_stride % VW == 0 && (uintptr_t)table % 16 == 0 &&
                        (out_stride * sizeof(O)) % 16 == 0 && (uintptr_t)out % 16 == 0 && dim % OV == 0;
-    if(packs) {
-        const uint64_t total = count * (dim / VW);
-        if(total >= 148ull * 2048 * 2) {
-            const uint64_t per = kThreads * 4;
-            lookup_pack_kernel<T, O, I, VW, 4><<<(unsigned)((total + per - 1) / per), kThreads, 0, stream>>>(
-                table, rows, (uint32_t)(dim / VW), table_stride, index, total, scale, out, out_stride, bad);
-        } else {
-            lookup_pack_kernel<T, O, I, VW, 1><<<(unsigned)((total + kThreads - 1) / kThreads), kThreads, 0, stream>>>(
-                table, rows, (uint32_t)(dim / VW), table_stride, index, total, scale, out, out_stride, bad);
+    const uint32_t stride_bytes = (uint32_t)(table_stride * sizeof(T));
+    if(dim <= 4 && out_stride == dim && (uintptr_t)out % 16 == 0) {
+        switch(dim) {
+        case 1: return launch_short<T, O, I, 1>(table, (uint32_t)rows, stride_bytes, index, count, scale, out, bad, stream);
+        case 2: return launch_short<T, O, I, 2>(table, (uint32_t)rows, stride_bytes, index, count, scale, out, bad, stream);
+        case 3: return launch_short<T, O, I, 3>(table, (uint32_t)rows, stride_bytes, index, count, scale, out, bad, stream);
+        default: return launch_short<T, O, I, 4>(table, (uint32_t)rows, stride_bytes, index, count, scale, out, bad, stream);
         }
-        return;
     }
-    const uint64_t total = count * dim;
-    if(out_stride == dim && (uintptr_t)out % 16 == 0) {
-        const uint64_t per = kThreads * OV;
-        lookup_flat_kernel<T, O, I, OV><<<(unsigned)((total + per - 1) / per), kThreads, 0, stream>>>(
-            table, rows, (uint32_t)dim, table_stride, index, total, scale, out, out_stride, bad);
-    } else {
-        lookup_flat_kernel<T, O, I, 1><<<(unsigned)((total + kThreads - 1) / kThreads), kThreads, 0, stream>>>(
-            table, rows, (uint32_t)dim, table_stride, index, total, scale, out, out_stride, bad);
+    if(packs) {
+        const uint64_t accesses = count * (dim / VW);
+        if(accesses >= 148ull * 2048 * 2) {
+            const uint64_t per = kThreads * 4;
+            lookup_pack_kernel<T, O, I, VW, 4><<<(unsigned)((accesses + per - 1) / per), kThreads, 0, stream>>>(
+                table, rows, (uint32_t)(dim / VW), table_stride, index, accesses, scale, out, out_stride, bad);
+        } else {
+            lookup_pack_kernel<T, O, I, VW, 1><<<(unsigned)((accesses + kThreads - 1) / kThreads), kThreads, 0, stream>>>(
+                table, rows, (uint32_t)(dim / VW), table_stride, index, accesses, scale, out, out_stride, bad);
+        }
+        return cudaSuccess;
     }
+    const unsigned ctas = (unsigned)((count + kWarps * 32 - 1) / (kWarps * 32));
+    auto launch = [&](auto kernel) {
+        kernel<<<ctas, kThreads, 0, stream>>>(table, (uint32_t)rows, (uint32_t)dim, stride_bytes, index, count, scale, out,
+                                              out_stride, bad);
+    };
+    if(dim <= 8) launch(lookup_warp_kernel<T, O, I, 1, 3>);
+    else if(dim <= 16) launch(lookup_warp_kernel<T, O, I, 1, 4>);
+    else if(dim <= 32) launch(lookup_warp_kernel<T, O, I, 1, 5>);
+    else if(dim <= 64) launch(lookup_warp_kernel<T, O, I, 2, 5>);
+    else launch(lookup_warp_kernel<T, O, I, 4, 5>);
+    return cudaSuccess;
 }
 
 /* ------------------------------------------------------------------------------------------ */
@@ -588,6 +701,9 @@ template <typename GT, typename TT, int VW, int NR>
 __global__ void __launch_bounds__(kThreads, NR * VW <= 8 ? 4 : 2) run_sum_kernel(const GT *__restrict__ grad, uint32_t stride_bytes, const Runs a,
                                                               const Table table)
 {
+    /* packs that are not there are read in the place of the first, added and not stored (a load under a condition becomes
+     * a branch); single elements of short rows are not, as the idle lanes' loads cost more */
+    constexpr bool kClamp = NR * VW > 1;
     constexpr int kRegs = NR * VW * (int)sizeof(GT) / 4 > 0 ? NR * VW * (int)sizeof(GT) / 4 : 1;
     constexpr int U = kRegs <= 3 ? 8 : kRegs <= 8 ? 4 : 2; /* a divisor of 8, as runs are multiples of 8 */
     extern __shared__ __align__(16) unsigned char smem[];
@@ -637,13 +753,13 @@ __global__ void __launch_bounds__(kThreads, NR * VW <= 8 ? 4 : 2) run_sum_kernel
         for(int r = 0; r < NR; ++r) {
             const uint32_t c = col0 + (uint32_t)((r * cl + cg) * VW);
             in[r] = c < a.dim;
-            base[r] = reinterpret_cast<const unsigned char *>(grad + c);
+            base[r] = reinterpret_cast<const unsigned char *>(grad + (!kClamp || in[r] ? c : 0u));
         }
         auto load = [&](Pack<GT, VW> (&x)[NR], int i) {
             const uint32_t p = mine[i].y;
 #pragma unroll
             for(int r = 0; r < NR; ++r)
-                if(in[r]) x[r] = *reinterpret_cast<const Pack<GT, VW> *>(base[r] + (uint64_t)p * stride_bytes);
+                if(kClamp || in[r]) x[r] = *reinterpret_cast<const Pack<GT, VW> *>(base[r] + (uint64_t)p * stride_bytes);
         };
         auto add = [&](const Pack<GT, VW> (&x)[NR]) {
 #pragma unroll
@@ -685,7 +801,7 @@ __global__ void __launch_bounds__(kThreads, NR * VW <= 8 ? 4 : 2) run_sum_kernel
             }
 #pragma unroll
             for(int u = 0; u < U; ++u)
-                if(i + u < r1) load(x[u], i + u);
+                load(x[u], i + u < r1 ? i + u : i);
 #pragma unroll
             for(int u = 0; u < U; ++u) {
                 if(i + u < r1) add(x[u]);
@@ -995,18 +1111,19 @@ extern "C" int gsx_b200_embedding_lookup(const void *table, int table_type, uint
     if((uintptr_t)table % float_bytes(table_type) || (uintptr_t)out % float_bytes(out_type) ||
        (uintptr_t)index % (index_type == GSX_B200_DATA_I32 ? 4 : 8))
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "pointers must be aligned to their element type");
+    if(table_stride * float_bytes(table_type) > 0xffffffffull)
+        return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "table_stride must be below 4 GiB");
     if(count * dim / 256 > (uint64_t)INT32_MAX)
         return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "count * dim must be below 2^39");
     cudaStream_t stream = (cudaStream_t)stream_;
+    cudaError_t e = cudaSuccess;
     GSX_WITH_FLOAT_TYPE(table_type, T, GSX_WITH_FLOAT_TYPE(out_type, O, {
-        if(index_type == GSX_B200_DATA_I32)
-            launch_lookup<T, O, int32_t>(table, rows, dim, table_stride, index, count, scale, out, out_stride,
-                                         device_out_of_range, stream);
-        else
-            launch_lookup<T, O, int64_t>(table, rows, dim, table_stride, index, count, scale, out, out_stride,
-                                         device_out_of_range, stream);
+        e = index_type == GSX_B200_DATA_I32 ? launch_lookup<T, O, int32_t>(table, rows, dim, table_stride, index, count, scale, out,
+                                                                           out_stride, device_out_of_range, stream)
+                                            : launch_lookup<T, O, int64_t>(table, rows, dim, table_stride, index, count, scale, out,
+                                                                           out_stride, device_out_of_range, stream);
     }));
-    return launch_status(cudaSuccess);
+    return launch_status(e);
 }
 
 extern "C" uint64_t gsx_b200_embedding_workspace_bytes(uint64_t count, uint64_t rows, uint64_t dim)

@@ -400,8 +400,8 @@ GSX_B200_API int gsx_b200_adc_select_keep(uint64_t n, const float *opacity, cons
 /*
  * Shared rows (no counterpart in the reference): a table whose rows many Gaussians share, with one row number
  * per Gaussian, or any other embedding table.  Tables, outputs and gradients are f32, f16 or bf16 in any
- * combination, indices i32 or i64; row strides are in elements and at least dim (that of grad_out is below
- * 4 GiB); rows, dim and count stay below 2^31.  An index outside [0, rows) sets *device_out_of_range to 1 (when non-NULL) and takes no part: its row of
+ * combination, indices i32 or i64; row strides are in elements and at least dim (those of a table that is
+ * read and of grad_out below 4 GiB); rows, dim and count stay below 2^31.  An index outside [0, rows) sets *device_out_of_range to 1 (when non-NULL) and takes no part: its row of
  * out stays untouched, its gradient is dropped.  Nothing waits, allocates or depends on values: the calls can be
  * captured into a graph.
  * gsx_b200_embedding_lookup: out[n] = scale * table[index[n]], computed in f32 and rounded once.
@@ -440,7 +440,7 @@ GSX_B200_API int gsx_b200_embedding_backward(const void *grad_out, int grad_type
  *   to +0.  kept[g] = min(entries in use, budget).  drop (may be NULL) receives the other entries, in increasing
  *   order: those in use less kept[g].  Places of keep and drop behind the lists are left as they were.
  *   workspace: gsx_b200_budget_workspace_bytes(groups, length) bytes of device memory, 4-byte aligned, of any
- *   content (0 bytes for groups of up to 49152 entries); calls that overlap on the GPU need one each.
+ *   content (0 bytes for groups of up to 393216 entries); calls that overlap on the GPU need one each.
  * gsx_b200_budget_gather: for every field and group, row r of dst = row keep[g, r] of src for r < kept[g]; later
  *   rows of dst are left as they were.  All fields in ONE launch.  Group g is (g / inner, g % inner) in a field's
  *   outer and inner strides (caches of [batch, head, entry] and [batch, entry, head] order alike).  A keep entry
@@ -451,7 +451,7 @@ GSX_B200_API int gsx_b200_embedding_backward(const void *grad_out, int grad_type
 typedef struct gsx_b200_gather_field {
     const void *src;
     void *dst;
-    uint64_t row_bytes; /* strides are in bytes */
+    uint64_t row_bytes; /* strides are in bytes; row strides below 4 GiB */
     uint64_t src_outer_stride, src_inner_stride, src_row_stride;
     uint64_t dst_outer_stride, dst_inner_stride, dst_row_stride;
 } gsx_b200_gather_field;

@@ -44,7 +44,7 @@ def _gather(fields=None, count=1, outer=1, inner=1, length=16, budget=8, keep=P,
 
 CASES = [
     (gb.NOT_SUPPORTED, _lookup, [dict(ttype=U8), dict(otype=I32), dict(itype=F32)]),
-    (gb.OUT_OF_RANGE, _lookup, [dict(rows=2 ** 31), dict(count=2 ** 31), dict(tstride=2 ** 41),
+    (gb.OUT_OF_RANGE, _lookup, [dict(rows=2 ** 31), dict(count=2 ** 31), dict(tstride=2 ** 41), dict(tstride=2 ** 30),
                                 dict(count=2 ** 30, dim=2 ** 30, tstride=2 ** 30, ostride=2 ** 30)]),
     (gb.INVALID_ARGUMENT, _lookup, [dict(table=None), dict(index=None), dict(out=None), dict(tstride=7), dict(ostride=7),
                                     dict(table=P + 2), dict(out=P + 1, otype=F16), dict(index=P + 4, itype=I64)]),
@@ -63,16 +63,16 @@ CASES = [
                                         dict(w=P + 64), dict(ostride=17)]),
     (_capi.SUCCESS, _accumulate, [dict(groups=0), dict(length=0)]),
     (gb.OUT_OF_RANGE, _select, [dict(groups=2 ** 31), dict(length=2 ** 31), dict(budget=2 ** 31),
-                                dict(groups=70_000, length=50_000, sstride=50_000)]),
+                                dict(groups=70_000, length=400_000, sstride=400_000), dict(groups=2 ** 28)]),
     (gb.INVALID_ARGUMENT, _select, [dict(first=9), dict(first=4, recent=5), dict(recent=2 ** 64 - 1), dict(score=None),
                                     dict(keep=None), dict(kept=None), dict(sstride=15), dict(kstride=7),
                                     dict(drop=P, dstride=15), dict(score=P + 1), dict(keep=P + 2),
-                                    dict(length=50_000, sstride=50_000),
-                                    dict(length=50_000, sstride=50_000, ws=P, size=100),
-                                    dict(length=50_000, sstride=50_000, ws=P + 1, size=1 << 30)]),
+                                    dict(length=400_000, sstride=400_000),
+                                    dict(length=400_000, sstride=400_000, ws=P, size=100),
+                                    dict(length=400_000, sstride=400_000, ws=P + 1, size=1 << 30)]),
     (_capi.SUCCESS, _select, [dict(groups=0)]),
     (gb.OUT_OF_RANGE, _gather, [dict(count=33), dict(count=-1), dict(outer=2 ** 16, inner=2 ** 16), dict(length=2 ** 31),
-                                dict(src_row_stride=2 ** 43), dict(row_bytes=2 ** 32, dst_row_stride=2 ** 32)]),
+                                dict(src_row_stride=2 ** 32), dict(src_outer_stride=2 ** 43), dict(row_bytes=2 ** 32, dst_row_stride=2 ** 32)]),
     (gb.INVALID_ARGUMENT, _gather, [dict(keep=None), dict(kept=None), dict(src=None), dict(dst=None),
                                     dict(dst_row_stride=11), dict(dst=P + 180), dict(dst=P - 12 * 7),
                                     dict(inner=2, kstride=7)]),
@@ -96,8 +96,8 @@ def test_workspace_sizes():
     one = L.gsx_b200_embedding_workspace_bytes(1_000_000, 256, 8)
     two = L.gsx_b200_embedding_workspace_bytes(1_000_000, 257, 8)
     assert 8_000_000 < one < 16_000_000 <= two < 24_000_000
-    assert L.gsx_b200_budget_workspace_bytes(32, 49_152) == 0
-    assert 0 < L.gsx_b200_budget_workspace_bytes(32, 49_153) < 4 << 20
+    assert L.gsx_b200_budget_workspace_bytes(32, 393_216) == 0
+    assert 0 < L.gsx_b200_budget_workspace_bytes(32, 393_217) < 4 << 20
 
 
 def test_python_calls_refuse_host_tensors():

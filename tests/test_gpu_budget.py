@@ -131,7 +131,8 @@ def _check_select(score, budget, lengths=None, first=0, recent=0):
 
 
 SELECT_SIZES = [(1, 1, 0), (1, 1, 1), (2, 5, 3), (3, 33, 32), (4, 1000, 1), (2, 1025, 1024), (3, 5000, 2500),
-                (1, 49_152, 30_000), (2, 49_153, 100), (3, 100_001, 77_777), (1, 400_000, 399_999), (40, 60_000, 512)]
+                (1, 49_152, 30_000), (2, 49_153, 100), (3, 100_001, 77_777), (1, 400_000, 399_999), (40, 60_000, 512), (3, 393_216, 20_000),
+                (2, 393_217, 200_000), (1, 1_000_003, 400_000), (5, 500_000, 7)]
 
 
 @pytest.mark.parametrize("groups,length,budget", SELECT_SIZES)
@@ -145,7 +146,7 @@ def test_select_sizes(cuda_device, groups, length, budget):
     _check_select(score, budget, recent=budget)
 
 
-@pytest.mark.parametrize("length", [2000, 60_000])
+@pytest.mark.parametrize("length", [2000, 60_000, 420_000])
 def test_select_ties_and_special_values(cuda_device, length):
     g = _gen(length)
     base = torch.randint(0, 4, (1, length), generator=g, device="cuda").float()
@@ -159,7 +160,7 @@ def test_select_ties_and_special_values(cuda_device, length):
             _check_select(score, budget, first=budget // 5, recent=budget // 4)
 
 
-@pytest.mark.parametrize("length", [300, 70_000])
+@pytest.mark.parametrize("length", [300, 70_000, 400_000])
 def test_select_ragged(cuda_device, length):
     g = _gen(5)
     score = torch.rand(7, length, generator=g, device="cuda")
@@ -185,16 +186,40 @@ def test_select_shapes_and_strides(cuda_device):
 
 
 @pytest.mark.parametrize("dtype,tail", [(F32, (3,)), (F32, ()), (torch.uint8, (5,)), (F16, (7,)), (F16, (128,)),
-                                        (F32, (15, 3)), (torch.int64, (2,)), (torch.uint8, (20_001,))])
+                                        (F32, (15, 3)), (torch.int64, (2,)), (torch.uint8, (20_001,)), (F32, (2,)),
+                                        (F32, (4,)), (F32, (5,)), (F32, (6,)), (F32, (7,)), (F32, (8,)), (F32, (9,)),
+                                        (F16, (6,)), (F16, (1,)), (torch.uint8, (1,)), (torch.int64, (1,))])
 def test_gather_rows_of_every_size(cuda_device, dtype, tail):
     g = _gen(7)
-    src = torch.randint(0, 200, (1000, *tail), generator=g, device="cuda").to(dtype)
-    keep = torch.sort(torch.randperm(1000, generator=g, device="cuda")[:400]).values.int()
-    dst = torch.full((410, *tail), 77, device="cuda").to(dtype)
-    kept = torch.tensor(399, dtype=torch.int32, device="cuda")
-    gb.budget_gather([(src, dst)], keep, kept)
-    assert torch.equal(dst[:399], src[keep[:399].long()])
-    assert bool((dst[399:] == 77).all())
+    # lists that keep few entries and lists that keep most
+    for rows, n in ((1000, 399), (6000, 2500), (5000, 1024), (7000, 5001), (4100, 4096), (9, 5), (300_000, 700)):
+        src = torch.randint(0, 200, (rows, *tail), generator=g, device="cuda").to(dtype)
+        keep = torch.sort(torch.randperm(rows, generator=g, device="cuda")[:n + 1]).values.int()
+        kept = torch.tensor(n, dtype=torch.int32, device="cuda")
+        if tail == (20_001,) and rows > 6000:
+            continue
+        for offset in (0, 1):  # a dst that starts on a 16-byte boundary, and one that need not
+            dst = torch.full((n + 11, *tail), 77, device="cuda").to(dtype)
+            gb.budget_gather([(src, dst[offset:])], keep, kept)
+            assert torch.equal(dst[offset:offset + n], src[keep[:n].long()])
+            assert bool((dst[offset + n:] == 77).all()) and bool((dst[:offset] == 77).all())
+
+
+@pytest.mark.parametrize("dim", [1, 2, 3, 4])
+def test_gather_short_rows_in_any_order_and_from_any_place(cuda_device, dim):
+    """Lists need not be sorted, may name an entry twice, and src may be strided or start anywhere."""
+    g = _gen(17)
+    flat = torch.randn(5000 * dim + 8, generator=g, device="cuda")
+    keep = torch.randint(1000, 2500, (3000,), generator=g, device="cuda", dtype=torch.int32)
+    kept = torch.tensor(2999, dtype=torch.int32, device="cuda")
+    for src in [flat[o:o + 5000 * dim].view(5000, dim) for o in range(4)] + [torch.randn(5000, dim + 1, generator=g, device="cuda")[:, :dim]]:
+        dst = torch.zeros(3000, dim, device="cuda")
+        gb.budget_gather([(src, dst)], keep, kept)
+        assert torch.equal(dst[:2999], src[keep[:2999].long()]) and bool((dst[2999] == 0).all())
+    one = torch.tensor([4999, 0], dtype=torch.int32, device="cuda")  # a single row, and the last word of src
+    dst = torch.zeros(2, dim, device="cuda")
+    gb.budget_gather([(flat[8:].view(5000, dim), dst)], one, torch.tensor(1, dtype=torch.int32, device="cuda"))
+    assert torch.equal(dst[0], flat[8:].view(5000, dim)[4999])
 
 
 @pytest.mark.parametrize("order", ["heads first", "entries first"])
@@ -221,9 +246,10 @@ def test_gather_caches_of_both_layouts(cuda_device, order):
             assert torch.equal(k2[b, h, n:], k0[b, h, n:])
 
 
-def test_gather_flags_entries_out_of_range(cuda_device):
-    src = torch.randn(10, 4, device="cuda")
-    dst = torch.zeros(4, 4, device="cuda")
+@pytest.mark.parametrize("dim", [1, 3, 4, 9])
+def test_gather_flags_entries_out_of_range(cuda_device, dim):
+    src = torch.randn(10, dim, device="cuda")
+    dst = torch.zeros(4, dim, device="cuda")
     bad = torch.zeros(1, dtype=torch.int32, device="cuda")
     keep = torch.tensor([1, 10, -1, 9], dtype=torch.int32, device="cuda")
     gb.budget_gather([(src, dst)], keep, torch.tensor(1, dtype=torch.int32, device="cuda"), bad=bad)
@@ -233,7 +259,7 @@ def test_gather_flags_entries_out_of_range(cuda_device):
     assert torch.equal(dst, torch.stack([src[1], src[0] * 0, src[0] * 0, src[9]]))
 
 
-@pytest.mark.parametrize("length", [900, 80_000])
+@pytest.mark.parametrize("length", [900, 80_000, 400_000])
 def test_evict_on_another_stream_and_in_a_replayed_graph(cuda_device, length):
     g = _gen(9)
     budget = length // 2

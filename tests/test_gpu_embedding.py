@@ -50,10 +50,18 @@ def test_lookup_types(cuda_device, table_type, out_type, itype):
 
 def test_lookup_large_takes_every_path(cuda_device):
     g = _gen(2)
-    for count, rows, dim, dtype in [(400_003, 4096, 3, F32), (200_001, 1000, 45, BF16), (300_000, 64, 32, F16)]:
+    for count, rows, dim, dtype in [(400_003, 4096, 3, F32), (200_001, 1000, 45, BF16), (300_000, 64, 32, F16),
+                                    (3_000_001, 1, 1, F32), (1_500_000, 700, 9, F16), (70_001, 5, 31, BF16)]:
         table = torch.randn(rows, dim, generator=g, device="cuda").to(dtype)
-        index = _index(g, count, rows, torch.int32, 2.0)
-        _check_lookup(gb.embedding_lookup(table, index, scale=0.25), table, index, 0.25)
+        for itype in (torch.int32, torch.int64):
+            index = _index(g, count, rows, itype, 2.0)
+            _check_lookup(gb.embedding_lookup(table, index, scale=0.25), table, index, 0.25)
+            index[5::7] = rows  # rows that stay as they were
+            out, bad = torch.full((count, dim), 7.0, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+            gb.embedding_lookup(table, index, out=out, scale=0.25, bad=bad)
+            assert int(bad) == 1 and bool((out[5::7] == 7.0).all())
+            used = index < rows
+            _check_lookup(out[used], table, index[used], 0.25)
 
 
 def test_lookup_index_shapes_and_empty_calls(cuda_device):
