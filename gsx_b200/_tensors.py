@@ -20,13 +20,13 @@ def type_code(t, types: dict, name: str) -> int:
     return code
 
 
-def on_device(device, **tensors):
+def on_device(device, *tensors):
     """Every tensor (None allowed) lives on the CUDA device `device`."""
     if device.type != "cuda":
         raise invalid("tensors must be on a CUDA device")
-    for name, t in tensors.items():
+    for t in tensors:
         if t is not None and t.device != device:
-            raise invalid(f"{name} must be on {device}, not {t.device}")
+            raise invalid(f"all tensors must be on {device}, one is on {t.device}")
 
 
 def row_stride(t, dim: int, name: str) -> int:
@@ -62,10 +62,10 @@ def word(t, name: str):
     return t.data_ptr()
 
 
-def below_2_31(**numbers):
-    for name, v in numbers.items():
-        if not 0 <= v < 2 ** 31:
-            raise GsxError(OUT_OF_RANGE, f"{name} must be in [0, 2^31)")
+def below_2_31(*numbers):
+    for v in numbers:
+        if not 0 <= v < 2147483648:
+            raise GsxError(OUT_OF_RANGE, f"counts and sizes must be in [0, 2^31), not {v}")
 
 
 def empty(shape, dtype, device, stream):
@@ -79,11 +79,15 @@ def empty(shape, dtype, device, stream):
 def launch(fn, device, stream, *args):
     """fn(*args, stream handle) with `device` current."""
     if stream is None:
-        stream = torch.cuda.current_stream(device)
+        handle = torch._C._cuda_getCurrentRawStream(device.index)
     elif stream.device != device:
         raise invalid(f"stream must be on {device}, not {stream.device}")
-    if torch.cuda.current_device() == device.index:
-        check(fn(*args, stream.cuda_stream))
+    else:
+        handle = stream.cuda_stream
+    if torch._C._cuda_getDevice() == device.index:
+        rc = fn(*args, handle)
     else:
         with torch.cuda.device(device):
-            check(fn(*args, stream.cuda_stream))
+            rc = fn(*args, handle)
+    if rc:
+        check(rc)

@@ -5,9 +5,11 @@ A score tensor is [length] for one set of entries (a scene) or [.., length] for 
 head); `lengths`, where given, is an int32 tensor of the leading shape with the entries in use."""
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
-from ._capi import GATHER_MAX_FIELDS, NOT_SUPPORTED, OUT_OF_RANGE, GatherField, GsxError, lib
+from ._capi import GATHER_MAX_FIELDS, NOT_SUPPORTED, OUT_OF_RANGE, GsxError, lib
 from ._tensors import FLOAT_TYPES, below_2_31, empty, group_stride, invalid, launch, on_device, type_code, word
 
 
@@ -16,9 +18,11 @@ def _score(score, name="score"):
     if score.dim() < 1 or score.dtype != torch.float32:
         raise invalid(f"{name} must be a float32 tensor of at least one dimension")
     length = score.shape[-1]
+    groups = score.shape[:-1].numel()
+    if score.is_contiguous():
+        return groups, length, length
     if length > 1 and score.stride(-1) != 1:
         raise invalid(f"the last dimension of {name} must be contiguous")
-    groups = score.shape[:-1].numel()
     return groups, length, group_stride(score, score.dim() - 1, name) if groups > 1 else length
 
 
@@ -42,13 +46,13 @@ def budget_accumulate(score, weights, out=None, decay: float = 1.0, lengths=None
     elif out.shape != score.shape:
         raise invalid("out must have score's shape")
     device = score.device
-    on_device(device, weights=weights, out=out, lengths=lengths, row_lengths=row_lengths)
+    on_device(device, weights, out, lengths, row_lengths)
     if weights.dim() != score.dim() + 1 or weights.shape[:-2] != lead or weights.shape[-1] != length:
         raise invalid(f"weights must be {(*lead, 'rows', length)}, not {tuple(weights.shape)}")
     rows = weights.shape[-2]
     if length > 1 and weights.stride(-1) != 1:
         raise invalid("the last dimension of weights must be contiguous")
-    below_2_31(groups=groups, rows=rows, length=length)
+    below_2_31(groups, rows, length)
     launch(lib().gsx_b200_budget_accumulate, device, stream, score.data_ptr(), stride, weights.data_ptr(),
            type_code(weights, FLOAT_TYPES, "weights"), group_stride(weights, weights.dim() - 2, "weights"),
            weights.stride(-2) if rows > 1 else length, groups, rows, length, _per_group(lengths, lead, "lengths"),
@@ -64,13 +68,13 @@ def budget_select(score, budget: int, lengths=None, first: int = 0, recent: int 
     drop, where given, int32 of score's shape, receives the others.  Places behind the lists are left as they were."""
     groups, length, stride = _score(score)
     lead = score.shape[:-1]
-    below_2_31(groups=groups, length=length, budget=budget)
+    below_2_31(groups, length, budget)
     if first < 0 or recent < 0:
         raise GsxError(OUT_OF_RANGE, "first and recent must not be negative")
     if first + recent > budget:
         raise invalid("first + recent must be at most budget")
     device = score.device
-    on_device(device, lengths=lengths, keep=keep, kept=kept, drop=drop)
+    on_device(device, lengths, keep, kept, drop)
     most = min(budget, length)
     if keep is None:
         keep = empty((*lead, most), torch.int32, device, stream)
@@ -90,18 +94,23 @@ def budget_select(score, budget: int, lengths=None, first: int = 0, recent: int 
     return keep, kept
 
 
-def _field(f, t, lead, tail, side):
-    """One side of a gather field: checks the shape, gives (entries, (outer, inner, row) strides in bytes)."""
+def _field(t, lead, tail, side):
+    """Entries and (outer, inner, row) strides in bytes of one side of a gather field; checks its shape."""
     n = len(lead)
-    if t.dim() < n + 1 or t.shape[:n] != lead or t.shape[n + 1:] != tail:
-        raise invalid(f"{side} {f} must be {(*lead, 'entries', *tail)}, not {tuple(t.shape)}")
+    shape, size = t.shape, t.element_size()
+    if len(shape) <= n or shape[:n] != lead or shape[n + 1:] != tail:
+        raise invalid(f"{side} must be {(*lead, 'entries', *tail)}, not {tuple(shape)}")
+    entries = shape[n]
+    if t.is_contiguous():
+        row = tail.numel() * size
+        inner = row * entries if n else 0
+        return entries, inner * lead[1] if n == 2 else 0, inner, row
     want = 1
-    for d in range(t.dim() - 1, n, -1):
-        if t.shape[d] > 1 and t.stride(d) != want:
-            raise invalid(f"the rows of {side} {f} must be contiguous")
-        want *= t.shape[d]
-    size = t.element_size()
-    return t.shape[n], [s * size for s in ([0] * (2 - n) + list(t.stride()[:n]))] + [t.stride(n) * size]
+    for d in range(len(shape) - 1, n, -1):
+        if shape[d] > 1 and t.stride(d) != want:
+            raise invalid(f"the rows of {side} must be contiguous")
+        want *= shape[d]
+    return (entries, t.stride(0) * size if n == 2 else 0, t.stride(n - 1) * size if n else 0, t.stride(n) * size)
 
 
 def budget_gather(fields, keep, kept, bad=None, stream=None):
@@ -115,26 +124,25 @@ def budget_gather(fields, keep, kept, bad=None, stream=None):
     if len(fields) > GATHER_MAX_FIELDS:
         raise GsxError(OUT_OF_RANGE, f"at most {GATHER_MAX_FIELDS} fields")
     device = keep.device
-    on_device(device, kept=kept, bad=bad)
+    on_device(device, kept, bad)
     budget = keep.shape[-1]
-    table = (GatherField * max(len(fields), 1))()
-    length = None
-    for f, (src, dst) in enumerate(fields):
-        on_device(device, src=src, dst=dst)
+    n = len(lead)
+    table, length = [], None
+    for src, dst in fields:
+        if src.device != device or dst.device != device:
+            raise invalid(f"all tensors must be on {device}")
         if src.dtype != dst.dtype:
             raise GsxError(NOT_SUPPORTED, "src and dst must have the same type")
-        tail = src.shape[len(lead) + 1:]
-        entries, s = _field(f, src, lead, tail, "src")
-        room, d = _field(f, dst, lead, tail, "dst")
+        tail = src.shape[n + 1:]
+        entries, src_outer, src_inner, src_row = _field(src, lead, tail, "src")
+        room, dst_outer, dst_inner, dst_row = _field(dst, lead, tail, "dst")
         if length is None:
             length = entries
         if entries != length or room < budget:
             raise invalid("every src must have the same number of entries, every dst at least keep's")
-        e = table[f]
-        e.src, e.dst = src.data_ptr(), dst.data_ptr()
-        e.row_bytes = tail.numel() * src.element_size()
-        e.src_outer_stride, e.src_inner_stride, e.src_row_stride = s
-        e.dst_outer_stride, e.dst_inner_stride, e.dst_row_stride = d
+        # the members of gsx_b200_gather_field, all 64 bits wide
+        table += (src.data_ptr(), dst.data_ptr(), tail.numel() * src.element_size(), src_outer, src_inner, src_row,
+                  dst_outer, dst_inner, dst_row)
     outer, inner = ([1] * (2 - len(lead)) + list(lead))
-    launch(lib().gsx_b200_budget_gather, device, stream, table, len(fields), outer, inner, length or 0, budget,
+    launch(lib().gsx_b200_budget_gather, device, stream, (ctypes.c_uint64 * len(table))(*table), len(fields), outer, inner, length or 0, budget,
            keep.data_ptr(), budget, _per_group(kept, lead, "kept"), word(bad, "bad"))

@@ -220,14 +220,15 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *s_warp, uin
     __syncthreads();
     if(lane == 31) s_warp[warp] = v;
     __syncthreads();
-    uint32_t before = 0, sum = 0;
-    for(int w = 0; w < warps; ++w) {
-        const uint32_t s = s_warp[w];
-        before += w < warp ? s : 0u;
-        sum += s;
+    const uint32_t mine = lane < warps ? s_warp[lane] : 0u;
+    uint32_t incl = mine;
+#pragma unroll
+    for(int d = 1; d < 32; d <<= 1) {
+        const uint32_t t = __shfl_up_sync(0xffffffffu, incl, d);
+        if(lane >= d) incl += t;
     }
-    if(total) *total = sum;
-    return before + v;
+    if(total) *total = __shfl_sync(0xffffffffu, incl, 31);
+    return v + __shfl_sync(0xffffffffu, incl - mine, warp);
 }
 
 /* The bin, from the top, in which the need-th largest element lies: s_out[0] = bin, s_out[1] = how many of the

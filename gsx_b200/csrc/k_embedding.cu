@@ -378,10 +378,10 @@ struct Use {
 };
 
 template <typename I>
-__device__ __forceinline__ bool takes_part(I s, const Use &use)
+__device__ __forceinline__ bool takes_part(I s, const Use &use, bool &outside)
 {
     const bool in = sizeof(I) == 4 ? (uint32_t)s < use.rows : (uint64_t)s < (uint64_t)use.rows;
-    if(!in && use.bad != nullptr) atomicExch(use.bad, 1u);
+    outside |= !in;
     return in && (uint32_t)s != use.padding;
 }
 
@@ -409,19 +409,21 @@ __device__ __forceinline__ uint32_t block_inclusive_scan(uint32_t v, uint32_t *s
 }
 
 /* A tile of (row, position) pairs that a CTA ranks by one digit of at most 8 bits. */
+constexpr int kHistRow = kMaxBins + 1; /* one more: elements that take no part */
 template <int THREADS, int ITEMS>
 struct SortShared {
     uint2 pair[THREADS * ITEMS];
-    uint32_t hist[THREADS / 32][kMaxBins];
-    uint32_t before[kMaxBins]; /* of a digit: the tile's pairs with smaller ones */
+    uint32_t hist[THREADS / 32][kHistRow];
+    uint32_t before[kHistRow]; /* of a digit: the tile's pairs with smaller ones */
     uint32_t warp[32];
 };
 
 /* Ranks the tile's pairs (warp w holds elements 32 * items * w + 32 * it + lane) by digit, stable in element
- * order, and leaves them in s.pair in that order.  Elements with valid[it] false are dropped.  Returns, for threads
- * below the number of digits, how many pairs have that digit.  Lanes with equal digits find one another by one
- * ballot per digit bit: __match_any_sync takes a step per distinct value on this GPU (a tile of 8192 ranked in 12 us
- * with it, in 4 us with ballots). */
+ * order, and leaves them in s.pair in that order, those with valid[it] false (their key is 0) behind the others.
+ * Returns, for threads below the number of digits, how many pairs have that digit.  Lanes with equal digits find one
+ * another by one ballot per digit bit: __match_any_sync takes a step per distinct value on this GPU (a tile of 8192
+ * ranked in 12 us with it, in 4 us with ballots).  No step is under a condition of the element: elements that take
+ * no part have a digit of their own (with branches a tile took 2.5 times as many instructions). */
 template <int THREADS, int ITEMS>
 __device__ __forceinline__ uint32_t sort_tile(SortShared<THREADS, ITEMS> &s, const uint32_t (&key)[ITEMS],
                                               const uint32_t (&pos)[ITEMS], const bool (&valid)[ITEMS], int items, int shift,
@@ -430,15 +432,16 @@ __device__ __forceinline__ uint32_t sort_tile(SortShared<THREADS, ITEMS> &s, con
     constexpr int WARPS = THREADS / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t bins = 1u << bits, mask = bins - 1u;
-    for(uint32_t j = threadIdx.x; j < WARPS * bins; j += THREADS) s.hist[j >> bits][j & mask] = 0u;
+    for(uint32_t j = threadIdx.x; j < WARPS * kHistRow; j += THREADS) (&s.hist[0][0])[j] = 0u;
     __syncthreads();
     uint32_t *wh = s.hist[warp];
-    uint32_t rank[ITEMS];
+    uint32_t rank[ITEMS], digit[ITEMS];
 #pragma unroll
     for(int it = 0; it < ITEMS; ++it) {
         if(it < items) {
             const uint32_t d = key[it] >> shift & mask;
-            unsigned peers = __ballot_sync(0xffffffffu, valid[it]);
+            const unsigned all = __ballot_sync(0xffffffffu, valid[it]);
+            unsigned peers = valid[it] ? all : ~all;
 #pragma unroll
             for(int b = 0; b < kMaxBits; ++b) {
                 if(b < bits) {
@@ -446,18 +449,17 @@ __device__ __forceinline__ uint32_t sort_tile(SortShared<THREADS, ITEMS> &s, con
                     peers &= ~(__ballot_sync(0xffffffffu, one != 0) ^ (unsigned)one);
                 }
             }
-            const unsigned lt = peers & ((1u << lane) - 1u);
-            uint32_t before = 0;
-            if(valid[it]) before = wh[d];
-            rank[it] = before + (uint32_t)__popc(lt);
+            digit[it] = valid[it] ? d : bins;
+            const uint32_t before = wh[digit[it]];
+            rank[it] = before + (uint32_t)__popc(peers & ((1u << lane) - 1u));
             __syncwarp();
-            if(valid[it] && lt == 0u) wh[d] = before + (uint32_t)__popc(peers);
+            wh[digit[it]] = before + (uint32_t)__popc(peers); /* the same from every lane of the digit */
             __syncwarp();
         }
     }
     __syncthreads();
     uint32_t count = 0;
-    if(threadIdx.x < bins) {
+    if(threadIdx.x <= bins) {
         uint32_t c[WARPS];
 #pragma unroll
         for(int w = 0; w < WARPS; ++w) c[w] = s.hist[w][threadIdx.x];
@@ -468,14 +470,11 @@ __device__ __forceinline__ uint32_t sort_tile(SortShared<THREADS, ITEMS> &s, con
         }
     }
     const uint32_t upto = block_inclusive_scan(count, s.warp, nullptr);
-    if(threadIdx.x < bins) s.before[threadIdx.x] = upto - count;
+    if(threadIdx.x <= bins) s.before[threadIdx.x] = upto - count;
     __syncthreads();
 #pragma unroll
     for(int it = 0; it < ITEMS; ++it)
-        if(it < items && valid[it]) {
-            const uint32_t d = key[it] >> shift & mask;
-            s.pair[s.before[d] + wh[d] + rank[it]] = make_uint2(key[it], pos[it]);
-        }
+        if(it < items) s.pair[s.before[digit[it]] + wh[digit[it]] + rank[it]] = make_uint2(key[it], pos[it]);
     __syncthreads();
     return count;
 }
@@ -498,14 +497,17 @@ __global__ void __launch_bounds__(kSmallThreads) small_sort_kernel(const I *__re
 #pragma unroll
     for(int it = 0; it < kSmallItems; ++it) {
         p[it] = wbase + (uint32_t)it * 32u;
-        raw[it] = it < items && p[it] < count ? __ldg(index + p[it]) : (I)0;
+        valid[it] = it < items && p[it] < count;
+        raw[it] = count > 0 ? __ldg(index + (valid[it] ? p[it] : 0u)) : (I)0;
     }
+    bool outside = false;
 #pragma unroll
     for(int it = 0; it < kSmallItems; ++it) {
-        k[it] = (uint32_t)raw[it];
-        valid[it] = it < items && p[it] < count && takes_part(raw[it], use);
+        valid[it] &= takes_part(valid[it] ? raw[it] : (I)0, use, outside);
+        k[it] = valid[it] ? (uint32_t)raw[it] : 0u;
         used += valid[it];
     }
+    if(outside && use.bad != nullptr) atomicExch(use.bad, 1u);
     uint32_t n;
     block_inclusive_scan(used, s.warp, &n);
     if(threadIdx.x == 0) *n_sorted = n;
@@ -519,9 +521,10 @@ __global__ void __launch_bounds__(kSmallThreads) small_sort_kernel(const I *__re
         for(int it = 0; it < kSmallItems; ++it) {
             const uint32_t i = wbase + (uint32_t)it * 32u;
             valid[it] = it < items && i < n;
-            if(valid[it]) {
-                k[it] = s.pair[i].x;
-                p[it] = s.pair[i].y;
+            if(it < items) {
+                const uint2 kp = s.pair[i];
+                k[it] = kp.x;
+                p[it] = kp.y;
             }
         }
         __syncthreads();
@@ -558,27 +561,30 @@ __device__ __forceinline__ void load_elements(const I *__restrict__ index, const
                                               uint32_t (&key)[kSortItems], uint32_t (&pos)[kSortItems],
                                               bool (&valid)[kSortItems])
 {
+    const uint32_t last = end - 1; /* elements behind the end are read in its place */
     if(kFirst) {
         I raw[kSortItems];
 #pragma unroll
         for(int it = 0; it < kSortItems; ++it) {
             pos[it] = first + it * step;
-            valid[it] = it < items && pos[it] < end;
-            raw[it] = valid[it] ? __ldg(index + pos[it]) : (I)0;
+            raw[it] = __ldg(index + (pos[it] < last ? pos[it] : last));
         }
+        bool outside = false;
 #pragma unroll
         for(int it = 0; it < kSortItems; ++it) {
-            key[it] = (uint32_t)raw[it];
-            valid[it] = valid[it] && takes_part(raw[it], use);
+            const bool in = it < items && pos[it] < end;
+            valid[it] = takes_part(raw[it], use, outside) && in;
+            key[it] = valid[it] ? (uint32_t)raw[it] : 0u;
         }
+        if(outside && use.bad != nullptr) atomicExch(use.bad, 1u);
         return;
     }
 #pragma unroll
     for(int it = 0; it < kSortItems; ++it) {
         const uint32_t i = first + it * step;
         valid[it] = it < items && i < end;
-        const uint2 kp = valid[it] ? __ldcg(pairs + i) : make_uint2(0u, 0u);
-        key[it] = kp.x;
+        const uint2 kp = __ldcg(pairs + (i < last ? i : last));
+        key[it] = valid[it] ? kp.x : 0u;
         pos[it] = kp.y;
     }
 }
@@ -591,9 +597,9 @@ __global__ void __launch_bounds__(kSortThreads) digit_count_kernel(const I *__re
                                                                    int shift, int bits, uint32_t *__restrict__ counts,
                                                                    const Table table, uint32_t dim)
 {
-    __shared__ uint32_t s_hist[kMaxBins];
+    __shared__ uint32_t s_hist[kHistRow];
     const uint32_t bins = 1u << bits;
-    for(uint32_t j = threadIdx.x; j < bins; j += kSortThreads) s_hist[j] = 0u;
+    for(uint32_t j = threadIdx.x; j <= bins; j += kSortThreads) s_hist[j] = 0u;
     __syncthreads();
     gsx_pdl_trigger();
     if(!kFirst) gsx_pdl_wait();
@@ -605,7 +611,7 @@ __global__ void __launch_bounds__(kSortThreads) digit_count_kernel(const I *__re
         load_elements<I, kFirst>(index, pairs, i0 + threadIdx.x, kSortThreads, kSortItems, end, use, key, pos, in);
 #pragma unroll
         for(int it = 0; it < kSortItems; ++it)
-            if(in[it]) atomicAdd(&s_hist[key[it] >> shift & (bins - 1u)], 1u);
+            atomicAdd(&s_hist[in[it] ? key[it] >> shift & (bins - 1u) : bins], 1u);
     }
     __syncthreads();
     for(uint32_t j = threadIdx.x; j < bins; j += kSortThreads) counts[blockIdx.x * bins + j] = s_hist[j];
@@ -638,7 +644,7 @@ __global__ void __launch_bounds__(kSortThreads) digit_scatter_kernel(const I *__
             all += v;
             before += c < blockIdx.x ? v : 0u;
         }
-        uint32_t *s_all = &s.hist[0][0], *s_before = s_all + kSortThreads;
+        uint32_t *s_all = &s.hist[0][0], *s_before = s_all + kSortThreads; /* of kSortThreads each */
         s_all[threadIdx.x] = all;
         s_before[threadIdx.x] = before;
         __syncthreads();

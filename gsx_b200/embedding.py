@@ -8,30 +8,26 @@ from ._tensors import (FLOAT_TYPES, INDEX_TYPES, below_2_31, empty, invalid, lau
                        word)
 
 
-def _check_table(table, name):
-    if table.dim() != 2:
-        raise invalid(f"{name} must be [rows, dim]")
-    below_2_31(rows=table.shape[0], dim=table.shape[1])
-
-
 def embedding_lookup(table, index, out=None, scale: float = 1.0, bad=None, stream=None):
     """out[n] = scale * table[index[n]] for a [rows, dim] table and an index tensor of any shape; out is
     index.shape + (dim,), of the table's type unless given (float32, float16 or bfloat16 each).  Rows may be
     strided.  An index outside the table sets the one-word tensor `bad` to 1 (where given) and leaves its row."""
-    _check_table(table, "table")
+    if table.dim() != 2:
+        raise invalid("table must be [rows, dim]")
     rows, dim = table.shape
     device = table.device
-    on_device(device, index=index, out=out, bad=bad)
+    on_device(device, index, out, bad)
     if not index.is_contiguous():
         raise invalid("index must be contiguous")
-    below_2_31(count=index.numel())
+    count = index.numel()
+    below_2_31(rows, dim, count)
     if out is None:
         out = empty((*index.shape, dim), table.dtype, device, stream)
-    elif out.shape != (*index.shape, dim):
+    elif out.shape[:-1] != index.shape or out.shape[-1:] != table.shape[1:]:
         raise invalid(f"out must be {(*index.shape, dim)}, not {tuple(out.shape)}")
     launch(lib().gsx_b200_embedding_lookup, device, stream, table.data_ptr(), type_code(table, FLOAT_TYPES, "table"),
            rows, dim, row_stride(table, dim, "table"), index.data_ptr(), type_code(index, INDEX_TYPES, "index"),
-           index.numel(), scale, out.data_ptr(), type_code(out, FLOAT_TYPES, "out"), row_stride(out, dim, "out"),
+           count, scale, out.data_ptr(), type_code(out, FLOAT_TYPES, "out"), row_stride(out, dim, "out"),
            word(bad, "bad"))
     return out
 
@@ -41,15 +37,16 @@ def embedding_backward(grad_out, index, grad_table, scale: float = 1.0, padding_
     """grad_table[v] = scale * sum of grad_out[n] over index[n] = v, written for every row (added to it when
     accumulate), in f32 sums whose order does not depend on the launch.  grad_out is index.shape + (dim,),
     grad_table [rows, dim].  Indices equal to padding_row take no part; out-of-range ones set `bad`."""
-    _check_table(grad_table, "grad_table")
+    if grad_table.dim() != 2:
+        raise invalid("grad_table must be [rows, dim]")
     rows, dim = grad_table.shape
     device = grad_table.device
-    on_device(device, grad_out=grad_out, index=index, bad=bad)
+    on_device(device, grad_out, index, bad)
     if not index.is_contiguous():
         raise invalid("index must be contiguous")
     count = index.numel()
-    below_2_31(count=count)
-    if grad_out.shape != (*index.shape, dim):
+    below_2_31(rows, dim, count)
+    if grad_out.shape[:-1] != index.shape or grad_out.shape[-1:] != grad_table.shape[1:]:
         raise invalid(f"grad_out must be {(*index.shape, dim)}, not {tuple(grad_out.shape)}")
     if padding_row is None:
         padding_row = -1
