@@ -52,11 +52,18 @@ def budget_accumulate(score, weights, out=None, decay: float = 1.0, lengths=None
     rows = weights.shape[-2]
     if length > 1 and weights.stride(-1) != 1:
         raise invalid("the last dimension of weights must be contiguous")
-    below_2_31(groups, rows, length)
+    if (groups | rows | length) >> 31:
+        below_2_31(groups, rows, length)
+    if weights.is_contiguous():
+        group_step, row_step = rows * length, length
+    else:
+        group_step = group_stride(weights, weights.dim() - 2, "weights")
+        row_step = weights.stride(-2) if rows > 1 else length
     launch(lib().gsx_b200_budget_accumulate, device, stream, score.data_ptr(), stride, weights.data_ptr(),
-           type_code(weights, FLOAT_TYPES, "weights"), group_stride(weights, weights.dim() - 2, "weights"),
-           weights.stride(-2) if rows > 1 else length, groups, rows, length, _per_group(lengths, lead, "lengths"),
-           _per_group(row_lengths, lead, "row_lengths"), decay, out.data_ptr(), _score(out, "out")[2])
+           type_code(weights, FLOAT_TYPES, "weights"), group_step, row_step, groups, rows, length,
+           None if lengths is None else _per_group(lengths, lead, "lengths"),
+           None if row_lengths is None else _per_group(row_lengths, lead, "row_lengths"), decay, out.data_ptr(),
+           length if out.is_contiguous() and out.dtype == torch.float32 else _score(out, "out")[2])
     return out
 
 
@@ -68,7 +75,8 @@ def budget_select(score, budget: int, lengths=None, first: int = 0, recent: int 
     drop, where given, int32 of score's shape, receives the others.  Places behind the lists are left as they were."""
     groups, length, stride = _score(score)
     lead = score.shape[:-1]
-    below_2_31(groups, length, budget)
+    if (groups | length | budget) >> 31:
+        below_2_31(groups, length, budget)
     if first < 0 or recent < 0:
         raise GsxError(OUT_OF_RANGE, "first and recent must not be negative")
     if first + recent > budget:
@@ -88,7 +96,8 @@ def budget_select(score, budget: int, lengths=None, first: int = 0, recent: int 
     size = L.gsx_b200_budget_workspace_bytes(groups, length)
     workspace = empty((size,), torch.uint8, device, stream) if size else None
     launch(L.gsx_b200_budget_select, device, stream, score.data_ptr(), stride, groups, length,
-           _per_group(lengths, lead, "lengths"), first, recent, budget, keep.data_ptr(), keep.shape[-1],
+           None if lengths is None else _per_group(lengths, lead, "lengths"), first, recent, budget, keep.data_ptr(),
+           keep.shape[-1],
            _per_group(kept, lead, "kept"), None if drop is None else drop.data_ptr(), length,
            None if workspace is None else workspace.data_ptr(), size)
     return keep, kept

@@ -22,6 +22,7 @@
 
 #include "gsx_detmath.h"
 
+#include <atomic>
 #include <utility>
 
 /* Programmatic dependent launch (sm_90+): a kernel launched with gsx_launch_pdl may start while the
@@ -47,6 +48,20 @@ cudaError_t gsx_launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+/* Lets `kernel` be launched with `bytes` of dynamic shared memory on the current device: asked of the runtime once a
+ * kernel and device (always with the same number). */
+template <auto kernel>
+cudaError_t gsx_allow_smem(size_t bytes)
+{
+    static std::atomic<bool> done[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if(e != cudaSuccess || (dev < 64 && done[dev].load(std::memory_order_relaxed))) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if(e == cudaSuccess && dev < 64) done[dev].store(true, std::memory_order_relaxed);
+    return e;
 }
 
 #define GSX_TILE 16

@@ -54,13 +54,19 @@ __device__ __forceinline__ uint32_t length_of(const int32_t *__restrict__ length
 
 constexpr int kAccumulateCtas = 4; /* an SM */
 
-/* U rows, hop elements apart, all in flight before the first is added */
-template <typename T, int VW, int U>
-__device__ __forceinline__ void add_rows(float (&acc)[VW], const T *__restrict__ w, uint64_t hop)
+/* U rows, hop elements apart, all in flight before the first is added: packs of VW elements, or (SPREAD) single elements
+ * at VW places `apart` from the first */
+template <typename T, int VW, int U, bool SPREAD>
+__device__ __forceinline__ void add_rows(float (&acc)[VW], const T *__restrict__ w, uint64_t hop, const uint32_t (&apart)[VW])
 {
     Pack<T, VW> x[U];
 #pragma unroll
-    for(int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const Pack<T, VW> *>(w + u * hop);
+    for(int u = 0; u < U; ++u) {
+        if(SPREAD)
+#pragma unroll
+            for(int v = 0; v < VW; ++v) x[u].v[v] = (w + u * hop)[apart[v]];
+        else x[u] = *reinterpret_cast<const Pack<T, VW> *>(w + u * hop);
+    }
 #pragma unroll
     for(int u = 0; u < U; ++u)
 #pragma unroll
@@ -69,8 +75,9 @@ __device__ __forceinline__ void add_rows(float (&acc)[VW], const T *__restrict__
 
 /* A cluster of CTAs owns kThreads / RG * VW columns of one group and deals their rows out: row r goes to CTA
  * (r / RG) mod clusters, thread row r mod RG.  A thread keeps U rows in flight; the RG threads of a column are joined in
- * shared memory, the CTAs in distributed shared memory, each in a fixed order. */
-template <typename T, int VW, int RG>
+ * shared memory, the CTAs in distributed shared memory, each in a fixed order.  SPREAD, for rows that no 4-byte access
+ * fits: a thread's VW columns lie CT apart, so that the lanes' single elements stay side by side. */
+template <typename T, int VW, int RG, bool SPREAD>
 __global__ void __launch_bounds__(kThreads, kAccumulateCtas) accumulate_kernel(const float *score, uint64_t score_stride,
                                                               const T *__restrict__ weights, uint64_t group_stride,
                                                               uint64_t row_stride, uint32_t groups, uint32_t rows,
@@ -79,38 +86,37 @@ __global__ void __launch_bounds__(kThreads, kAccumulateCtas) accumulate_kernel(c
                                                               float *out, uint64_t out_stride)
 {
     constexpr int CT = kThreads / RG;
-    constexpr int U = VW == 1 && sizeof(T) == 2 ? 16 : 8;
+    constexpr int U = 8;
     __shared__ float s_part[RG * CT * VW];
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t splits = cluster.num_blocks(), split = cluster.block_rank();
     const int ct = threadIdx.x % CT, rg = threadIdx.x / CT;
-    const uint32_t step = RG * splits, j = (blockIdx.x / splits * (uint32_t)CT + (uint32_t)ct) * VW;
+    const uint32_t step = RG * splits, c0 = blockIdx.x / splits * (uint32_t)(CT * VW);
+    const uint32_t j = SPREAD ? c0 + (uint32_t)ct : c0 + (uint32_t)ct * VW; /* the thread's first column */
     for(uint32_t g = blockIdx.y; g < groups; g += gridDim.y) {
         const uint32_t n = length_of(lengths, g, length);
         const uint32_t nr = length_of(row_lengths, g, rows);
         float acc[VW] = {};
         if(j < n) {
+            uint32_t apart[VW]; /* columns that are not in use are read in the place of the last */
+#pragma unroll
+            for(int v = 0; v < VW; ++v) apart[v] = j + v * CT < n ? v * CT : n - 1 - j;
             const T *w = weights + (uint64_t)g * group_stride + j + (uint64_t)(split * RG + (uint32_t)rg) * row_stride;
             const uint64_t hop = (uint64_t)step * row_stride;
             /* rows of this thread */
             int left = nr > split * RG + (uint32_t)rg ? (int)((nr - split * RG - (uint32_t)rg + step - 1) / step) : 0;
-            for(; left >= U; left -= U, w += U * hop) add_rows<T, VW, U>(acc, w, hop);
-            if(U > 8 && left >= 8) {
-                add_rows<T, VW, 8>(acc, w, hop);
-                left -= 8;
-                w += 8 * hop;
-            }
+            for(; left >= U; left -= U, w += U * hop) add_rows<T, VW, U, SPREAD>(acc, w, hop, apart);
             if(left >= 4) {
-                add_rows<T, VW, 4>(acc, w, hop);
+                add_rows<T, VW, 4, SPREAD>(acc, w, hop, apart);
                 left -= 4;
                 w += 4 * hop;
             }
             if(left >= 2) {
-                add_rows<T, VW, 2>(acc, w, hop);
+                add_rows<T, VW, 2, SPREAD>(acc, w, hop, apart);
                 left -= 2;
                 w += 2 * hop;
             }
-            if(left) add_rows<T, VW, 1>(acc, w, hop);
+            if(left) add_rows<T, VW, 1, SPREAD>(acc, w, hop, apart);
         }
         if(RG > 1 || splits > 1) {
             __syncthreads();
@@ -141,14 +147,14 @@ __global__ void __launch_bounds__(kThreads, kAccumulateCtas) accumulate_kernel(c
         float *to = out + (uint64_t)g * out_stride;
 #pragma unroll
         for(int v = 0; v < VW; ++v) {
-            const uint32_t c = j + v;
+            const uint32_t c = SPREAD ? j + v * CT : j + v;
             if(c < n) to[c] = decay == 0.0f ? acc[v] : fmaf(decay, in[c], acc[v]);
             else if(c < length && to != in) to[c] = in[c];
         }
     }
 }
 
-template <typename T, int VW, int RG>
+template <typename T, int VW, int RG, bool SPREAD>
 cudaError_t launch_accumulate_rg(const float *score, uint64_t score_stride, const T *weights, uint64_t group_stride,
                                  uint64_t row_stride, uint32_t groups, uint32_t rows, uint32_t length,
                                  const int32_t *lengths, const int32_t *row_lengths, float decay, float *out,
@@ -170,23 +176,30 @@ cudaError_t launch_accumulate_rg(const float *score, uint64_t score_stride, cons
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, accumulate_kernel<T, VW, RG>, score, score_stride, weights, group_stride, row_stride, groups,
-                              rows, length, lengths, row_lengths, decay, out, out_stride);
+    return cudaLaunchKernelEx(&cfg, accumulate_kernel<T, VW, RG, SPREAD>, score, score_stride, weights, group_stride, row_stride,
+                              groups, rows, length, lengths, row_lengths, decay, out, out_stride);
 }
 
-template <typename T, int VW>
-cudaError_t launch_accumulate(const float *score, uint64_t score_stride, const void *weights, uint64_t group_stride,
+/* `unit`: the widest access in bytes (up to 16) that every row's start and the length are multiples of */
+template <typename T>
+cudaError_t launch_accumulate(uint64_t unit, const float *score, uint64_t score_stride, const void *weights, uint64_t group_stride,
                               uint64_t row_stride, uint32_t groups, uint32_t rows, uint32_t length, const int32_t *lengths,
                               const int32_t *row_lengths, float decay, float *out, uint64_t out_stride, cudaStream_t stream)
 {
-    const T *w = static_cast<const T *>(weights);
+    auto run = [&](auto launch) {
+        return launch(score, score_stride, static_cast<const T *>(weights), group_stride, row_stride, groups, rows, length, lengths,
+                      row_lengths, decay, out, out_stride, stream);
+    };
     /* many rows: fewer columns to a CTA, whose threads share them (512 bytes of a row a CTA where it reads packs) */
-    constexpr int RG = VW > 1 ? 8 : 2;
-    if(rows >= 32)
-        return launch_accumulate_rg<T, VW, RG>(score, score_stride, w, group_stride, row_stride, groups, rows, length, lengths,
-                                               row_lengths, decay, out, out_stride, stream);
-    return launch_accumulate_rg<T, VW, 1>(score, score_stride, w, group_stride, row_stride, groups, rows, length, lengths,
-                                          row_lengths, decay, out, out_stride, stream);
+    constexpr int W = 16 / sizeof(T);
+    const bool many = rows >= 32;
+    if(unit == 16) return many ? run(launch_accumulate_rg<T, W, 8, false>) : run(launch_accumulate_rg<T, W, 1, false>);
+    if(unit == 8) return many ? run(launch_accumulate_rg<T, W / 2, 4, false>) : run(launch_accumulate_rg<T, W / 2, 1, false>);
+    if(unit == 4 && sizeof(T) == 2) return many ? run(launch_accumulate_rg<T, 2, 2, false>) : run(launch_accumulate_rg<T, 2, 1, false>);
+    if(many) return run(launch_accumulate_rg<T, 4, 4, true>);
+    /* four columns a thread where that still fills the GPU, else one */
+    if((uint64_t)groups * ((length + kThreads * 4 - 1) / (kThreads * 4)) >= 148 * kAccumulateCtas) return run(launch_accumulate_rg<T, 4, 1, true>);
+    return run(launch_accumulate_rg<T, 1, 1, false>);
 }
 
 /* ------------------------------------------------------------------------------------------ */
@@ -820,24 +833,16 @@ extern "C" int gsx_b200_budget_accumulate(const float *score, uint64_t score_str
     if(rows > 0 && overlap(out, out_bytes, weights, es * ((groups - 1) * group_stride + (rows - 1) * row_stride + length)))
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "out must not overlap weights");
     cudaStream_t stream = (cudaStream_t)stream_;
-    const bool vec = (uintptr_t)weights % 16 == 0 && (groups == 1 || group_stride * es % 16 == 0) &&
-                     (rows <= 1 || row_stride * es % 16 == 0) && length * es % 16 == 0;
-#define GSX_ACCUMULATE(T, VW)                                                                                              \
-    e = launch_accumulate<T, VW>(score, score_stride, weights, group_stride, row_stride, (uint32_t)groups, (uint32_t)rows, \
-                                 (uint32_t)length, lengths, row_lengths, decay, out, out_stride, stream)
-    cudaError_t e;
-    if(weight_type == GSX_B200_DATA_F32) {
-        if(vec) GSX_ACCUMULATE(float, 4);
-        else GSX_ACCUMULATE(float, 1);
-    } else if(weight_type == GSX_B200_DATA_F16) {
-        if(vec) GSX_ACCUMULATE(__half, 8);
-        else GSX_ACCUMULATE(__half, 1);
-    } else {
-        if(vec) GSX_ACCUMULATE(__nv_bfloat16, 8);
-        else GSX_ACCUMULATE(__nv_bfloat16, 1);
-    }
-#undef GSX_ACCUMULATE
-    return launch_status(e);
+    const uint64_t all = (uint64_t)(uintptr_t)weights | length * es | (groups > 1 ? group_stride * es : 0) | (rows > 1 ? row_stride * es : 0);
+    uint64_t unit = 16;
+    while(all % unit) unit /= 2;
+    auto run = [&](auto launch) {
+        return launch_status(launch(unit, score, score_stride, weights, group_stride, row_stride, (uint32_t)groups, (uint32_t)rows,
+                                    (uint32_t)length, lengths, row_lengths, decay, out, out_stride, stream));
+    };
+    if(weight_type == GSX_B200_DATA_F32) return run(launch_accumulate<float>);
+    if(weight_type == GSX_B200_DATA_F16) return run(launch_accumulate<__half>);
+    return run(launch_accumulate<__nv_bfloat16>);
 }
 
 extern "C" uint64_t gsx_b200_budget_workspace_bytes(uint64_t groups, uint64_t length)
@@ -886,7 +891,7 @@ extern "C" int gsx_b200_budget_select(const float *score, uint64_t score_stride,
         while(ctas < 8 && (length > (uint64_t)ctas * kCtaKeys || (groups * ctas * 2 <= 148 * 2 && length >= (uint64_t)ctas * 2 * 2048)))
             ctas *= 2;
         const size_t part = ((length + ctas - 1) / ctas + 3) / 4 * 4;
-        cudaError_t e = cudaFuncSetAttribute(select_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kCtaKeys * 4));
+        cudaError_t e = gsx_allow_smem<select_cluster_kernel>(kCtaKeys * 4);
         if(e != cudaSuccess) return launch_status(e);
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)(groups * ctas));

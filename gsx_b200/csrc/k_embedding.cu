@@ -247,8 +247,7 @@ cudaError_t launch_short(const T *table, uint32_t rows, uint32_t stride_bytes, c
     const size_t bytes = (size_t)rows * DIM * sizeof(O);
     /* a small table that is read many times over: each of two CTAs an SM copies it to shared memory once */
     if(bytes <= kShortTable && count >= (uint64_t)rows * 64 && count >= (1u << 18)) {
-        const cudaError_t e = cudaFuncSetAttribute(lookup_short_kernel<T, O, I, DIM, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   (int)kShortTable);
+        const cudaError_t e = gsx_allow_smem<lookup_short_kernel<T, O, I, DIM, true>>(kShortTable);
         if(e != cudaSuccess) return e;
         lookup_short_kernel<T, O, I, DIM, true><<<148 * 2, 1024, bytes, stream>>>(table, rows, stride_bytes, index, count, scale, out, bad);
         return cudaSuccess;
@@ -429,6 +428,7 @@ __device__ __forceinline__ uint32_t sort_tile(SortShared<THREADS, ITEMS> &s, con
                                               const uint32_t (&pos)[ITEMS], const bool (&valid)[ITEMS], int items, int shift,
                                               int bits)
 {
+    static_assert(THREADS >= kMaxBins, "a thread to each digit");
     constexpr int WARPS = THREADS / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t bins = 1u << bits, mask = bins - 1u;
@@ -458,19 +458,25 @@ __device__ __forceinline__ uint32_t sort_tile(SortShared<THREADS, ITEMS> &s, con
         }
     }
     __syncthreads();
-    uint32_t count = 0;
-    if(threadIdx.x <= bins) {
-        uint32_t c[WARPS];
+    /* counts -> places before each warp's, for every digit and the one of the elements that take no part; that is the last
+     * and may find no thread of its own */
+    auto warps_before = [&](uint32_t d) {
+        uint32_t c[WARPS], sum = 0;
 #pragma unroll
-        for(int w = 0; w < WARPS; ++w) c[w] = s.hist[w][threadIdx.x];
+        for(int w = 0; w < WARPS; ++w) c[w] = s.hist[w][d];
 #pragma unroll
         for(int w = 0; w < WARPS; ++w) {
-            s.hist[w][threadIdx.x] = count;
-            count += c[w];
+            s.hist[w][d] = sum;
+            sum += c[w];
         }
-    }
-    const uint32_t upto = block_inclusive_scan(count, s.warp, nullptr);
-    if(threadIdx.x <= bins) s.before[threadIdx.x] = upto - count;
+        return sum;
+    };
+    const uint32_t count = threadIdx.x < bins ? warps_before(threadIdx.x) : 0u;
+    if(threadIdx.x == THREADS - 1) warps_before(bins);
+    uint32_t total;
+    const uint32_t upto = block_inclusive_scan(count, s.warp, &total);
+    if(threadIdx.x < bins) s.before[threadIdx.x] = upto - count;
+    if(threadIdx.x == THREADS - 1) s.before[bins] = total;
     __syncthreads();
 #pragma unroll
     for(int it = 0; it < ITEMS; ++it)
@@ -553,25 +559,25 @@ __device__ __forceinline__ void chunk_range(uint32_t n, uint32_t &begin, uint32_
     end = n - begin < len ? n : begin + len;
 }
 
-/* Up to kSortItems elements of a pass's input, at first + it * step below end: of the indices themselves in the
+/* Up to ITEMS elements of a pass's input, at first + it * step below end: of the indices themselves in the
  * first pass (kFirst), of sorted pairs else.  All loads are issued before the first is looked at. */
-template <typename I, bool kFirst>
+template <typename I, bool kFirst, int ITEMS>
 __device__ __forceinline__ void load_elements(const I *__restrict__ index, const uint2 *__restrict__ pairs, uint32_t first,
                                               uint32_t step, int items, uint32_t end, const Use &use,
-                                              uint32_t (&key)[kSortItems], uint32_t (&pos)[kSortItems],
-                                              bool (&valid)[kSortItems])
+                                              uint32_t (&key)[ITEMS], uint32_t (&pos)[ITEMS],
+                                              bool (&valid)[ITEMS])
 {
     const uint32_t last = end - 1; /* elements behind the end are read in its place */
     if(kFirst) {
-        I raw[kSortItems];
+        I raw[ITEMS];
 #pragma unroll
-        for(int it = 0; it < kSortItems; ++it) {
+        for(int it = 0; it < ITEMS; ++it) {
             pos[it] = first + it * step;
             raw[it] = __ldg(index + (pos[it] < last ? pos[it] : last));
         }
         bool outside = false;
 #pragma unroll
-        for(int it = 0; it < kSortItems; ++it) {
+        for(int it = 0; it < ITEMS; ++it) {
             const bool in = it < items && pos[it] < end;
             valid[it] = takes_part(raw[it], use, outside) && in;
             key[it] = valid[it] ? (uint32_t)raw[it] : 0u;
@@ -580,7 +586,7 @@ __device__ __forceinline__ void load_elements(const I *__restrict__ index, const
         return;
     }
 #pragma unroll
-    for(int it = 0; it < kSortItems; ++it) {
+    for(int it = 0; it < ITEMS; ++it) {
         const uint32_t i = first + it * step;
         valid[it] = it < items && i < end;
         const uint2 kp = __ldcg(pairs + (i < last ? i : last));
@@ -608,7 +614,7 @@ __global__ void __launch_bounds__(kSortThreads) digit_count_kernel(const I *__re
     for(uint32_t i0 = begin; i0 < end; i0 += kTile) {
         uint32_t key[kSortItems], pos[kSortItems];
         bool in[kSortItems];
-        load_elements<I, kFirst>(index, pairs, i0 + threadIdx.x, kSortThreads, kSortItems, end, use, key, pos, in);
+        load_elements<I, kFirst, kSortItems>(index, pairs, i0 + threadIdx.x, kSortThreads, kSortItems, end, use, key, pos, in);
 #pragma unroll
         for(int it = 0; it < kSortItems; ++it)
             atomicAdd(&s_hist[in[it] ? key[it] >> shift & (bins - 1u) : bins], 1u);
@@ -666,7 +672,7 @@ __global__ void __launch_bounds__(kSortThreads) digit_scatter_kernel(const I *__
         const int items = end - i0 >= (uint32_t)kTile ? kSortItems : (int)((end - i0 + kSortThreads - 1) / kSortThreads);
         uint32_t k[kSortItems], p[kSortItems];
         bool valid[kSortItems];
-        load_elements<I, kFirst>(index, pairs, i0 + (uint32_t)(warp * 32 * items + lane), 32, items, end, use, k, p, valid);
+        load_elements<I, kFirst, kSortItems>(index, pairs, i0 + (uint32_t)(warp * 32 * items + lane), 32, items, end, use, k, p, valid);
         const uint32_t c = sort_tile(s, k, p, valid, items, shift, bits);
         if(threadIdx.x < bins) {
             s_to[threadIdx.x] = s_place[threadIdx.x] - s.before[threadIdx.x];
@@ -900,12 +906,145 @@ __global__ void __launch_bounds__(kThreads) row_join_kernel(const Runs a, const 
 }
 
 /* ------------------------------------------------------------------------------------------ */
+/* Small tables of short rows (a codebook of colours) and many positions: the positions need not be sorted as a whole.
+ * A CTA keeps a table of sums in shared memory and walks a chunk of the positions in tiles: it ranks a tile by the low
+ * 8 bits of the row, and thread t adds up the positions of the rows that end in t, in order.  The CTAs' tables are then
+ * added up in the order of the chunks.  Lists of more than kOwnLong positions are walked by a warp, 32 at a time. */
+constexpr int kOwnThreads = 256;
+constexpr int kOwnItems = 16;
+constexpr uint32_t kOwnTile = kOwnThreads * kOwnItems;
+constexpr uint64_t kOwnDim = 16;
+constexpr size_t kOwnTable = 68 * 1024; /* two CTAs an SM */
+constexpr uint32_t kOwnLong = 64;
+constexpr int kOwnCols = 4; /* columns of a walk */
+static_assert(kOwnThreads == kMaxBins, "thread t owns digit t");
+
+template <typename GT, typename I>
+__global__ void __launch_bounds__(kOwnThreads, 2) own_table_kernel(const GT *__restrict__ grad, uint32_t stride_bytes,
+                                                                   const I *__restrict__ index, uint32_t count, const Use use,
+                                                                   uint32_t dim, float *__restrict__ partial)
+{
+    using Shared = SortShared<kOwnThreads, kOwnItems>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    Shared &s = *reinterpret_cast<Shared *>(smem);
+    float *table = reinterpret_cast<float *>(smem + sizeof(Shared));
+    __shared__ uint32_t s_count[kOwnThreads];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t size = use.rows * dim;
+    for(uint32_t j = threadIdx.x; j < size; j += kOwnThreads) table[j] = 0.0f;
+    const unsigned char *bytes = reinterpret_cast<const unsigned char *>(grad);
+    uint32_t begin, end;
+    chunk_range(count, begin, end);
+    for(uint32_t i0 = begin; i0 < end; i0 += kOwnTile) {
+        const int items = end - i0 >= kOwnTile ? kOwnItems : (int)((end - i0 + kOwnThreads - 1) / kOwnThreads);
+        uint32_t k[kOwnItems], p[kOwnItems];
+        bool valid[kOwnItems];
+        load_elements<I, true, kOwnItems>(index, nullptr, i0 + (uint32_t)(warp * 32 * items + lane), 32, items, end, use, k, p, valid);
+        s_count[threadIdx.x] = sort_tile(s, k, p, valid, items, 0, kMaxBits);
+        __syncthreads();
+        for(uint32_t c0 = 0; c0 < dim; c0 += kOwnCols) {
+            const uint32_t cols = dim - c0 < (uint32_t)kOwnCols ? dim - c0 : kOwnCols;
+            const GT *from[kOwnCols]; /* columns that are not there are read in the place of the first */
+#pragma unroll
+            for(int c = 0; c < kOwnCols; ++c) from[c] = reinterpret_cast<const GT *>(bytes) + c0 + ((uint32_t)c < cols ? c : 0);
+            auto load = [&](GT(&x)[kOwnCols], uint32_t pos) {
+#pragma unroll
+                for(int c = 0; c < kOwnCols; ++c)
+                    x[c] = *reinterpret_cast<const GT *>(reinterpret_cast<const unsigned char *>(from[c]) + (uint64_t)pos * stride_bytes);
+            };
+            const uint32_t first = s.before[threadIdx.x], n = s_count[threadIdx.x];
+            if(n <= kOwnLong)
+                for(uint32_t j = 0; j < n; j += 4) {
+                    uint2 kp[4];
+                    GT x[4][kOwnCols];
+#pragma unroll
+                    for(uint32_t u = 0; u < 4; ++u) kp[u] = s.pair[first + (j + u < n ? j + u : n - 1)];
+#pragma unroll
+                    for(uint32_t u = 0; u < 4; ++u) load(x[u], kp[u].y);
+#pragma unroll
+                    for(uint32_t u = 0; u < 4; ++u)
+                        if(j + u < n) {
+                            float *to = table + kp[u].x * dim + c0;
+#pragma unroll
+                            for(int c = 0; c < kOwnCols; ++c)
+                                if((uint32_t)c < cols) to[c] += to_f32(x[u][c]);
+                        }
+                }
+            /* the long lists, dealt to the warps: the sums of a step's distinct rows one after another */
+            for(int t = warp; t < kOwnThreads; t += kOwnThreads / 32) {
+                const uint32_t m = s_count[t], at = s.before[t];
+                if(m <= kOwnLong) continue;
+                for(uint32_t j = 0; j < m; j += 32) {
+                    const bool in = j + lane < m;
+                    const uint2 kp = s.pair[at + (in ? j + lane : m - 1)];
+                    GT x[kOwnCols];
+                    load(x, kp.y);
+                    unsigned rest = __ballot_sync(0xffffffffu, in);
+                    while(rest != 0u) {
+                        const uint32_t row = __shfl_sync(0xffffffffu, kp.x, __ffs(rest) - 1);
+                        const bool mine = in && kp.x == row;
+                        float v[kOwnCols];
+#pragma unroll
+                        for(int c = 0; c < kOwnCols; ++c) {
+                            v[c] = mine ? to_f32(x[c]) : 0.0f;
+#pragma unroll
+                            for(int o = 16; o > 0; o >>= 1) v[c] += __shfl_xor_sync(0xffffffffu, v[c], o);
+                        }
+                        if((uint32_t)lane < cols)
+                            table[row * dim + c0 + lane] += lane == 0 ? v[0] : lane == 1 ? v[1] : lane == 2 ? v[2] : v[3];
+                        rest &= ~__ballot_sync(0xffffffffu, mine);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        __syncthreads();
+    }
+    __syncthreads();
+    for(uint32_t j = threadIdx.x; j < size; j += kOwnThreads) partial[(uint64_t)blockIdx.x * size + j] = table[j];
+}
+
+/* the chunks' tables added up: 32 elements a CTA, an eighth of the chunks a warp */
+template <typename TT>
+__global__ void __launch_bounds__(kThreads) own_join_kernel(const float *partial, uint32_t size, uint32_t chunks, uint32_t dim,
+                                                            const Table table)
+{
+    __shared__ float s_part[kWarps][32];
+    gsx_pdl_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t j = blockIdx.x * 32 + lane, per = (chunks + kWarps - 1) / kWarps;
+    const uint32_t c0 = per * warp < chunks ? per * warp : chunks, c1 = c0 + per < chunks ? c0 + per : chunks;
+    const float *from = partial + (j < size ? j : size - 1);
+    float sum[1] = { 0.0f };
+#pragma unroll 8
+    for(uint32_t c = c0; c < c1; ++c) sum[0] += __ldcg(from + (uint64_t)c * size);
+    s_part[warp][lane] = sum[0];
+    __syncthreads();
+    if(warp != 0 || j >= size) return;
+#pragma unroll
+    for(int w = 1; w < kWarps; ++w) sum[0] += s_part[w][lane];
+    store_sums<TT, 1>(table, j / dim, j % dim, sum);
+}
+
+/* Chunks of a call that takes this path, or 0: the table fits, and there are enough positions for half the GPU's CTAs
+ * with tables that cost no more to write and read than the gradients. */
+uint32_t own_chunks(uint64_t count, uint64_t rows, uint64_t dim)
+{
+    if(dim > kOwnDim || rows * dim * 4 > kOwnTable) return 0;
+    uint64_t chunks = count / kOwnTile, most = count / (2 * rows);
+    if(chunks > most) chunks = most;
+    if(chunks < 148) return 0;
+    return (uint32_t)(chunks < 296 ? chunks : 296);
+}
+
+/* ------------------------------------------------------------------------------------------ */
 /* workspace: n_sorted | counts | pairs, pairs | sums of rows across CTAs */
 
 struct Plan {
     int passes = 0; /* 0: the one-CTA sort */
     int bits[4] = {};
     uint32_t chunks = 0;
+    uint32_t own = 0; /* chunks of the path with tables in shared memory */
     /* the sums */
     int clog = 0, nr = 1, run = 8;
     uint32_t ctas = 0, tiles = 1;
@@ -949,6 +1088,12 @@ Plan make_plan(uint64_t count, uint64_t rows, uint64_t dim, uint64_t vec)
 {
     Plan p;
     size_t o = 256;
+    p.own = own_chunks(count, rows, dim);
+    if(p.own) {
+        p.o_head = o;
+        p.bytes = o + sizeof(float) * p.own * rows * dim;
+        return p;
+    }
     if(count > (uint64_t)kSmallCount) {
         int bits = 1;
         while(bits < 32 && (rows - 1) >> bits) ++bits;
@@ -975,19 +1120,13 @@ Plan make_plan(uint64_t count, uint64_t rows, uint64_t dim, uint64_t vec)
     return p;
 }
 
-template <typename K>
-cudaError_t allow_smem(K kernel, size_t bytes)
-{
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-}
-
 template <typename I, bool kFirst>
 cudaError_t launch_pass(const I *index, const uint2 *pairs, uint32_t count, uint32_t *n_sorted, const Use &use, int shift,
                         int bits, uint32_t chunks, uint32_t *counts, uint2 *out, const Table &table, uint32_t dim,
                         cudaStream_t stream)
 {
     constexpr size_t smem = sizeof(SortShared<kSortThreads, kSortItems>);
-    cudaError_t e = allow_smem(digit_scatter_kernel<I, kFirst>, smem);
+    cudaError_t e = gsx_allow_smem<digit_scatter_kernel<I, kFirst>>(smem);
     if(e != cudaSuccess) return e;
     if(kFirst)
         digit_count_kernel<I, true><<<chunks, kSortThreads, 0, stream>>>(index, pairs, count, n_sorted, use, shift, bits,
@@ -1014,7 +1153,7 @@ cudaError_t launch_sort(const Plan &plan, unsigned char *ws, const void *index_,
     if(plan.passes == 0) {
         *out_pairs = pairs[0];
         constexpr size_t smem = sizeof(SortShared<kSmallThreads, kSmallItems>);
-        cudaError_t e = allow_smem(small_sort_kernel<I>, smem);
+        cudaError_t e = gsx_allow_smem<small_sort_kernel<I>>(smem);
         if(e != cudaSuccess) return e;
         small_sort_kernel<I><<<1, kSmallThreads, smem, stream>>>(index, count, use, pairs[0], n_sorted);
         if(!table.accumulate) {
@@ -1043,7 +1182,7 @@ cudaError_t launch_runs(const GT *grad, uint64_t stride, const Plan &plan, const
                         cudaStream_t stream)
 {
     const size_t fixed = sizeof(float) * 2 * kThreads * NR * VW;
-    const cudaError_t e = allow_smem(run_sum_kernel<GT, TT, VW, NR>, fixed + sizeof(uint2) * (kMaxPositions + kThreads / 4));
+    const cudaError_t e = gsx_allow_smem<run_sum_kernel<GT, TT, VW, NR>>(fixed + sizeof(uint2) * (kMaxPositions + kThreads / 4));
     if(e != cudaSuccess) return e;
     return gsx_launch_pdl(run_sum_kernel<GT, TT, VW, NR>, dim3(plan.ctas, plan.tiles), dim3(kThreads),
                           fixed + sizeof(uint2) * (size_t)(kThreads >> plan.clog) * (plan.run + 1), stream, grad,
@@ -1068,6 +1207,20 @@ cudaError_t launch_sums(const void *grad_, uint64_t stride, uint64_t vec, const 
     if(e == cudaSuccess && plan.ctas > 1)
         e = gsx_launch_pdl(row_join_kernel<TT>, dim3(plan.ctas - 1, (runs.dim + 255) / 256), dim3(kThreads), 0, stream, runs, table);
     return e;
+}
+
+template <typename GT, typename TT, typename I>
+cudaError_t launch_own(const void *grad, uint64_t stride, const void *index, uint32_t count, const Use &use, const Plan &plan,
+                       float *partial, const Table &table, uint32_t dim, cudaStream_t stream)
+{
+    constexpr size_t shared = sizeof(SortShared<kOwnThreads, kOwnItems>);
+    const cudaError_t e = gsx_allow_smem<own_table_kernel<GT, I>>(shared + kOwnTable);
+    if(e != cudaSuccess) return e;
+    const uint32_t size = (uint32_t)table.rows * dim;
+    own_table_kernel<GT, I><<<plan.own, kOwnThreads, shared + size * 4, stream>>>(
+        static_cast<const GT *>(grad), (uint32_t)(stride * sizeof(GT)), static_cast<const I *>(index), count, use, dim, partial);
+    return gsx_launch_pdl(own_join_kernel<TT>, dim3((size + 31) / 32), dim3(kThreads), 0, stream, (const float *)partial, size,
+                          plan.own, dim, table);
 }
 
 bool float_type(int t) { return t == GSX_B200_DATA_F32 || t == GSX_B200_DATA_F16 || t == GSX_B200_DATA_BF16; }
@@ -1181,6 +1334,15 @@ extern "C" int gsx_b200_embedding_backward(const void *grad_out, int grad_type, 
     unsigned char *ws = static_cast<unsigned char *>(workspace);
     const Use use = { (uint32_t)rows, padding_row < 0 ? UINT32_MAX : (uint32_t)padding_row, device_out_of_range };
     cudaError_t e = cudaSuccess;
+    if(plan.own) {
+        GSX_WITH_FLOAT_TYPE(grad_type, GT, GSX_WITH_FLOAT_TYPE(table_type, TT, {
+            float *partial = reinterpret_cast<float *>(ws + plan.o_head);
+            e = index_type == GSX_B200_DATA_I32
+                    ? launch_own<GT, TT, int32_t>(grad_out, grad_stride, index, (uint32_t)count, use, plan, partial, table, (uint32_t)dim, stream)
+                    : launch_own<GT, TT, int64_t>(grad_out, grad_stride, index, (uint32_t)count, use, plan, partial, table, (uint32_t)dim, stream);
+        }));
+        return launch_status(e);
+    }
     Runs runs;
     e = index_type == GSX_B200_DATA_I32
             ? launch_sort<int32_t>(plan, ws, index, (uint32_t)count, use, table, (uint32_t)dim, &runs.pairs, stream)

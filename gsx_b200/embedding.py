@@ -20,15 +20,16 @@ def embedding_lookup(table, index, out=None, scale: float = 1.0, bad=None, strea
     if not index.is_contiguous():
         raise invalid("index must be contiguous")
     count = index.numel()
-    below_2_31(rows, dim, count)
+    if (rows | dim | count) >> 31:
+        below_2_31(rows, dim, count)
     if out is None:
         out = empty((*index.shape, dim), table.dtype, device, stream)
     elif out.shape[:-1] != index.shape or out.shape[-1:] != table.shape[1:]:
         raise invalid(f"out must be {(*index.shape, dim)}, not {tuple(out.shape)}")
     launch(lib().gsx_b200_embedding_lookup, device, stream, table.data_ptr(), type_code(table, FLOAT_TYPES, "table"),
-           rows, dim, row_stride(table, dim, "table"), index.data_ptr(), type_code(index, INDEX_TYPES, "index"),
-           count, scale, out.data_ptr(), type_code(out, FLOAT_TYPES, "out"), row_stride(out, dim, "out"),
-           word(bad, "bad"))
+           rows, dim, dim if table.is_contiguous() else row_stride(table, dim, "table"), index.data_ptr(),
+           type_code(index, INDEX_TYPES, "index"), count, scale, out.data_ptr(), type_code(out, FLOAT_TYPES, "out"),
+           dim if out.is_contiguous() else row_stride(out, dim, "out"), None if bad is None else word(bad, "bad"))
     return out
 
 
@@ -45,7 +46,8 @@ def embedding_backward(grad_out, index, grad_table, scale: float = 1.0, padding_
     if not index.is_contiguous():
         raise invalid("index must be contiguous")
     count = index.numel()
-    below_2_31(rows, dim, count)
+    if (rows | dim | count) >> 31:
+        below_2_31(rows, dim, count)
     if grad_out.shape[:-1] != index.shape or grad_out.shape[-1:] != grad_table.shape[1:]:
         raise invalid(f"grad_out must be {(*index.shape, dim)}, not {tuple(grad_out.shape)}")
     if padding_row is None:

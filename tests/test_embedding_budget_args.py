@@ -93,9 +93,11 @@ def test_workspace_sizes():
     small = L.gsx_b200_embedding_workspace_bytes(100, 50, 4)
     assert 800 <= small < 1 << 20
     # (row, position) pairs: once for a sort of one pass (up to 256 rows), twice for more
-    one = L.gsx_b200_embedding_workspace_bytes(1_000_000, 256, 8)
-    two = L.gsx_b200_embedding_workspace_bytes(1_000_000, 257, 8)
-    assert 8_000_000 < one < 16_000_000 <= two < 24_000_000
+    one = L.gsx_b200_embedding_workspace_bytes(500_000, 256, 8)
+    two = L.gsx_b200_embedding_workspace_bytes(500_000, 257, 8)
+    assert 4_000_000 < one < 8_000_000 <= two < 12_000_000
+    # many positions, short rows and a table that fits shared memory: one table of sums for each of 296 chunks
+    assert L.gsx_b200_embedding_workspace_bytes(3_000_000, 4096, 3) == 256 + 296 * 4096 * 3 * 4
     assert L.gsx_b200_budget_workspace_bytes(32, 393_216) == 0
     assert 0 < L.gsx_b200_budget_workspace_bytes(32, 393_217) < 4 << 20
 

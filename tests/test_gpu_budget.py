@@ -34,7 +34,8 @@ def _check_accumulate(out, score, weights, decay, lengths=None, row_lengths=None
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("groups,rows,length", [(1, 0, 5), (1, 1, 1), (3, 1, 8), (2, 3, 1000), (5, 64, 257), (1, 200, 2048),
-                                                (2, 130, 4099), (4, 1000, 64), (1, 5000, 1), (70, 8, 33), (1, 8, 100_000)])
+                                                (2, 130, 4099), (4, 1000, 64), (1, 5000, 1), (70, 8, 33), (1, 8, 100_000), (2, 40, 1004),
+                                                (3, 6, 1002), (1, 70, 514), (2, 33, 1001), (1, 9, 3)])
 def test_accumulate_sizes(cuda_device, groups, rows, length, dtype):
     g = _gen(groups * 7 + rows + length)
     score = torch.rand(groups, length, generator=g, device="cuda")

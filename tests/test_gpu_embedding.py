@@ -127,7 +127,8 @@ def _check_gradient(got, grad, index, rows, scale, before=None, drop=None):
 GRADIENT_SIZES = [(0, 5, 3), (1, 1, 1), (5, 1, 4), (100, 256, 8), (8192, 300, 7), (8193, 300, 7), (9000, 1, 3),
                   (20_000, 4096, 3), (20_000, 4097, 4), (50_000, 70_000, 2), (33_333, 5000, 45), (300, 1000, 2048),
                   (12_000, 3, 260), (2000, 50, 33), (200_001, 100, 1), (300_000, 1000, 2), (700_000, 4096, 3),
-                  (150_000, 777, 4), (60_000, 1, 3)]
+                  (150_000, 777, 4), (60_000, 1, 3), (700_001, 1000, 3), (1_300_000, 4096, 4),
+                  (650_000, 17, 9), (620_000, 1152, 16), (606_208, 1, 1)]
 
 
 @pytest.mark.parametrize("count,rows,dim", GRADIENT_SIZES)
@@ -146,7 +147,7 @@ def test_gradient_sizes(cuda_device, count, rows, dim):
 @pytest.mark.parametrize("grad_type", [F32, F16, BF16])
 def test_gradient_types(cuda_device, grad_type, table_type, itype):
     g = _gen(5)
-    for count, rows, dim in [(700, 40, 64), (9001, 600, 5), (900, 30, 16), (90_000, 300, 3), (80_000, 9, 1)]:
+    for count, rows, dim in [(700, 40, 64), (9001, 600, 5), (900, 30, 16), (90_000, 300, 3), (80_000, 9, 1), (650_000, 300, 3)]:
         grad = torch.randn(count, dim, generator=g, device="cuda").to(grad_type)
         index = _index(g, count, rows, itype, 3.0)
         got = gb.embedding_backward(grad, index, torch.empty(rows, dim, dtype=table_type, device="cuda"), scale=1.5)
@@ -167,7 +168,7 @@ def test_gradient_three_digit_sort(cuda_device):
     _check_gradient(got, grad, index, rows, 1.0)
 
 
-@pytest.mark.parametrize("count", [3000, 40_000, 300_000])
+@pytest.mark.parametrize("count", [3000, 40_000, 300_000, 800_000])
 @pytest.mark.parametrize("dim", [3, 64, 300])
 def test_gradient_of_one_row_that_has_nearly_all(cuda_device, count, dim):
     g = _gen(7)
@@ -179,7 +180,7 @@ def test_gradient_of_one_row_that_has_nearly_all(cuda_device, count, dim):
 
 
 @pytest.mark.parametrize("dim", [3, 6])
-@pytest.mark.parametrize("count,rows", [(500, 64), (500, 63), (30_000, 4096), (30_000, 9000), (90_000, 500)])
+@pytest.mark.parametrize("count,rows", [(500, 64), (500, 63), (30_000, 4096), (30_000, 9000), (90_000, 500), (800_000, 500)])
 def test_gradient_drops_padding_and_out_of_range(cuda_device, count, rows, dim):
     g = _gen(8)
     grad = torch.randn(count, dim, generator=g, device="cuda")
@@ -203,7 +204,7 @@ def test_gradient_drops_padding_and_out_of_range(cuda_device, count, rows, dim):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("dim,count", [(8, 10_000), (21, 10_000), (600, 10_000), (3, 100_000)])
+@pytest.mark.parametrize("dim,count", [(8, 10_000), (21, 10_000), (600, 10_000), (3, 100_000), (5, 800_000)])
 def test_gradient_strided(cuda_device, dtype, dim, count):
     g = _gen(9)
     for offset in (0, 1):
