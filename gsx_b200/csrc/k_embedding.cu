@@ -913,7 +913,7 @@ __global__ void __launch_bounds__(kThreads) row_join_kernel(const Runs a, const 
 constexpr int kOwnThreads = 256;
 constexpr int kOwnItems = 16;
 constexpr uint32_t kOwnTile = kOwnThreads * kOwnItems;
-constexpr uint64_t kOwnDim = 16;
+constexpr uint64_t kOwnDim = 4, kOwnRows = 128;
 constexpr size_t kOwnTable = 68 * 1024; /* two CTAs an SM */
 constexpr uint32_t kOwnLong = 64;
 constexpr int kOwnCols = 4; /* columns of a walk */
@@ -1027,10 +1027,12 @@ __global__ void __launch_bounds__(kThreads) own_join_kernel(const float *partial
 }
 
 /* Chunks of a call that takes this path, or 0: the table fits, and there are enough positions for half the GPU's CTAs
- * with tables that cost no more to write and read than the gradients. */
+ * with tables that cost no more to write and read than the gradients.  Measured against the sort of all positions
+ * (us, here / there): 3M x 3 into 4096 rows 63 / 105, into 256 59 / 79, into 64 79 / 71 (few long lists); 2M x 4 into
+ * 512 rows 49 / 72; 2M x 9 into 1000 rows 91 / 89, 2M x 16 276 / 94 (a walk of the lists for every four columns). */
 uint32_t own_chunks(uint64_t count, uint64_t rows, uint64_t dim)
 {
-    if(dim > kOwnDim || rows * dim * 4 > kOwnTable) return 0;
+    if(dim > kOwnDim || rows < kOwnRows || rows * dim * 4 > kOwnTable) return 0;
     uint64_t chunks = count / kOwnTile, most = count / (2 * rows);
     if(chunks > most) chunks = most;
     if(chunks < 148) return 0;

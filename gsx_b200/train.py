@@ -11,23 +11,32 @@ from __future__ import annotations
 import numpy as np
 import torch
 
-from . import FORWARD_TRAIN, Adam, Camera, ParamGroup, RenderContext, Renderer, l1_ssim
+from . import FORWARD_TRAIN, INVALID_ARGUMENT, NOT_SUPPORTED, Adam, Camera, GsxError, ParamGroup, RenderContext, Renderer, l1_ssim
+from .budget import budget_accumulate, budget_gather, budget_select
+from .embedding import embedding_backward, embedding_lookup
 
 FIELD_ORDER = ("mean3d", "logscale", "rotation", "opacity", "sh0", "sh1", "sh2", "sh3")
 FIELD_COLS = {"mean3d": (3,), "logscale": (3,), "rotation": (4,), "opacity": (), "sh0": (3,), "sh1": (3, 3),
               "sh2": (5, 3), "sh3": (7, 3)}
 DEFAULT_LR = {"mean3d": 1e-3, "logscale": 1e-2, "rotation": 1e-2, "opacity": 1e-2, "sh0": 1e-2, "sh1": 1e-2,
               "sh2": 1e-2, "sh3": 1e-2}
+SH_C0 = 0.28209479177387814  # the constant spherical harmonic: d colour / d sh0
 
 
 class GaussianModel:
     """Gaussian parameters and gradients as views into two flat, 16-byte-aligned allocations."""
 
     def __init__(self, arrays: dict, device="cuda:0", sh_degree: int = 0):
-        self.n = int(arrays["mean3d"].shape[0])
         self.sh_degree = sh_degree
         self.fields = [f for f in FIELD_ORDER if f in ("mean3d", "logscale", "rotation", "opacity", "sh0")
                        or int(f[2]) <= sh_degree]
+        self._allocate(int(arrays["mean3d"].shape[0]), device)
+        for f in self.fields:
+            src = np.ascontiguousarray(arrays[f], dtype=np.float32).reshape(self.params[f].shape)
+            self.params[f].copy_(torch.from_numpy(src))
+
+    def _allocate(self, n, device):
+        self.n = n
         offs, o = {}, 0
         for f in self.fields:
             cnt = self.n * int(np.prod(FIELD_COLS[f], dtype=np.int64))
@@ -38,9 +47,6 @@ class GaussianModel:
         # each field's padded [begin, end) in the flat buffers (16-byte aligned on both ends)
         self.field_ranges = {f: (a, a + (c + 3) // 4 * 4) for f, (a, c) in offs.items()}
         self._bind(torch.zeros(o, dtype=torch.float32, device=device), torch.zeros(o, dtype=torch.float32, device=device))
-        for f in self.fields:
-            src = np.ascontiguousarray(arrays[f], dtype=np.float32).reshape(self.params[f].shape)
-            self.params[f].copy_(torch.from_numpy(src))
 
     def _bind(self, flat_param, flat_grad):
         self.flat_param, self.flat_grad = flat_param, flat_grad
@@ -58,12 +64,32 @@ class GaussianModel:
         self._bind(flat_param, flat_grad)
 
 
+class SharedRows:
+    """A field whose rows many Gaussians share (a codebook of colours or of higher-order coefficients): the field is
+    scale * table[index], the trained parameter is the table ([rows, columns of the field], f32), index is one int32
+    or int64 row number per Gaussian."""
+
+    def __init__(self, table, index, scale: float = 1.0):
+        self.table, self.index, self.scale = table, index, float(scale)
+        self.grad = torch.empty_like(table)
+
+    def expand(self, field):
+        """Write the field's rows ([N, ..] f32) from the table."""
+        embedding_lookup(self.table, self.index, out=field.view(field.shape[0], -1), scale=self.scale)
+
+    def reduce(self, field_grad):
+        """The table's gradient from the field's, summed by row."""
+        embedding_backward(field_grad.view(field_grad.shape[0], -1), self.index, self.grad, scale=self.scale)
+
+
 class Trainer:
     """One view per call of step(); `group` is a torch.distributed process group (None = 1 GPU)."""
 
     def __init__(self, model: GaussianModel, width: int, height: int, lr: dict | None = None, l1_weight=0.8,
-                 ssim_weight=0.2, background=(0.0, 0.0, 0.0), group=None, device="cuda:0", exchange="fused"):
-        """exchange (with a group): "fused" = gsx_b200.dp.ShardedAdam (gradient average + sharded Adam +
+                 ssim_weight=0.2, background=(0.0, 0.0, 0.0), group=None, device="cuda:0", exchange="fused", shared: dict | None = None):
+        """shared: {field: SharedRows}; such a field is written from its table before each render and its table is
+        trained in its place (one GPU only: the exchange covers the fields).
+        exchange (with a group): "fused" = gsx_b200.dp.ShardedAdam (gradient average + sharded Adam +
         parameter all-gather in one NVLink kernel per rank), through the NVSwitch (multimem reduce-load and
         multicast store) from 4 ranks up where every GPU supports it, else over peer loads and stores;
         "nvls" / "peer" force one form; "nccl" = all-reduce AVG then Adam everywhere."""
@@ -77,13 +103,25 @@ class Trainer:
         self.l1_weight, self.ssim_weight = l1_weight, ssim_weight
         self.background = background
         self.group = group
-        lr = dict(DEFAULT_LR, **(lr or {}))
+        self.lr = lr = dict(DEFAULT_LR, **(lr or {}))
+        self.shared = dict(shared or {})
+        if self.shared and group is not None:
+            raise GsxError(NOT_SUPPORTED, "shared rows train on one GPU")
+        for f, rows in self.shared.items():
+            if f not in model.fields or rows.table.dtype != torch.float32 or rows.index.shape != (model.n,):
+                raise GsxError(NOT_SUPPORTED, "shared rows need a field of the model, a float32 table and an index per Gaussian")
         self.sharded = None
         self.exchange = "nccl" if group is not None else None
         if group is not None and exchange in ("fused", "nvls", "peer"):
             self._setup_fused(model, group, device, lr, exchange)
         if self.sharded is None:
-            self.optim = Adam([ParamGroup(f, model.params[f], model.grads[f], lr[f]) for f in model.fields])
+            self.optim = Adam(self._groups())
+
+    def _groups(self):
+        """Adam's parameter groups, one per field of the model (a shared field's table in its place)."""
+        m = self.model
+        return [ParamGroup(f, self.shared[f].table, self.shared[f].grad, self.lr[f]) if f in self.shared
+                else ParamGroup(f, m.params[f], m.grads[f], self.lr[f]) for f in m.fields]
 
     def _setup_fused(self, model, group, device, lr, exchange):
         """Map the flat buffers into every rank (NVSwitch multicast or CUDA IPC) and build the sharded
@@ -122,6 +160,8 @@ class Trainer:
     def gradients(self, camera: Camera, target, events=None):
         """Render TRAIN, fused L1+SSIM, render backward: this rank's gradients in model.flat_grad."""
         m = self.model
+        for f, rows in self.shared.items():
+            rows.expand(m.params[f])
         self.renderer.render(self.ctx, m.params, camera, self.out, background=self.background,
                              sh_degree=m.sh_degree, forward_type=FORWARD_TRAIN)
         self.loss_sum.zero_()
@@ -132,6 +172,51 @@ class Trainer:
         if events:
             events[0][1].record()
         self.renderer.backward(self.ctx, self.grad_rgb, m.grads)
+        for f, rows in self.shared.items():
+            rows.reduce(m.grads[f])
+
+    def blend_weights(self, camera: Camera, score, decay: float = 1.0):
+        """score ([N] f32) = decay * score + the blend weight of every Gaussian in this view: the sum over the pixels of
+        alpha times transmittance, with which its colour enters them.  (It is the gradient of the sum of the image by
+        that colour, taken with all colours grey so that none is clamped, so it follows the backward's rule and counts
+        alphas below 1/255 as well; model.grads is overwritten.)"""
+        m = self.model
+        grey = dict(m.params, sh0=torch.zeros_like(m.params["sh0"]))
+        self.renderer.render(self.ctx, grey, camera, self.out, background=self.background, sh_degree=0,
+                             forward_type=FORWARD_TRAIN)
+        self.grad_rgb.zero_()
+        self.grad_rgb[0] = 1.0 / SH_C0
+        self.renderer.backward(self.ctx, self.grad_rgb, m.grads)
+        return budget_accumulate(score, m.grads["sh0"][:, 0].contiguous().view(1, -1), decay=decay)
+
+    def keep_budget(self, score, budget: int, first: int = 0, recent: int = 0):
+        """Drop Gaussians until `budget` are left: the `first` first, the `recent` last (just grown) and the largest
+        scores of the others stay, in order, with their Adam moments and row numbers.  Returns their scores."""
+        m = self.model
+        if self.group is not None:
+            raise GsxError(NOT_SUPPORTED, "keep_budget runs on one GPU")
+        if score.shape != (m.n,) or budget < 1:
+            raise GsxError(INVALID_ARGUMENT, "score must hold one value per Gaussian, the budget be at least one")
+        if budget >= m.n:
+            return score
+        keep, kept = budget_select(score, budget, first=first, recent=recent)
+        before, optim = m.params, self.optim
+        m._allocate(int(budget), m.flat_param.device)
+        out = torch.empty(m.n, dtype=torch.float32, device=score.device)
+        gather = [(score, out)] + [(before[f], m.params[f]) for f in m.fields]
+        for rows in self.shared.values():
+            index = torch.empty(m.n, dtype=rows.index.dtype, device=rows.index.device)
+            gather.append((rows.index, index))
+            rows.index = index
+        self.optim = Adam(self._groups())
+        self.optim.steps = list(optim.steps)
+        for i, f in enumerate(m.fields):
+            if f in self.shared:
+                self.optim.m1[i], self.optim.m2[i] = optim.m1[i], optim.m2[i]
+            else:
+                gather += [(optim.m1[i], self.optim.m1[i]), (optim.m2[i], self.optim.m2[i])]
+        budget_gather(gather, keep, kept)
+        return out
 
     def update(self, events=None):
         """The gradient exchange (with a group) and Adam; returns the loss-sum device scalar."""

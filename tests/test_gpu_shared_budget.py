@@ -1,0 +1,128 @@
+"""Shared rows and the budget where the trainer uses them: lookup before the render, the table's gradient after its
+backward, Adam on the table; blend weights accumulated over views, eviction to a budget, training on."""
+import numpy as np
+import pytest
+import torch
+
+import gsx_b200 as gb
+from gsx_b200 import scenes
+from gsx_b200.train import GaussianModel, SharedRows, Trainer
+from oracle import pyoracle as po
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+W, H = 96, 80
+
+
+def _ocam(cam):
+    return po.Camera(cam.width, cam.height, cam.fx, cam.fy, cam.cx, cam.cy, cam.rot_xyzw, cam.transl, cam.near_plane, cam.far_plane)
+
+
+def _trainer(n=3000, rows=50, sh_degree=0, fields=("sh0",)):
+    g, cam = scenes.small_scene(3, n, W, H, sh_degree)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    model = GaussianModel(g, sh_degree=sh_degree)
+    shared = {}
+    for f in fields:
+        cols = model.params[f].view(n, -1).shape[1]
+        shared[f] = SharedRows(torch.randn(rows, cols, generator=gen, device="cuda") * 0.3,
+                               torch.randint(0, rows, (n,), generator=gen, device="cuda", dtype=torch.int32), scale=0.5)
+    target = torch.rand(3, H, W, generator=gen, device="cuda")
+    return Trainer(model, W, H, shared=shared), cam, target
+
+
+@pytest.mark.parametrize("sh_degree,fields", [(0, ("sh0",)), (1, ("sh0", "sh1"))])
+def test_a_step_with_shared_rows(cuda_device, sh_degree, fields):
+    tr, cam, target = _trainer(sh_degree=sh_degree, fields=fields)
+    m = tr.model
+    tr.gradients(cam, target)
+    for f in fields:
+        rows = tr.shared[f]
+        n = m.n
+        assert torch.equal(m.params[f].view(n, -1), rows.table[rows.index.long()] * 0.5)
+        grad = m.grads[f].view(n, -1).double()
+        want = torch.zeros_like(rows.table, dtype=torch.float64).index_add_(0, rows.index.long(), grad) * 0.5
+        size = torch.zeros_like(want).index_add_(0, rows.index.long(), grad.abs()) * 0.5
+        count = torch.bincount(rows.index.long(), minlength=rows.table.shape[0]).double()[:, None]
+        assert bool(((rows.grad.double() - want).abs() <= 1.01 * size * (count + 2) * U).all())
+        assert float(rows.grad.abs().max()) > 0
+    before = {f: tr.shared[f].table.clone() for f in fields}
+    other = m.params["mean3d"].clone()
+    tr.update()
+    for f in fields:  # the table took the place of the field in Adam
+        alone = before[f].clone()
+        gb.Adam([gb.ParamGroup(f, alone, tr.shared[f].grad, tr.lr[f])]).step()
+        assert torch.equal(alone, tr.shared[f].table)
+    assert not torch.equal(other, m.params["mean3d"])
+
+
+def test_blend_weights_are_the_colour_gradient_of_the_oracle(cuda_device):
+    tr, cam, _ = _trainer()
+    for rows in tr.shared.values():
+        rows.expand(tr.model.params["sh0"])
+    score = torch.full((tr.model.n,), 2.0, device="cuda")
+    assert tr.blend_weights(cam, score, decay=0.0) is score
+    g = {k: v.cpu().numpy() for k, v in tr.model.params.items()}
+    g["sh0"] = np.zeros_like(g["sh0"])
+    ref = po.render_forward(g, _ocam(cam))
+    grad = np.zeros((3, H, W), np.float32)
+    grad[0] = np.float32(1.0 / 0.28209479177387814)
+    want = po.render_backward(g, _ocam(cam), ref, grad)["sh0"][:, 0].astype(np.float64)
+    got = score.cpu().numpy().astype(np.float64)
+    assert np.linalg.norm(got - want) <= 1e-3 * np.linalg.norm(want)
+    assert (got >= 0).all() and got.max() > 1
+    once = score.clone()
+    tr.blend_weights(cam, score, decay=0.5)
+    # the backward adds up with atomics, so a second run differs by its order (the bar above); the decay is exact
+    assert float((score - 1.5 * once).norm()) <= 2e-3 * float(once.norm())
+
+
+def test_train_evict_and_train_on(cuda_device):
+    tr, cam, target = _trainer(n=4001, sh_degree=1, fields=("sh1",))
+    for _ in range(3):
+        tr.step(cam, target)
+    m = tr.model
+    score = torch.zeros(m.n, device="cuda")
+    for _ in range(2):
+        tr.blend_weights(cam, score, decay=0.9)
+    old = {f: v.clone() for f, v in m.params.items()}
+    m1 = [t.clone() for t in tr.optim.m1]
+    m2 = [t.clone() for t in tr.optim.m2]
+    index, table = tr.shared["sh1"].index.clone(), tr.shared["sh1"].table.clone()
+    left = tr.keep_budget(score, 1500, first=10, recent=200)
+    s = score.cpu().numpy().astype(np.float64)
+    middle = np.arange(10, 4001 - 200)
+    best = middle[np.lexsort((middle, -s[middle]))][:1500 - 210]
+    keep = torch.from_numpy(np.sort(np.concatenate([np.arange(10), best, np.arange(3801, 4001)]))).cuda()
+    assert m.n == 1500 and torch.equal(left, score[keep])
+    for f in m.fields:
+        assert torch.equal(m.params[f], old[f][keep]), f
+    assert torch.equal(tr.shared["sh1"].index, index[keep]) and torch.equal(tr.shared["sh1"].table, table)
+    assert tr.optim.steps == [3] * len(m.fields)
+    for i, f in enumerate(m.fields):
+        rows = slice(None) if f == "sh1" else keep
+        assert torch.equal(tr.optim.m1[i], m1[i][rows]) and torch.equal(tr.optim.m2[i], m2[i][rows])
+    assert tr.keep_budget(left, 1500) is left
+    for _ in range(2):
+        loss = tr.step(cam, target)
+    assert bool(torch.isfinite(loss).all()) and tr.optim.steps[0] == 5
+
+
+
+def test_refusals(cuda_device):
+    tr, cam, target = _trainer(n=200)
+    m = tr.model
+    rows = tr.shared["sh0"]
+    for bad in (SharedRows(rows.table.half(), rows.index), SharedRows(rows.table, rows.index[:-1])):
+        with pytest.raises(gb.GsxError) as e:
+            Trainer(m, W, H, shared={"sh0": bad})
+        assert e.value.code == gb.NOT_SUPPORTED
+    with pytest.raises(gb.GsxError) as e:
+        Trainer(m, W, H, shared={"sh2": rows})
+    assert e.value.code == gb.NOT_SUPPORTED
+    for call in (lambda: tr.keep_budget(torch.zeros(199, device="cuda"), 10), lambda: tr.keep_budget(torch.zeros(200, device="cuda"), 0),
+                 lambda: tr.keep_budget(torch.zeros(200, device="cuda"), 10, first=6, recent=5)):
+        with pytest.raises(gb.GsxError) as e:
+            call()
+        assert e.value.code == gb.INVALID_ARGUMENT
+        assert m.n == 200
