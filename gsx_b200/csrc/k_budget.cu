@@ -821,7 +821,7 @@ extern "C" int gsx_b200_budget_accumulate(const float *score, uint64_t score_str
     if(score == nullptr || out == nullptr || (rows > 0 && weights == nullptr))
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "score, weights and out must be non-null");
     const uint64_t es = weight_type == GSX_B200_DATA_F32 ? 4 : 2;
-    if((uintptr_t)score % 4 || (uintptr_t)out % 4 || (uintptr_t)weights % es)
+    if((uintptr_t)score % 4 || (uintptr_t)out % 4 || (uintptr_t)weights % es || (uintptr_t)lengths % 4 || (uintptr_t)row_lengths % 4)
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "pointers must be aligned to their element type");
     if((groups > 1 && (score_stride < length || out_stride < length)) || (rows > 1 && row_stride < length))
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "strides must be at least length elements");
@@ -865,7 +865,7 @@ extern "C" int gsx_b200_budget_select(const float *score, uint64_t score_stride,
     if(groups == 0) return GSX_B200_SUCCESS;
     if(kept == nullptr || (length > 0 && score == nullptr) || (length > 0 && budget > 0 && keep == nullptr))
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "score, keep and kept must be non-null");
-    if((uintptr_t)score % 4 || (uintptr_t)keep % 4 || (uintptr_t)kept % 4 || (uintptr_t)drop % 4)
+    if((uintptr_t)score % 4 || (uintptr_t)keep % 4 || (uintptr_t)kept % 4 || (uintptr_t)drop % 4 || (uintptr_t)lengths % 4)
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "pointers must be aligned to 4 bytes");
     const uint64_t most = budget < length ? budget : length;
     if(groups > 1 && (score_stride < length || keep_stride < most || (drop != nullptr && drop_stride < length)))
@@ -945,6 +945,7 @@ extern "C" int gsx_b200_budget_gather(const gsx_b200_gather_field *fields, int32
         return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "outer * inner, length and budget must be below 2^31");
     if(outer * inner == 0 || budget == 0 || field_count == 0) return GSX_B200_SUCCESS;
     if(keep == nullptr || kept == nullptr) return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "keep and kept must be non-null");
+    if((uintptr_t)keep % 4 || (uintptr_t)kept % 4) return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "pointers must be aligned to 4 bytes");
     if(outer * inner > 1 && keep_stride < budget)
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "keep_stride must be at least budget");
     Fields t;

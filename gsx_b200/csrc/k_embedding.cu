@@ -1023,6 +1023,7 @@ __global__ void __launch_bounds__(kThreads) own_join_kernel(const float *partial
     if(warp != 0 || j >= size) return;
 #pragma unroll
     for(int w = 1; w < kWarps; ++w) sum[0] += s_part[w][lane];
+    if(table.accumulate && sum[0] == 0.0f) return; /* rows that no index names stay as they are, to the bit */
     store_sums<TT, 1>(table, j / dim, j % dim, sum);
 }
 
@@ -1235,6 +1236,15 @@ int launch_status(cudaError_t e)
     return e == cudaSuccess ? GSX_B200_SUCCESS : gsx_internal_fail(GSX_B200_UNKNOWN, cudaGetErrorString(e));
 }
 
+/* whether two spans of rows share bytes */
+bool overlap(const void *a, uint64_t a_rows, uint64_t a_step, uint64_t a_row, const void *b, uint64_t b_rows, uint64_t b_step,
+             uint64_t b_row)
+{
+    if(a_rows == 0 || b_rows == 0) return false;
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return x < y + (b_rows - 1) * b_step + b_row && y < x + (a_rows - 1) * a_step + a_row;
+}
+
 int check_shape(uint64_t rows, uint64_t dim, uint64_t stride_a, uint64_t stride_b, uint64_t count)
 {
     if(rows > (uint64_t)INT32_MAX || dim > (uint64_t)INT32_MAX || count > (uint64_t)INT32_MAX)
@@ -1276,6 +1286,10 @@ extern "C" int gsx_b200_embedding_lookup(const void *table, int table_type, uint
         return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "table_stride must be below 4 GiB");
     if(count * dim / 256 > (uint64_t)INT32_MAX)
         return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "count * dim must be below 2^39");
+    const uint64_t tb = float_bytes(table_type), ob = float_bytes(out_type), ib = index_type == GSX_B200_DATA_I32 ? 4 : 8;
+    if(overlap(out, count, out_stride * ob, dim * ob, table, rows, table_stride * tb, dim * tb) ||
+       overlap(out, count, out_stride * ob, dim * ob, index, 1, 0, count * ib))
+        return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "out must not overlap table or index");
     cudaStream_t stream = (cudaStream_t)stream_;
     cudaError_t e = cudaSuccess;
     GSX_WITH_FLOAT_TYPE(table_type, T, GSX_WITH_FLOAT_TYPE(out_type, O, {
@@ -1316,6 +1330,13 @@ extern "C" int gsx_b200_embedding_backward(const void *grad_out, int grad_type, 
        (uintptr_t)index % (index_type == GSX_B200_DATA_I32 ? 4 : 8) || (uintptr_t)workspace % 16)
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT,
                                  "pointers must be aligned to their element type, the workspace to 16 bytes");
+    if(!(scale - scale == 0.0f)) return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "scale must be finite");
+    {
+        const uint64_t tb = float_bytes(table_type), ob = float_bytes(grad_type), ib = index_type == GSX_B200_DATA_I32 ? 4 : 8;
+        if(overlap(grad_table, rows, table_stride * tb, dim * tb, grad_out, count, grad_stride * ob, dim * ob) ||
+           overlap(grad_table, rows, table_stride * tb, dim * tb, index, 1, 0, count * ib))
+            return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "grad_table must not overlap grad_out or index");
+    }
     Table table;
     table.data = grad_table;
     table.stride = table_stride;

@@ -402,13 +402,13 @@ GSX_B200_API int gsx_b200_adc_select_keep(uint64_t n, const float *opacity, cons
  * per Gaussian, or any other embedding table.  Tables, outputs and gradients are f32, f16 or bf16 in any
  * combination, indices i32 or i64; row strides are in elements and at least dim (those of a table that is
  * read and of grad_out below 4 GiB); rows, dim and count stay below 2^31.  An index outside [0, rows) sets *device_out_of_range to 1 (when non-NULL) and takes no part: its row of
- * out stays untouched, its gradient is dropped.  Nothing waits, allocates or depends on values: the calls can be
- * captured into a graph.
+ * out stays untouched, its gradient is dropped.  Outputs must not overlap inputs (by address range).  Nothing
+ * waits or allocates: the calls can be captured into a graph.
  * gsx_b200_embedding_lookup: out[n] = scale * table[index[n]], computed in f32 and rounded once.
  * gsx_b200_embedding_backward: grad_table[v] = scale * (sum of grad_out[n] over index[n] = v), written for every
  * row (zero where no index names it), or added to it when accumulate != 0 (rows that no index names are then left
  * as they are).  The positions are sorted by row first, so every sum runs in the order of n whatever the
- * launch: the same inputs give the same bits.  Sums are f32, rounded once.  Indices equal to padding_row (-1: none)
+ * launch: the same inputs give the same bits.  Sums are f32, rounded once.  scale must be finite.  Indices equal to padding_row (-1: none)
  * take no part.  workspace: gsx_b200_embedding_workspace_bytes(count, rows, dim) bytes of device memory, 16-byte
  * aligned, of any content; calls that overlap on the GPU need one each.
  */
@@ -444,8 +444,9 @@ GSX_B200_API int gsx_b200_embedding_backward(const void *grad_out, int grad_type
  * gsx_b200_budget_gather: for every field and group, row r of dst = row keep[g, r] of src for r < kept[g]; later
  *   rows of dst are left as they were.  All fields in ONE launch.  Group g is (g / inner, g % inner) in a field's
  *   outer and inner strides (caches of [batch, head, entry] and [batch, entry, head] order alike).  A keep entry
- *   outside [0, length) sets *device_out_of_range to 1 (when non-NULL) and leaves its row untouched.  No field's
- *   dst may overlap any field's src.
+ *   outside [0, length) sets *device_out_of_range to 1 (when non-NULL) and leaves its row untouched.  keep holds
+ *   `budget` places a group, of any content behind kept[g], and need not be in order.  No field's dst may overlap any
+ *   field's src, or another's dst.
  */
 #define GSX_B200_GATHER_MAX_FIELDS 32
 typedef struct gsx_b200_gather_field {

@@ -11,14 +11,14 @@ P = 4096  # an aligned non-null address: every call here returns before it is us
 F32, F16, BF16, U8, I32, I64 = 0, 1, 2, 8, 12, 13
 
 
-def _lookup(table=P, ttype=F32, rows=4, dim=8, tstride=8, index=P, itype=I32, count=3, out=P, otype=F32, ostride=8):
+def _lookup(table=1 << 20, ttype=F32, rows=4, dim=8, tstride=8, index=1 << 16, itype=I32, count=3, out=P, otype=F32, ostride=8):
     return _capi.lib().gsx_b200_embedding_lookup(table, ttype, rows, dim, tstride, index, itype, count, 1.0, out, otype,
                                                  ostride, None, None)
 
 
-def _backward(grad=P, gtype=F32, gstride=8, index=P, itype=I32, count=3, padding=-1, table=P, ttype=F32, rows=4, dim=8,
+def _backward(grad=1 << 20, gtype=F32, gstride=8, index=1 << 16, itype=I32, count=3, padding=-1, scale=1.0, table=P, ttype=F32, rows=4, dim=8,
               tstride=8, ws=P, size=1 << 40):
-    return _capi.lib().gsx_b200_embedding_backward(grad, gtype, gstride, index, itype, count, 1.0, padding, table, ttype,
+    return _capi.lib().gsx_b200_embedding_backward(grad, gtype, gstride, index, itype, count, scale, padding, table, ttype,
                                                    rows, dim, tstride, 0, ws, size, None, None)
 
 
@@ -47,13 +47,16 @@ CASES = [
     (gb.OUT_OF_RANGE, _lookup, [dict(rows=2 ** 31), dict(count=2 ** 31), dict(tstride=2 ** 41), dict(tstride=2 ** 30),
                                 dict(count=2 ** 30, dim=2 ** 30, tstride=2 ** 30, ostride=2 ** 30)]),
     (gb.INVALID_ARGUMENT, _lookup, [dict(table=None), dict(index=None), dict(out=None), dict(tstride=7), dict(ostride=7),
-                                    dict(table=P + 2), dict(out=P + 1, otype=F16), dict(index=P + 4, itype=I64)]),
+                                    dict(table=(1 << 20) + 2), dict(out=P + 1, otype=F16), dict(index=(1 << 16) + 4, itype=I64),
+                                    dict(out=(1 << 20) + 64), dict(out=(1 << 20) - 32), dict(out=(1 << 16) - 64)]),
     (_capi.SUCCESS, _lookup, [dict(count=0), dict(dim=0)]),
     (gb.NOT_SUPPORTED, _backward, [dict(gtype=U8), dict(ttype=I32), dict(itype=U8)]),
     (gb.OUT_OF_RANGE, _backward, [dict(rows=2 ** 31), dict(padding=4), dict(gstride=2 ** 30),
                                   dict(dim=2 ** 22, gstride=2 ** 22, tstride=2 ** 22)]),
     (gb.INVALID_ARGUMENT, _backward, [dict(grad=None), dict(index=None), dict(table=None), dict(ws=None), dict(gstride=7),
-                                      dict(tstride=7), dict(size=100), dict(ws=P + 8), dict(grad=P + 2),
+                                      dict(tstride=7), dict(size=100), dict(ws=P + 8), dict(grad=(1 << 20) + 2),
+                                      dict(scale=float('inf')), dict(scale=float('nan')), dict(table=(1 << 20) - 64),
+                                      dict(table=(1 << 16) - 64),
                                       dict(rows=0)]),
     (_capi.SUCCESS, _backward, [dict(dim=0), dict(rows=0, count=0)]),
     (gb.NOT_SUPPORTED, _accumulate, [dict(wtype=U8)]),
@@ -75,7 +78,7 @@ CASES = [
                                 dict(src_row_stride=2 ** 32), dict(src_outer_stride=2 ** 43), dict(row_bytes=2 ** 32, dst_row_stride=2 ** 32)]),
     (gb.INVALID_ARGUMENT, _gather, [dict(keep=None), dict(kept=None), dict(src=None), dict(dst=None),
                                     dict(dst_row_stride=11), dict(dst=P + 180), dict(dst=P - 12 * 7),
-                                    dict(inner=2, kstride=7)]),
+                                    dict(inner=2, kstride=7), dict(keep=P + 2), dict(kept=P + 1)]),
     (_capi.SUCCESS, _gather, [dict(count=0), dict(outer=0), dict(budget=0), dict(row_bytes=0)]),
 ]
 

@@ -218,6 +218,50 @@ def test_gradient_strided(cuda_device, dtype, dim, count):
         assert bool((rest == 3.0).all())
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("count,rows,dim", [(500, 900, 4), (20_000, 3000, 40), (700_000, 2000, 3)])
+def test_gradient_accumulated_leaves_unnamed_rows_to_the_bit(cuda_device, count, rows, dim, dtype):
+    g = _gen(12)
+    index = _index(g, count, rows // 2, torch.int32) * 2
+    before = torch.randn(rows, dim, generator=g, device="cuda").to(dtype)
+    before[1::4] = -0.0
+    before[3::8] = float("nan")
+    before[7::16] = float("inf")
+    got = gb.embedding_backward(torch.randn(count, dim, generator=g, device="cuda"), index, before.clone(), scale=-2.0,
+                                accumulate=True)
+    bits = torch.int32 if dtype == F32 else torch.int16
+    assert torch.equal(got[1::2].view(bits), before[1::2].view(bits))
+    assert not torch.equal(got[::2], before[::2])
+
+
+def test_gradients_that_are_not_finite_stay_in_their_rows(cuda_device):
+    for count, rows, dim in [(300, 20, 5), (50_000, 700, 24), (700_000, 300, 3)]:
+        g = _gen(13)
+        grad = torch.randn(count, dim, generator=g, device="cuda")
+        index = _index(g, count, rows, torch.int64)
+        grad[index == 3] = float("nan")
+        grad[index == 5, 0] = float("inf")
+        got = gb.embedding_backward(grad, index, torch.empty(rows, dim, device="cuda"))
+        finite = torch.isfinite(got)
+        assert not bool(finite[3].any()) and not bool(finite[5, 0])
+        finite[3] = finite[5, 0] = True
+        assert bool(finite.all())
+
+
+def test_very_long_rows_and_empty_tables(cuda_device):
+    g = _gen(14)
+    for dim in (70_001, 65_536):
+        table = torch.randn(3, dim, generator=g, device="cuda")
+        index = torch.tensor([2, 0, 2, 1, 2], device="cuda")
+        _check_lookup(gb.embedding_lookup(table, index, scale=3.0), table, index, 3.0)
+        grad = torch.randn(5, dim, generator=g, device="cuda")
+        _check_gradient(gb.embedding_backward(grad, index, torch.empty_like(table)), grad, index, 3, 1.0)
+    for dim in (3, 8, 13):
+        out, bad = torch.full((4, dim), 2.0, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+        gb.embedding_lookup(torch.empty(0, dim, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda"), out=out, bad=bad)
+        assert int(bad) == 1 and bool((out == 2.0).all())
+
+
 def test_gradient_matches_differences_of_the_lookup(cuda_device):
     """A loss sum(c * lookup(table)) is linear in the table: moving one element by 1 moves it by its gradient."""
     g = _gen(10)
