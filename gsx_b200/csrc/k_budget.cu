@@ -206,8 +206,10 @@ cudaError_t launch_accumulate(uint64_t unit, const float *score, uint64_t score_
 /* select */
 
 constexpr int kCtaThreads = 1024;
-constexpr uint32_t kCtaKeys = 49152;             /* 192 KB of keys */
-constexpr uint32_t kClusterKeys = 8 * kCtaKeys; /* of the eight CTAs of a cluster */
+constexpr uint32_t kCtaKeys = 16384;
+/* of the eight CTAs of a cluster; a group of 393216 took 48 us in a cluster (of 49152 keys a CTA) and 23 us spread over
+ * the GPU, eight of 131072 25 and 30 us */
+constexpr uint32_t kClusterKeys = 8 * kCtaKeys;
 constexpr int kBins = 2048;
 constexpr int kPasses = 3;
 __device__ constexpr int kShift[kPasses] = { 21, 10, 0 };
@@ -409,7 +411,7 @@ __global__ void __launch_bounds__(kCtaThreads) select_cluster_kernel(const Selec
         }
         uint32_t all;
         block_scan(gt | eq << 16, s_warp, &all);
-        if(threadIdx.x == 0) s_counts = all; /* each at most kCtaKeys < 65536 */
+        if(threadIdx.x == 0) s_counts = all; /* each at most kCtaKeys */
         cluster.sync();
         for(uint32_t k = 0; k < rank; ++k) {
             const uint32_t c = *cluster.map_shared_rank(&s_counts, k);
@@ -859,7 +861,7 @@ extern "C" int gsx_b200_budget_select(const float *score, uint64_t score_stride,
     if(groups > (uint64_t)INT32_MAX || length > (uint64_t)INT32_MAX || budget > (uint64_t)INT32_MAX)
         return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "groups, length and budget must be below 2^31");
     if(groups > (length > kClusterKeys ? 65535u : 1u << 27))
-        return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "at most 65535 groups of more than 393216 entries, 2^27 of fewer");
+        return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "at most 65535 groups of more than 131072 entries, 2^27 of fewer");
     if(first > budget || recent > budget - first)
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "first + recent must be at most budget");
     if(groups == 0) return GSX_B200_SUCCESS;
@@ -886,9 +888,11 @@ extern "C" int gsx_b200_budget_select(const float *score, uint64_t score_stride,
     a.drop = drop;
     a.drop_stride = drop_stride;
     if(length <= kClusterKeys) {
-        /* as many CTAs as the keys need, and more while the GPU is not full (two an SM) and a part keeps 2048 entries */
+        /* as many CTAs as the keys need, and more while the GPU is not full (two an SM) and a part keeps 8192 entries
+         * (barriers between more CTAs cost more than they save: 32 groups of 32768 took 20.7 us with parts of 4096,
+         * 18.4 with 8192) */
         uint32_t ctas = 1;
-        while(ctas < 8 && (length > (uint64_t)ctas * kCtaKeys || (groups * ctas * 2 <= 148 * 2 && length >= (uint64_t)ctas * 2 * 2048)))
+        while(ctas < 8 && (length > (uint64_t)ctas * kCtaKeys || (groups * ctas * 2 <= 148 * 2 && length >= (uint64_t)ctas * 2 * 8192)))
             ctas *= 2;
         const size_t part = ((length + ctas - 1) / ctas + 3) / 4 * 4;
         cudaError_t e = gsx_allow_smem<select_cluster_kernel>(kCtaKeys * 4);

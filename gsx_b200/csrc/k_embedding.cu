@@ -641,6 +641,16 @@ __global__ void __launch_bounds__(kSortThreads) digit_scatter_kernel(const I *__
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     gsx_pdl_trigger();
     gsx_pdl_wait();
+    uint32_t begin, end;
+    chunk_range(kFirst ? count : __ldcg(n_pairs), begin, end);
+    uint32_t k[kSortItems], p[kSortItems];
+    bool valid[kSortItems];
+    auto load = [&](uint32_t i0) {
+        const int items = end - i0 >= (uint32_t)kTile ? kSortItems : (int)((end - i0 + kSortThreads - 1) / kSortThreads);
+        load_elements<I, kFirst, kSortItems>(index, pairs, i0 + (uint32_t)(warp * 32 * items + lane), 32, items, end, use, k, p, valid);
+        return items;
+    };
+    int items = begin < end ? load(begin) : 0; /* on their way while the counts are added up */
     {
         const uint32_t d = threadIdx.x & mask, parts = kSortThreads >> bits;
         uint32_t all = 0, before = 0;
@@ -666,19 +676,14 @@ __global__ void __launch_bounds__(kSortThreads) digit_scatter_kernel(const I *__
         if(kFirst && blockIdx.x == 0 && threadIdx.x == 0) *n_pairs = n;
         __syncthreads();
     }
-    uint32_t begin, end;
-    chunk_range(kFirst ? count : __ldcg(n_pairs), begin, end);
     for(uint32_t i0 = begin; i0 < end; i0 += kTile) {
-        const int items = end - i0 >= (uint32_t)kTile ? kSortItems : (int)((end - i0 + kSortThreads - 1) / kSortThreads);
-        uint32_t k[kSortItems], p[kSortItems];
-        bool valid[kSortItems];
-        load_elements<I, kFirst, kSortItems>(index, pairs, i0 + (uint32_t)(warp * 32 * items + lane), 32, items, end, use, k, p, valid);
         const uint32_t c = sort_tile(s, k, p, valid, items, shift, bits);
         if(threadIdx.x < bins) {
             s_to[threadIdx.x] = s_place[threadIdx.x] - s.before[threadIdx.x];
             s_place[threadIdx.x] += c;
             if(threadIdx.x == bins - 1) s_n = s.before[threadIdx.x] + c;
         }
+        if(end - i0 > (uint32_t)kTile) items = load(i0 + kTile); /* on their way while this tile is written */
         __syncthreads();
         const uint32_t n = s_n;
         for(uint32_t j = threadIdx.x; j < n; j += kSortThreads) {
@@ -868,15 +873,21 @@ __global__ void __launch_bounds__(kThreads) row_join_kernel(const Runs a, const 
     const uint32_t row = __ldcg(&a.pairs[b1 - 1].x);
     if(__ldcg(&a.pairs[b1].x) != row) return;
     if(b0 > 0 && __ldcg(&a.pairs[b0].x) == row && __ldcg(&a.pairs[b0 - 1].x) == row) return; /* began before */
-    /* the last CTA whose first position has the row */
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    /* the last CTA whose first position has the row: among the next 32, or by halving behind them */
     uint32_t lo = b + 1, hi = (n - 1) / R;
+    const uint32_t look = lo + lane <= hi ? __ldcg(&a.pairs[(uint64_t)(lo + lane) * R].x) : UINT32_MAX;
+    const unsigned same = __ballot_sync(0xffffffffu, look == row);
+    if(same != 0xffffffffu) {
+        hi = lo + (uint32_t)__ffs(~same) - 2; /* the first of them has the row */
+        lo = hi;
+    }
     while(lo < hi) {
         const uint32_t mid = (lo + hi + 1) / 2;
         if(__ldcg(&a.pairs[(uint64_t)mid * R].x) == row) lo = mid;
         else hi = mid - 1;
     }
     const uint32_t parts = lo - b;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t c0 = blockIdx.y * 256u;
     if(parts <= kFewParts) {
         const uint32_t c = c0 + threadIdx.x;

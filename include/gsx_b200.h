@@ -440,7 +440,7 @@ GSX_B200_API int gsx_b200_embedding_backward(const void *grad_out, int grad_type
  *   to +0.  kept[g] = min(entries in use, budget).  drop (may be NULL) receives the other entries, in increasing
  *   order: those in use less kept[g].  Places of keep and drop behind the lists are left as they were.
  *   workspace: gsx_b200_budget_workspace_bytes(groups, length) bytes of device memory, 4-byte aligned, of any
- *   content (0 bytes for groups of up to 393216 entries); calls that overlap on the GPU need one each.
+ *   content (0 bytes for groups of up to 131072 entries); calls that overlap on the GPU need one each.
  * gsx_b200_budget_gather: for every field and group, row r of dst = row keep[g, r] of src for r < kept[g]; later
  *   rows of dst are left as they were.  All fields in ONE launch.  Group g is (g / inner, g % inner) in a field's
  *   outer and inner strides (caches of [batch, head, entry] and [batch, entry, head] order alike).  A keep entry

@@ -101,8 +101,8 @@ def test_workspace_sizes():
     assert 4_000_000 < one < 8_000_000 <= two < 12_000_000
     # many positions, short rows and a table that fits shared memory: one table of sums for each of 296 chunks
     assert L.gsx_b200_embedding_workspace_bytes(3_000_000, 4096, 3) == 256 + 296 * 4096 * 3 * 4
-    assert L.gsx_b200_budget_workspace_bytes(32, 393_216) == 0
-    assert 0 < L.gsx_b200_budget_workspace_bytes(32, 393_217) < 4 << 20
+    assert L.gsx_b200_budget_workspace_bytes(32, 131_072) == 0
+    assert 0 < L.gsx_b200_budget_workspace_bytes(32, 131_073) < 4 << 20
 
 
 def test_python_calls_refuse_host_tensors():

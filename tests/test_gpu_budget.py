@@ -132,7 +132,7 @@ def _check_select(score, budget, lengths=None, first=0, recent=0):
 
 
 SELECT_SIZES = [(1, 1, 0), (1, 1, 1), (2, 5, 3), (3, 33, 32), (4, 1000, 1), (2, 1025, 1024), (3, 5000, 2500),
-                (1, 49_152, 30_000), (2, 49_153, 100), (3, 100_001, 77_777), (1, 400_000, 399_999), (40, 60_000, 512), (3, 393_216, 20_000),
+                (1, 49_152, 30_000), (2, 49_153, 100), (3, 100_001, 77_777), (1, 400_000, 399_999), (40, 60_000, 512), (3, 131_072, 20_000), (2, 131_073, 200),
                 (2, 393_217, 200_000), (1, 1_000_003, 400_000), (5, 500_000, 7)]
 
 
