@@ -294,6 +294,38 @@ __device__ __forceinline__ int place_of(const Select &a, uint32_t n, uint32_t j,
     return is_protected(a, n, j) || key > t ? 1 : key == t ? 0 : -1;
 }
 
+/* A tile of compact(): four consecutive entries a thread.  kWhole: all lie before `end`.  kMiddle: none is protected. */
+template <bool kWhole, bool kMiddle>
+__device__ __forceinline__ void compact_tile(const Select &a, uint32_t n, uint32_t j0, uint32_t end, uint32_t &gt0, uint32_t &eq0,
+                                             uint32_t t, uint32_t need, const uint32_t (&key)[4], int32_t *keep, int32_t *drop,
+                                             uint32_t *s_warp)
+{
+    bool gt[4], eq[4];
+    uint32_t sum = 0; /* above | equal << 16 */
+#pragma unroll
+    for(int k = 0; k < 4; ++k) {
+        const bool in = kWhole || j0 + k < end;
+        const bool forced = !kMiddle && is_protected(a, n, j0 + k);
+        gt[k] = in && (forced || key[k] > t);
+        eq[k] = in && !forced && key[k] == t;
+        sum += (gt[k] ? 1u : 0u) + (eq[k] ? 0x10000u : 0u);
+    }
+    uint32_t all;
+    const uint32_t before = block_scan(sum, s_warp, &all) - sum;
+    uint32_t g = gt0 + (before & 0xffffu), e = eq0 + (before >> 16);
+#pragma unroll
+    for(int k = 0; k < 4; ++k) {
+        const uint32_t kept_before = g + (e < need ? e : need);
+        const bool stays = gt[k] || (eq[k] && e < need);
+        if(stays) keep[kept_before] = (int32_t)(j0 + k);
+        if(drop != nullptr && !stays && (kWhole || j0 + k < end)) drop[j0 + k - kept_before] = (int32_t)(j0 + k);
+        g += gt[k] ? 1u : 0u;
+        e += eq[k] ? 1u : 0u;
+    }
+    gt0 += all & 0xffffu;
+    eq0 += all >> 16;
+}
+
 /* Ordered compaction of [begin, end): entries above the threshold (or protected) and the first `need` equal ones go
  * to keep, the others to drop.  gt0 / eq0: entries above / equal before `begin`.  load(j, key) gives the keys of four
  * consecutive entries, of which those behind `end` are not looked at. */
@@ -303,31 +335,16 @@ __device__ __forceinline__ void compact(const Select &a, uint32_t g, uint32_t n,
 {
     int32_t *keep = a.keep + (uint64_t)g * a.keep_stride;
     int32_t *drop = a.drop != nullptr ? a.drop + (uint64_t)g * a.drop_stride : nullptr;
-    for(uint32_t base = begin; base < end; base += blockDim.x * 4) {
+    const uint32_t tile = blockDim.x * 4;
+    for(uint32_t base = begin; base < end; base += tile) {
         const uint32_t j0 = base + threadIdx.x * 4;
-        uint32_t key[4];
-        int at[4];
-        uint32_t sum = 0; /* above | equal << 16 */
-        load(j0, key);
-#pragma unroll
-        for(int k = 0; k < 4; ++k) {
-            at[k] = j0 + k < end ? place_of(a, n, j0 + k, key[k], t) : -1;
-            sum += at[k] > 0 ? 1u : at[k] == 0 ? 0x10000u : 0u;
-        }
-        uint32_t all;
-        const uint32_t before = block_scan(sum, s_warp, &all) - sum;
-        uint32_t gt = gt0 + (before & 0xffffu), eq = eq0 + (before >> 16);
-#pragma unroll
-        for(int k = 0; k < 4; ++k)
-            if(j0 + k < end) {
-                const uint32_t kept_before = gt + (eq < need ? eq : need);
-                if(at[k] > 0 || (at[k] == 0 && eq < need)) keep[kept_before] = (int32_t)(j0 + k);
-                else if(drop != nullptr) drop[j0 + k - kept_before] = (int32_t)(j0 + k);
-                gt += at[k] > 0;
-                eq += at[k] == 0;
-            }
-        gt0 += all & 0xffffu;
-        eq0 += all >> 16;
+        const bool whole = end - base >= tile;
+        uint32_t key[4] = {};
+        load(j0, key, whole);
+        if(whole && base >= a.first && base + tile <= n - a.recent)
+            compact_tile<true, true>(a, n, j0, end, gt0, eq0, t, need, key, keep, drop, s_warp);
+        else
+            compact_tile<false, false>(a, n, j0, end, gt0, eq0, t, need, key, keep, drop, s_warp);
     }
 }
 
@@ -351,15 +368,15 @@ __global__ void __launch_bounds__(kCtaThreads) select_cluster_kernel(const Selec
         for(uint32_t j = begin + threadIdx.x; j < end; j += kCtaThreads) a.keep[(uint64_t)g * a.keep_stride + j] = (int32_t)j;
         return;
     }
-    for(uint32_t j0 = begin + threadIdx.x; j0 < end; j0 += kCtaThreads * 4) {
+    uint32_t j0 = begin; /* whole rounds without a condition an entry, then the rest */
+    for(; end - j0 >= kCtaThreads * 4; j0 += kCtaThreads * 4) {
         float x[4];
 #pragma unroll
-        for(int k = 0; k < 4; ++k)
-            if(j0 + k * kCtaThreads < end) x[k] = __ldg(score + j0 + k * kCtaThreads);
+        for(int k = 0; k < 4; ++k) x[k] = __ldg(score + j0 + threadIdx.x + k * kCtaThreads);
 #pragma unroll
-        for(int k = 0; k < 4; ++k)
-            if(j0 + k * kCtaThreads < end) s_keys[j0 + k * kCtaThreads - begin] = key_of(x[k]);
+        for(int k = 0; k < 4; ++k) s_keys[j0 + threadIdx.x + k * kCtaThreads - begin] = key_of(x[k]);
     }
+    for(uint32_t j = j0 + threadIdx.x; j < end; j += kCtaThreads) s_keys[j - begin] = key_of(__ldg(score + j));
     uint32_t need = a.budget - a.first - a.recent, prefix = 0;
     uint32_t t = 0xffffffffu; /* no key reaches 0xffffffff */
     const uint32_t from = begin > a.first ? begin : a.first, to = end < n - a.recent ? end : n - a.recent;
@@ -421,7 +438,7 @@ __global__ void __launch_bounds__(kCtaThreads) select_cluster_kernel(const Selec
         cluster.sync(); /* nobody leaves while its counts are read */
     }
     compact(a, g, n, begin, end, gt0, eq0, t, need,
-            [&](uint32_t j, uint32_t (&key)[4]) {
+            [&](uint32_t j, uint32_t (&key)[4], bool) {
                 if(j >= end) return;
                 const uint4 v = *reinterpret_cast<const uint4 *>(s_keys + (j - begin));
                 key[0] = v.x;
@@ -469,27 +486,39 @@ __device__ __forceinline__ void segment(uint32_t n, uint32_t &begin, uint32_t &e
 __device__ __forceinline__ bool last_block(uint32_t *ticket)
 {
     __shared__ bool s_last;
-    __threadfence();
     __syncthreads();
-    if(threadIdx.x == 0) s_last = atomicAdd(ticket, 1u) == gridDim.x - 1;
+    if(threadIdx.x == 0) { /* its fences stand for the block: what the others wrote is ordered by the barriers */
+        __threadfence();
+        s_last = atomicAdd(ticket, 1u) == gridDim.x - 1;
+        __threadfence();
+    }
     __syncthreads();
-    if(s_last) __threadfence();
     return s_last;
 }
 
-/* f(entry, key) for the entries [begin, end) of a group, dealt to the threads, eight loads in flight */
+/* f(entry, key) for the entries [begin, end) of a group, dealt to the threads, eight loads in flight; whole rounds without a
+ * condition an entry (one makes a branch of each) */
 template <typename F>
 __device__ __forceinline__ void for_keys(const float *__restrict__ score, uint32_t begin, uint32_t end, const F &f)
 {
-    for(uint32_t j0 = begin + threadIdx.x; j0 < end; j0 += kSegThreads * 8) {
+    uint32_t j0 = begin;
+    for(; end - j0 >= kSegThreads * 8; j0 += kSegThreads * 8) {
         float x[8];
 #pragma unroll
-        for(int k = 0; k < 8; ++k)
-            if(j0 + k * kSegThreads < end) x[k] = __ldg(score + j0 + k * kSegThreads);
+        for(int k = 0; k < 8; ++k) x[k] = __ldg(score + j0 + threadIdx.x + k * kSegThreads);
 #pragma unroll
-        for(int k = 0; k < 8; ++k)
-            if(j0 + k * kSegThreads < end) f(j0 + k * kSegThreads, key_of(x[k]));
+        for(int k = 0; k < 8; ++k) f(j0 + threadIdx.x + k * kSegThreads, key_of(x[k]));
     }
+    if(j0 >= end) return;
+    float x[8]; /* entries behind the end are read in the place of the last */
+#pragma unroll
+    for(int k = 0; k < 8; ++k) {
+        const uint32_t j = j0 + threadIdx.x + k * kSegThreads;
+        x[k] = __ldg(score + (j < end ? j : end - 1));
+    }
+#pragma unroll
+    for(int k = 0; k < 8; ++k)
+        if(j0 + threadIdx.x + k * kSegThreads < end) f(j0 + threadIdx.x + k * kSegThreads, key_of(x[k]));
 }
 
 template <int P>
@@ -602,15 +631,23 @@ __global__ void __launch_bounds__(kSegThreads) select_write_kernel(const Select 
     threshold(a, w.state + (uint64_t)g * kState, t, need);
     const uint32_t *counts = w.counts + ((uint64_t)g * gridDim.x + blockIdx.x) * 2;
     const float *score = a.score + (uint64_t)g * a.score_stride;
+    const bool wide = (uintptr_t)(score + begin) % 16 == 0;
     compact(a, g, n, begin, end, __ldcg(counts), __ldcg(counts + 1), t, need,
-            [&](uint32_t j, uint32_t (&key)[4]) {
-                float x[4];
+            [&](uint32_t j, uint32_t (&key)[4], bool whole) {
+                float x[4] = {};
+                if(whole && wide) {
+                    const float4 v = __ldg(reinterpret_cast<const float4 *>(score + j));
+                    x[0] = v.x;
+                    x[1] = v.y;
+                    x[2] = v.z;
+                    x[3] = v.w;
+                } else {
 #pragma unroll
-                for(int k = 0; k < 4; ++k)
-                    if(j + k < end) x[k] = __ldg(score + j + k);
+                    for(int k = 0; k < 4; ++k)
+                        if(j + k < end) x[k] = __ldg(score + j + k);
+                }
 #pragma unroll
-                for(int k = 0; k < 4; ++k)
-                    if(j + k < end) key[k] = key_of(x[k]);
+                for(int k = 0; k < 4; ++k) key[k] = key_of(x[k]);
             },
             s_warp);
 }
