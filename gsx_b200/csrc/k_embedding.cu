@@ -186,28 +186,31 @@ __global__ void __launch_bounds__(kTable ? 1024 : kThreads) lookup_short_kernel(
     }
 }
 
-/* Any row: 2^CLOG lanes take a row's elements side by side (NC of them each, 2^CLOG apart), a warp 32 consecutive rows,
- * whose indices it loads at once and hands round; U steps of rows in flight.  Longer rows than 32 * NC take several
- * turns. */
-template <typename T, typename O, typename I, int NC, int CLOG>
+/* Any row: 2^CLOG lanes take a row's elements side by side (NC of them each, 2^CLOG apart), a warp ROWS consecutive
+ * rows, whose indices it loads at once and hands round, with U steps of rows in flight.  Longer rows than NC * 32 are cut
+ * into tiles (y).  Elements and rows that are not there are read in the place of ones that are (a load under a condition
+ * becomes a branch of some ten instructions) and not stored.  1M rows of 45 from 16-bit rows: 43 us, bound by the
+ * instructions an element (0.66 of the issue slots); writing its 180 MB alone takes 28. */
+template <typename T, typename O, typename I, int NC, int CLOG, int ROWS>
 __global__ void __launch_bounds__(kThreads) lookup_warp_kernel(const T *__restrict__ table, uint32_t rows, uint32_t dim,
                                                                uint32_t stride_bytes, const I *__restrict__ index,
                                                                uint64_t count, float scale, O *__restrict__ out,
                                                                uint64_t out_stride, uint32_t *__restrict__ bad)
 {
-    constexpr int U = 8 / NC, cl = 1 << CLOG, per = 32 >> CLOG; /* rows a step */
+    constexpr int kSteps = ROWS >> (5 - CLOG), U = 8 / NC < kSteps ? 8 / NC : kSteps, per = 32 >> CLOG; /* rows a step */
+    static_assert(kSteps % U == 0, "whole rounds");
     const int lane = threadIdx.x & 31;
-    const uint64_t n0 = ((uint64_t)blockIdx.x * kWarps + (threadIdx.x >> 5)) * 32;
+    const uint64_t n0 = ((uint64_t)blockIdx.x * kWarps + (threadIdx.x >> 5)) * ROWS;
     if(n0 >= count) return;
-    const int left = count - n0 < 32 ? (int)(count - n0) : 32;
+    const int left = count - n0 < ROWS ? (int)(count - n0) : ROWS;
     const uint32_t mine = lane < left ? row_number(__ldg(index + n0 + lane)) : UINT32_MAX;
     if(bad != nullptr && lane < left && mine >= rows) atomicExch(bad, 1u);
     if(rows == 0) return;
     const unsigned char *bytes = reinterpret_cast<const unsigned char *>(table);
     const uint64_t hop = out_stride * per;
-    for(uint32_t c0 = lane & (cl - 1); c0 - (lane & (cl - 1)) < dim; c0 += NC << CLOG) {
-        /* elements and rows that are not there are read in the place of ones that are (a load under a condition becomes a
-         * branch of some ten instructions) and not stored */
+    uint32_t tile = NC == 4 ? blockIdx.y : 0;
+    do {
+        const uint32_t c0 = tile * (NC << CLOG) + (lane & ((1 << CLOG) - 1));
         const unsigned char *from[NC];
         bool in[NC];
 #pragma unroll
@@ -218,7 +221,7 @@ __global__ void __launch_bounds__(kThreads) lookup_warp_kernel(const T *__restri
         }
         O *to = out + (n0 + (lane >> CLOG)) * out_stride + c0;
 #pragma unroll 1
-        for(int j = 0; j < cl; j += U) { /* cl steps of `per` rows are the warp's 32 */
+        for(int j = 0; j < kSteps; j += U) {
             uint32_t s[U];
             T x[U][NC];
 #pragma unroll
@@ -236,7 +239,8 @@ __global__ void __launch_bounds__(kThreads) lookup_warp_kernel(const T *__restri
                 to += hop;
             }
         }
-    }
+        tile += gridDim.y;
+    } while(NC == 4 && tile * (uint64_t)(NC << CLOG) < dim);
 }
 
 template <typename T, typename O, typename I, int DIM>
@@ -258,6 +262,27 @@ cudaError_t launch_short(const T *table, uint32_t rows, uint32_t stride_bytes, c
     return cudaSuccess;
 }
 
+/* whether the call can move packs of VW elements; if so, it has */
+template <typename T, typename O, typename I, int VW>
+bool launch_packs(const T *table, uint64_t rows, uint64_t dim, uint64_t table_stride, const I *index, uint64_t count, float scale,
+                  O *out, uint64_t out_stride, uint32_t *bad, cudaStream_t stream)
+{
+    constexpr uint64_t TA = alignof(Pack<T, VW>), OA = alignof(Pack<O, VW>);
+    if(dim % VW != 0 || (uintptr_t)table % TA != 0 || table_stride * sizeof(T) % TA != 0 || (uintptr_t)out % OA != 0 ||
+       out_stride * sizeof(O) % OA != 0)
+        return false;
+    const uint64_t accesses = count * (dim / VW);
+    if(accesses >= 148ull * 2048 * 2) {
+        const uint64_t per = kThreads * 4;
+        lookup_pack_kernel<T, O, I, VW, 4><<<(unsigned)((accesses + per - 1) / per), kThreads, 0, stream>>>(
+            table, rows, (uint32_t)(dim / VW), table_stride, index, accesses, scale, out, out_stride, bad);
+    } else {
+        lookup_pack_kernel<T, O, I, VW, 1><<<(unsigned)((accesses + kThreads - 1) / kThreads), kThreads, 0, stream>>>(
+            table, rows, (uint32_t)(dim / VW), table_stride, index, accesses, scale, out, out_stride, bad);
+    }
+    return true;
+}
+
 template <typename T, typename O, typename I>
 cudaError_t launch_lookup(const void *table_, uint64_t rows, uint64_t dim, uint64_t table_stride, const void *index_,
                           uint64_t count, float scale, void *out_, uint64_t out_stride, uint32_t *bad, cudaStream_t stream)
@@ -265,10 +290,6 @@ cudaError_t launch_lookup(const void *table_, uint64_t rows, uint64_t dim, uint6
     const T *table = static_cast<const T *>(table_);
     const I *index = static_cast<const I *>(index_);
     O *out = static_cast<O *>(out_);
-    constexpr int VW = 16 / sizeof(T);
-    constexpr int OV = 16 / sizeof(O);
-    const bool packs = dim % VW == 0 && table_stride % VW == 0 && (uintptr_t)table % 16 == 0 &&
-                       (out_stride * sizeof(O)) % 16 == 0 && (uintptr_t)out % 16 == 0 && dim % OV == 0;
     const uint32_t stride_bytes = (uint32_t)(table_stride * sizeof(T));
     if(dim <= 4 && out_stride == dim && (uintptr_t)out % 16 == 0) {
         switch(dim) {
@@ -278,28 +299,25 @@ cudaError_t launch_lookup(const void *table_, uint64_t rows, uint64_t dim, uint6
         default: return launch_short<T, O, I, 4>(table, (uint32_t)rows, stride_bytes, index, count, scale, out, bad, stream);
         }
     }
-    if(packs) {
-        const uint64_t accesses = count * (dim / VW);
-        if(accesses >= 148ull * 2048 * 2) {
-            const uint64_t per = kThreads * 4;
-            lookup_pack_kernel<T, O, I, VW, 4><<<(unsigned)((accesses + per - 1) / per), kThreads, 0, stream>>>(
-                table, rows, (uint32_t)(dim / VW), table_stride, index, accesses, scale, out, out_stride, bad);
-        } else {
-            lookup_pack_kernel<T, O, I, VW, 1><<<(unsigned)((accesses + kThreads - 1) / kThreads), kThreads, 0, stream>>>(
-                table, rows, (uint32_t)(dim / VW), table_stride, index, accesses, scale, out, out_stride, bad);
-        }
+    /* the widest pack of elements that every row is a whole number of, on both sides */
+    constexpr int VW = 16 / sizeof(T);
+    if(launch_packs<T, O, I, VW>(table, rows, dim, table_stride, index, count, scale, out, out_stride, bad, stream) ||
+       launch_packs<T, O, I, VW / 2>(table, rows, dim, table_stride, index, count, scale, out, out_stride, bad, stream))
         return cudaSuccess;
-    }
-    const unsigned ctas = (unsigned)((count + kWarps * 32 - 1) / (kWarps * 32));
-    auto launch = [&](auto kernel) {
-        kernel<<<ctas, kThreads, 0, stream>>>(table, (uint32_t)rows, (uint32_t)dim, stride_bytes, index, count, scale, out,
-                                              out_stride, bad);
+    if(VW == 8 && launch_packs<T, O, I, VW == 8 ? 2 : VW>(table, rows, dim, table_stride, index, count, scale, out, out_stride, bad, stream))
+        return cudaSuccess;
+    auto launch = [&](auto kernel, uint64_t warp_rows, uint64_t tiles) {
+        const uint64_t ctas = (count + kWarps * warp_rows - 1) / (kWarps * warp_rows);
+        kernel<<<dim3((unsigned)ctas, (unsigned)(tiles < 65535 ? tiles : 65535)), kThreads, 0, stream>>>(
+            table, (uint32_t)rows, (uint32_t)dim, stride_bytes, index, count, scale, out, out_stride, bad);
     };
-    if(dim <= 8) launch(lookup_warp_kernel<T, O, I, 1, 3>);
-    else if(dim <= 16) launch(lookup_warp_kernel<T, O, I, 1, 4>);
-    else if(dim <= 32) launch(lookup_warp_kernel<T, O, I, 1, 5>);
-    else if(dim <= 64) launch(lookup_warp_kernel<T, O, I, 2, 5>);
-    else launch(lookup_warp_kernel<T, O, I, 4, 5>);
+    const uint64_t tiles = (dim + 127) / 128;
+    if(dim <= 8) launch(lookup_warp_kernel<T, O, I, 1, 3, 32>, 32, 1);
+    else if(dim <= 16) launch(lookup_warp_kernel<T, O, I, 1, 4, 32>, 32, 1);
+    else if(dim <= 32) launch(lookup_warp_kernel<T, O, I, 1, 5, 32>, 32, 1);
+    else if(dim <= 64) launch(lookup_warp_kernel<T, O, I, 2, 5, 32>, 32, 1);
+    else if((count + 31) / 32 * tiles >= 148 * 32) launch(lookup_warp_kernel<T, O, I, 4, 5, 32>, 32, tiles);
+    else launch(lookup_warp_kernel<T, O, I, 4, 5, 2>, 2, tiles); /* few long rows: 4 of 2709 took 69 us at 32 a warp */
     return cudaSuccess;
 }
 

@@ -41,7 +41,8 @@ def _check_lookup(out, table, index, scale):
 def test_lookup_types(cuda_device, table_type, out_type, itype):
     g = _gen(1)
     for count, rows, dim in [(1, 1, 1), (1, 5, 4096), (7, 3, 8), (1000, 17, 3), (1001, 300, 45), (513, 1000, 128),
-                             (40, 2, 12)]:
+                             (40, 2, 12), (4, 7, 2709), (43, 9, 685), (999, 20, 131), (130, 6, 33), (77, 9, 6),
+                             (77, 9, 20), (50, 9, 300)]:
         table = torch.randn(rows, dim, generator=g, device="cuda").to(table_type)
         index = _index(g, count, rows, itype)
         _check_lookup(gb.embedding_lookup(table, index, out=torch.empty(count, dim, dtype=out_type, device="cuda"),
@@ -51,7 +52,8 @@ def test_lookup_types(cuda_device, table_type, out_type, itype):
 def test_lookup_large_takes_every_path(cuda_device):
     g = _gen(2)
     for count, rows, dim, dtype in [(400_003, 4096, 3, F32), (200_001, 1000, 45, BF16), (300_000, 64, 32, F16),
-                                    (3_000_001, 1, 1, F32), (1_500_000, 700, 9, F16), (70_001, 5, 31, BF16)]:
+                                    (3_000_001, 1, 1, F32), (1_500_000, 700, 9, F16), (70_001, 5, 31, BF16),
+                                    (100_003, 50, 130, BF16), (200_000, 40, 28, F16)]:
         table = torch.randn(rows, dim, generator=g, device="cuda").to(dtype)
         for itype in (torch.int32, torch.int64):
             index = _index(g, count, rows, itype, 2.0)
