@@ -67,54 +67,72 @@ struct alignas(sizeof(T) * VW > 16 ? 16 : sizeof(T) * VW) Pack {
 /* ------------------------------------------------------------------------------------------ */
 /* lookup */
 
-/* rows of whole VW-element packs: one pack per thread and step */
-template <typename T, typename O, typename I, int VW, int U>
-__global__ void __launch_bounds__(kThreads) lookup_pack_kernel(const T *__restrict__ table, uint64_t rows,
-                                                               uint32_t packs, uint64_t table_stride,
-                                                               const I *__restrict__ index, uint64_t total, float scale,
-                                                               O *__restrict__ out, uint64_t out_stride,
-                                                               uint32_t *__restrict__ bad)
-{
-    const uint64_t w0 = (uint64_t)blockIdx.x * (kThreads * U) + threadIdx.x;
-    uint64_t n[U];
-    uint32_t c[U];
-    I s[U];
-    Pack<T, VW> x[U];
-#pragma unroll
-    for(int u = 0; u < U; ++u) {
-        const uint64_t w = w0 + (uint64_t)u * kThreads;
-        n[u] = total <= 0xffffffffull ? (uint64_t)((uint32_t)w / packs) : w / packs;
-        c[u] = (uint32_t)(w - n[u] * packs);
-        s[u] = w < total ? __ldg(index + n[u]) : (I)-1;
-    }
-    if(rows == 0) {
-        if(w0 < total && bad != nullptr) atomicExch(bad, 1u);
-        return;
-    }
-#pragma unroll
-    for(int u = 0; u < U; ++u) {
-        const uint64_t row = (uint64_t)s[u] < rows ? (uint64_t)s[u] : 0; /* a negative index is a large one here */
-        x[u] = *reinterpret_cast<const Pack<T, VW> *>(table + row * table_stride + (uint64_t)c[u] * VW);
-    }
-#pragma unroll
-    for(int u = 0; u < U; ++u) {
-        if(w0 + (uint64_t)u * kThreads >= total) continue;
-        if((uint64_t)s[u] >= rows) {
-            if(bad != nullptr && c[u] == 0) atomicExch(bad, 1u);
-            continue;
-        }
-        Pack<O, VW> y;
-#pragma unroll
-        for(int k = 0; k < VW; ++k) y.v[k] = from_f32<O>(scale * to_f32(x[u].v[k]));
-        *reinterpret_cast<Pack<O, VW> *>(out + n[u] * out_stride + (uint64_t)c[u] * VW) = y;
-    }
-}
-
 /* an index as a row number, or a number no table has */
 template <typename I>
 __device__ __forceinline__ uint32_t row_number(I v)
 {
     return sizeof(I) == 8 && ((uint64_t)v >> 32) != 0 ? UINT32_MAX : (uint32_t)v;
+}
+
+/* i / d for i < 2^31 by one multiplication (division by an invariant, Granlund and Montgomery 1994): with 2^s >= d
+ * and m = floor(2^(31 + s) / d) + 1, i / d = i * m >> (31 + s) */
+struct Divider {
+    uint32_t mul, shift;
+    explicit Divider(uint32_t d) : mul(0), shift(0)
+    {
+        while((1ull << shift) < d) ++shift;
+        if(shift) mul = (uint32_t)((1ull << (31 + shift)) / d + 1);
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t i) const { return shift ? __umulhi(i, mul) >> (shift - 1) : i; }
+};
+
+/* Rows of whole VW-element packs: a CTA makes U * kThreads packs of out in order, U of a thread in flight.  Packs behind the
+ * end, and of rows that are not there, are read in the place of row 0 and not stored.  kDense: the rows of out have
+ * no gaps. */
+template <typename T, typename O, typename I, int VW, int U, bool kDense>
+__global__ void __launch_bounds__(kThreads) lookup_pack_kernel(const T *__restrict__ table, uint32_t rows, uint32_t packs,
+                                                               uint32_t stride_bytes, const I *__restrict__ index,
+                                                               uint64_t count, uint64_t total, float scale,
+                                                               O *__restrict__ out, uint64_t out_stride,
+                                                               const Divider by_packs, uint32_t *__restrict__ bad)
+{
+    const uint64_t w0 = (uint64_t)blockIdx.x * (kThreads * U);
+    const uint64_t n0 = total <= 0xffffffffull ? (uint64_t)((uint32_t)w0 / packs) : w0 / packs; /* the CTA's first row */
+    const uint32_t c0 = (uint32_t)(w0 - n0 * packs) + threadIdx.x;
+    const uint32_t left = total - w0 < kThreads * U ? (uint32_t)(total - w0) : kThreads * U;
+    const uint32_t last = (uint32_t)(count - 1 - n0 < 0x7fffffffull ? count - 1 - n0 : 0x7fffffffull);
+    const I *ix = index + n0;
+    uint32_t n[U], s[U];
+    Pack<T, VW> x[U];
+#pragma unroll
+    for(int u = 0; u < U; ++u) {
+        n[u] = by_packs(c0 + u * kThreads);
+        s[u] = row_number(__ldg(ix + (n[u] < last ? n[u] : last)));
+    }
+    if(rows == 0) {
+        if(bad != nullptr) atomicExch(bad, 1u);
+        return;
+    }
+    const unsigned char *bytes = reinterpret_cast<const unsigned char *>(table);
+#pragma unroll
+    for(int u = 0; u < U; ++u) {
+        const unsigned char *row = bytes + (uint64_t)(s[u] < rows ? s[u] : 0u) * stride_bytes;
+        x[u] = reinterpret_cast<const Pack<T, VW> *>(row)[c0 + u * kThreads - n[u] * packs];
+    }
+    bool all = true;
+#pragma unroll
+    for(int u = 0; u < U; ++u) {
+        Pack<O, VW> y;
+#pragma unroll
+        for(int k = 0; k < VW; ++k) y.v[k] = from_f32<O>(scale * to_f32(x[u].v[k]));
+        const bool in = threadIdx.x + u * kThreads < left;
+        all &= s[u] < rows || !in;
+        if(s[u] < rows && in) {
+            if(kDense) (reinterpret_cast<Pack<O, VW> *>(out) + w0)[threadIdx.x + u * kThreads] = y;
+            else reinterpret_cast<Pack<O, VW> *>(out + (n0 + n[u]) * out_stride)[c0 + u * kThreads - n[u] * packs] = y;
+        }
+    }
+    if(!all && bad != nullptr) atomicExch(bad, 1u);
 }
 
 /* Rows of DIM <= 4 elements into an out without gaps: a thread makes R of them, whole 16-byte stores.  A lane an element
@@ -271,14 +289,20 @@ bool launch_packs(const T *table, uint64_t rows, uint64_t dim, uint64_t table_st
     if(dim % VW != 0 || (uintptr_t)table % TA != 0 || table_stride * sizeof(T) % TA != 0 || (uintptr_t)out % OA != 0 ||
        out_stride * sizeof(O) % OA != 0)
         return false;
-    const uint64_t accesses = count * (dim / VW);
-    if(accesses >= 148ull * 2048 * 2) {
-        const uint64_t per = kThreads * 4;
-        lookup_pack_kernel<T, O, I, VW, 4><<<(unsigned)((accesses + per - 1) / per), kThreads, 0, stream>>>(
-            table, rows, (uint32_t)(dim / VW), table_stride, index, accesses, scale, out, out_stride, bad);
+    const uint64_t total = count * (dim / VW);
+    const Divider by_packs((uint32_t)(dim / VW));
+    auto launch = [&](auto kernel, uint64_t per) {
+        kernel<<<(unsigned)((total + per - 1) / per), kThreads, 0, stream>>>(table, (uint32_t)rows, (uint32_t)(dim / VW),
+                                                                             (uint32_t)(table_stride * sizeof(T)), index, count,
+                                                                             total, scale, out, out_stride, by_packs, bad);
+    };
+    const bool dense = out_stride == dim;
+    if(total >= 148ull * 2048 * 2) {
+        if(dense) launch(lookup_pack_kernel<T, O, I, VW, 4, true>, kThreads * 4);
+        else launch(lookup_pack_kernel<T, O, I, VW, 4, false>, kThreads * 4);
     } else {
-        lookup_pack_kernel<T, O, I, VW, 1><<<(unsigned)((accesses + kThreads - 1) / kThreads), kThreads, 0, stream>>>(
-            table, rows, (uint32_t)(dim / VW), table_stride, index, accesses, scale, out, out_stride, bad);
+        if(dense) launch(lookup_pack_kernel<T, O, I, VW, 1, true>, kThreads);
+        else launch(lookup_pack_kernel<T, O, I, VW, 1, false>, kThreads);
     }
     return true;
 }
