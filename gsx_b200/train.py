@@ -181,6 +181,8 @@ class Trainer:
         that colour, taken with all colours grey so that none is clamped, so it follows the backward's rule and counts
         alphas below 1/255 as well; model.grads is overwritten.)"""
         m = self.model
+        for f, rows in self.shared.items():
+            rows.expand(m.params[f])
         grey = dict(m.params, sh0=torch.zeros_like(m.params["sh0"]))
         self.renderer.render(self.ctx, grey, camera, self.out, background=self.background, sh_degree=0,
                              forward_type=FORWARD_TRAIN)
@@ -195,11 +197,13 @@ class Trainer:
         m = self.model
         if self.group is not None:
             raise GsxError(NOT_SUPPORTED, "keep_budget runs on one GPU")
-        if score.shape != (m.n,) or budget < 1:
-            raise GsxError(INVALID_ARGUMENT, "score must hold one value per Gaussian, the budget be at least one")
+        if score.shape != (m.n,) or score.dtype != torch.float32 or budget < 1:
+            raise GsxError(INVALID_ARGUMENT, "score must hold one float32 value per Gaussian, the budget be at least one")
         if budget >= m.n:
             return score
         keep, kept = budget_select(score, budget, first=first, recent=recent)
+        for f, rows in self.shared.items():  # the tables may have moved since the last render
+            rows.expand(m.params[f])
         before, optim = m.params, self.optim
         m._allocate(int(budget), m.flat_param.device)
         out = torch.empty(m.n, dtype=torch.float32, device=score.device)

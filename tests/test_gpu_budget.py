@@ -247,6 +247,19 @@ def test_gather_caches_of_both_layouts(cuda_device, order):
             assert torch.equal(k2[b, h, n:], k0[b, h, n:])
 
 
+def test_gather_offsets_behind_32_bits(cuda_device):
+    for row in (12, 1008):  # short rows and long ones, 4.8 GB each
+        n = 4_800_000_000 // row
+        src = torch.zeros(n, row, dtype=torch.uint8, device="cuda")
+        src[-1] = 9
+        src[-3] = 4
+        keep = torch.tensor([0, n - 3, n - 1], dtype=torch.int32, device="cuda")
+        dst = torch.full((3, row), 1, dtype=torch.uint8, device="cuda")
+        gb.budget_gather([(src, dst)], keep, torch.tensor(3, dtype=torch.int32, device="cuda"))
+        assert dst[:, 0].tolist() == [0, 4, 9] and torch.equal(dst, dst[:, :1].expand(3, row))
+        del src
+
+
 @pytest.mark.parametrize("dim", [1, 3, 4, 9])
 def test_gather_flags_entries_out_of_range(cuda_device, dim):
     src = torch.randn(10, dim, device="cuda")

@@ -250,6 +250,35 @@ def test_gradients_that_are_not_finite_stay_in_their_rows(cuda_device):
         assert bool(finite.all())
 
 
+def test_offsets_behind_32_bits(cuda_device):
+    """Tables, outputs and gradients of more than 4 GiB: their last rows are read and written at their own place."""
+    dim = 1024
+    rows = 2_300_000  # 4.7 GB of bf16
+    index = torch.tensor([rows - 1, 5, rows - 2, rows - 1], device="cuda")
+    table = torch.zeros(rows, dim, dtype=BF16, device="cuda")
+    table[rows - 2:] = 3.0
+    table[5] = 7.0
+    out = gb.embedding_lookup(table, index, scale=2.0)
+    assert out[:, 0].tolist() == [6.0, 14.0, 6.0, 6.0] and torch.equal(out, out[:, :1].expand(-1, dim))
+    got = gb.embedding_backward(torch.ones(4, dim, dtype=BF16, device="cuda"), index, table)
+    assert bool((got[rows - 1] == 2).all()) and bool((got[rows - 2] == 1).all()) and bool((got[5] == 1).all())
+    assert int((got != 0).any(1).sum()) == 3
+    del got
+    grad = table.zero_()  # as a gradient of 2.3M positions
+    grad[-1] = 4.0
+    grad[1] = 0.5
+    which = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    which[-1] = 1
+    got = gb.embedding_backward(grad, which, torch.empty(300, dim, device="cuda"))
+    assert bool((got[1] == 4).all()) and bool((got[0] == 0.5).all()) and bool((got[2:] == 0).all())
+    small = torch.arange(12, device="cuda").view(3, 4).float()  # an out of more than 2^32 bytes, short rows
+    where = torch.zeros(280_000_000, dtype=torch.int32, device="cuda")
+    where[-1] = 2
+    del table, grad, got
+    out = gb.embedding_lookup(small, where)
+    assert torch.equal(out[-1], small[2]) and torch.equal(out[-2], small[0]) and torch.equal(out[0], small[0])
+
+
 def test_very_long_rows_and_empty_tables(cuda_device):
     g = _gen(14)
     for dim in (70_001, 65_536):

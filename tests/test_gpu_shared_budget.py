@@ -108,6 +108,15 @@ def test_train_evict_and_train_on(cuda_device):
     assert bool(torch.isfinite(loss).all()) and tr.optim.steps[0] == 5
 
 
+def test_a_table_set_between_renders_is_seen(cuda_device):
+    tr, cam, _ = _trainer(n=500)
+    rows, m = tr.shared["sh0"], tr.model
+    tr.blend_weights(cam, torch.zeros(500, device="cuda"))
+    assert torch.equal(m.params["sh0"].view(500, -1), rows.table[rows.index.long()] * 0.5)
+    rows.table.add_(1.0)
+    tr.keep_budget(torch.arange(500, device="cuda").float(), 100)
+    assert torch.equal(m.params["sh0"].view(100, -1), rows.table[rows.index.long()] * 0.5)
+
 
 def test_refusals(cuda_device):
     tr, cam, target = _trainer(n=200)
@@ -121,6 +130,7 @@ def test_refusals(cuda_device):
         Trainer(m, W, H, shared={"sh2": rows})
     assert e.value.code == gb.NOT_SUPPORTED
     for call in (lambda: tr.keep_budget(torch.zeros(199, device="cuda"), 10), lambda: tr.keep_budget(torch.zeros(200, device="cuda"), 0),
+                 lambda: tr.keep_budget(torch.zeros(200, device="cuda", dtype=torch.float16), 10),
                  lambda: tr.keep_budget(torch.zeros(200, device="cuda"), 10, first=6, recent=5)):
         with pytest.raises(gb.GsxError) as e:
             call()
