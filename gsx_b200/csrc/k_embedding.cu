@@ -1,22 +1,26 @@
 /*
  * Shared rows: out[n] = scale * table[index[n]], and the gradient of the table.
  *
- * The gradient grad_table[v] = scale * sum of grad_out[n] over the n with index[n] = v is summed in the order of
- * the positions n, grouped by row: a stable counting sort of the positions by row, then one sum per row.  No
- * floating-point atomics: the same inputs give the same bits.
+ * Lookup.  It reads the indices and the table's rows (mostly from L2) and writes out; what bounds it is the writing of
+ * out and, for rows that are no whole number of packs, the instructions an element.  Three forms, by the row: packs of
+ * 16, 8 or 4 bytes; up to four elements (a thread makes whole rows, small tables lie in shared memory); any other (lanes
+ * side by side on a row's elements).
  *
- *   sort    count <= kSmallCount: one CTA sorts (row, position) in shared memory by 8-bit digits.
- *           else, per digit of at most 12 bits: per-chunk digit counts, an exclusive scan over (digit, chunk), a
- *           scatter in which every warp ranks its own part of the chunk (__match_any_sync).  Tables of up to 4096
- *           rows need one pass.  Positions whose index is the padding row or out of range are dropped in the
- *           first pass.
- *   pieces  the sorted order is cut into pieces of kPiece positions; a piece that lies in one row is summed by a
- *           CTA of its own, so that a row which holds most of the positions is spread over the whole GPU.
- *   rows    a warp sums each row of up to kWarpMax positions, a CTA each longer one (its pieces' sums and the raw
- *           positions before and after them), scales, rounds once and stores.  Rows without positions get zeros.
+ * Gradient.  grad_table[v] = scale * sum of grad_out[n] over the n with index[n] = v, summed in the order of n, grouped
+ * by row.  No floating-point atomics: the same inputs give the same bits.
+ *   sort    a stable sort of (row, position) by the row's bits, in digits of at most 8.  Up to kSmallCount positions: one
+ *           CTA, in shared memory, while other CTAs write the table's zeros.  More: per digit the counts of 148 chunks,
+ *           then a scatter in which every CTA adds up the chunks' counts itself and ranks its chunk in tiles.  Positions
+ *           whose index is the padding row or out of range are dropped in the first pass.
+ *   sums    every CTA takes as many sorted positions as the others, whatever their rows: rows of any popularity cost the
+ *           same (a warp for each row took 3 to 4 times as long on skewed indices).  Groups of lanes walk runs of
+ *           positions with the gradients of the next ones in flight; rows that cross runs or CTAs are joined in order.
+ *   small tables of up to four columns with many positions skip the sort as a whole (own_table_kernel).
+ * The kernels of a call are launched so that each starts while the one before ends (gsx_launch_pdl).
  *
- * Sums are held in 32 bits: a row is split over the lanes that share its columns, then warps, then pieces, so no
- * chain of additions is longer than kPiece / 8 = 64 positions plus one term a piece.
+ * Sums are held in 32 bits.  No chain of additions is longer than a run (128 positions), plus one term for every group
+ * of a CTA (64) and an eighth of the CTAs that a row crosses; in the tables in shared memory a chain has the chunk's
+ * positions of the row, plus one term for every 37 chunks and eight of those.
  */
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -582,7 +586,7 @@ __global__ void __launch_bounds__(kSmallThreads) small_sort_kernel(const I *__re
         if(valid[it]) pairs[wbase + (uint32_t)it * 32u] = make_uint2(k[it], p[it]);
 }
 
-/* the table's zeros, beside small_sort_kernel; the last CTA ends after that */
+/* the table's zeros, beside small_sort_kernel; the last CTA ends after that.  268 MB: 39 us, 6.9 TB/s */
 __global__ void __launch_bounds__(kThreads) zero_kernel(const Table table, uint32_t dim)
 {
     gsx_pdl_trigger();
@@ -738,6 +742,9 @@ __global__ void __launch_bounds__(kSortThreads) digit_scatter_kernel(const I *__
 
 /* ------------------------------------------------------------------------------------------ */
 /* sums of sorted positions by row
+ *
+ * 1M x 45 f32 into 16384 rows: 57 us for 243 MB (a row of 180 bytes touches 64-byte pieces that it shares with its
+ * neighbours) in random order, 0.52 of the DRAM's peak, bound by the latency of the gathers; 40 more for the sort.
  *
  * A CTA owns R consecutive sorted positions.  A group of 2^clog lanes, each with NR packs of VW columns, walks a run
  * of C of them in order, with the rows of the next positions in flight, and stores a row whenever the row number
@@ -960,6 +967,7 @@ __global__ void __launch_bounds__(kThreads) row_join_kernel(const Runs a, const 
 
 /* ------------------------------------------------------------------------------------------ */
 /* Small tables of short rows (a codebook of colours) and many positions: the positions need not be sorted as a whole.
+ * 3M x 3 f32 into 4096 rows: 60 us, bound by latency (two CTAs an SM, 0.31 of the issue slots; the data alone takes 7).
  * A CTA keeps a table of sums in shared memory and walks a chunk of the positions in tiles: it ranks a tile by the low
  * 8 bits of the row, and thread t adds up the positions of the rows that end in t, in order.  The CTAs' tables are then
  * added up in the order of the chunks.  Lists of more than kOwnLong positions are walked by a warp, 32 at a time. */
