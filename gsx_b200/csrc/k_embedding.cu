@@ -597,10 +597,18 @@ __global__ void __launch_bounds__(kThreads) zero_kernel(const Table table, uint3
 /* The kernels from here on are launched before the one ahead of them has ended (gsx_launch_pdl) and read what it wrote
  * after gsx_pdl_wait: with __ldcg, since a read-only load may return what the SM's cache held before. */
 
+/* The table's zeros, written beside the sort: each of its kernels has CTAs behind those of its chunks that write the part of
+ * that kernel, while the others wait for counts and ranks (30000 positions into 67 MB: 311 us with the zeros in the four CTAs
+ * of the first count, 35 so). */
+struct Zeros {
+    Table table;
+    uint32_t dim, ctas, first, parts; /* parts of the table: CTAs of this kernel, the first one's part, all parts */
+};
+
 /* the part of a pass's input that belongs to this CTA */
-__device__ __forceinline__ void chunk_range(uint32_t n, uint32_t &begin, uint32_t &end)
+__device__ __forceinline__ void chunk_range(uint32_t n, uint32_t chunks, uint32_t &begin, uint32_t &end)
 {
-    const uint32_t len = (n + gridDim.x - 1) / gridDim.x;
+    const uint32_t len = (n + chunks - 1) / chunks;
     begin = len * blockIdx.x < n ? len * blockIdx.x : n;
     end = n - begin < len ? n : begin + len;
 }
@@ -641,22 +649,26 @@ __device__ __forceinline__ void load_elements(const I *__restrict__ index, const
     }
 }
 
-/* counts[c][d] = elements of chunk c with digit d; the first pass also writes the table's zeros */
+/* counts[c][d] = elements of chunk c with digit d */
 template <typename I, bool kFirst>
 __global__ void __launch_bounds__(kSortThreads) digit_count_kernel(const I *__restrict__ index,
                                                                    const uint2 *__restrict__ pairs, uint32_t count,
                                                                    const uint32_t *__restrict__ n_pairs, const Use use,
-                                                                   int shift, int bits, uint32_t *__restrict__ counts,
-                                                                   const Table table, uint32_t dim)
+                                                                   int shift, int bits, uint32_t chunks,
+                                                                   uint32_t *__restrict__ counts, const Zeros zeros)
 {
     __shared__ uint32_t s_hist[kHistRow];
     const uint32_t bins = 1u << bits;
     for(uint32_t j = threadIdx.x; j <= bins; j += kSortThreads) s_hist[j] = 0u;
     __syncthreads();
     gsx_pdl_trigger();
+    if(blockIdx.x >= chunks) {
+        zero_rows(zeros.table, zeros.dim, zeros.first + blockIdx.x - chunks, zeros.parts);
+        return;
+    }
     if(!kFirst) gsx_pdl_wait();
     uint32_t begin, end;
-    chunk_range(kFirst ? count : __ldcg(n_pairs), begin, end);
+    chunk_range(kFirst ? count : __ldcg(n_pairs), chunks, begin, end);
     for(uint32_t i0 = begin; i0 < end; i0 += kTile) {
         uint32_t key[kSortItems], pos[kSortItems];
         bool in[kSortItems];
@@ -666,8 +678,8 @@ __global__ void __launch_bounds__(kSortThreads) digit_count_kernel(const I *__re
             atomicAdd(&s_hist[in[it] ? key[it] >> shift & (bins - 1u) : bins], 1u);
     }
     __syncthreads();
-    for(uint32_t j = threadIdx.x; j < bins; j += kSortThreads) counts[blockIdx.x * bins + j] = s_hist[j];
-    if(kFirst && !table.accumulate) zero_rows(table, dim, blockIdx.x, gridDim.x);
+    const uint32_t padded = bins < 4 ? 4 : bins; /* read four at a time */
+    for(uint32_t j = threadIdx.x; j < padded; j += kSortThreads) counts[blockIdx.x * padded + j] = j < bins ? s_hist[j] : 0u;
 }
 
 /* every pair to its place, in input order within a digit.  Each CTA adds up the counts of all chunks itself. */
@@ -675,8 +687,9 @@ template <typename I, bool kFirst>
 __global__ void __launch_bounds__(kSortThreads) digit_scatter_kernel(const I *__restrict__ index,
                                                                         const uint2 *__restrict__ pairs, uint32_t count,
                                                                         uint32_t *n_pairs, const Use use, int shift,
-                                                                        int bits, const uint32_t *__restrict__ counts,
-                                                                        uint2 *__restrict__ out)
+                                                                        int bits, uint32_t chunks,
+                                                                        const uint32_t *__restrict__ counts,
+                                                                        uint2 *__restrict__ out, const Zeros zeros)
 {
     extern __shared__ __align__(16) unsigned char smem[];
     auto &s = *reinterpret_cast<SortShared<kSortThreads, kSortItems> *>(smem);
@@ -686,9 +699,13 @@ __global__ void __launch_bounds__(kSortThreads) digit_scatter_kernel(const I *__
     const uint32_t bins = 1u << bits, mask = bins - 1u;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     gsx_pdl_trigger();
+    if(blockIdx.x >= chunks) {
+        zero_rows(zeros.table, zeros.dim, zeros.first + blockIdx.x - chunks, zeros.parts);
+        return;
+    }
     gsx_pdl_wait();
     uint32_t begin, end;
-    chunk_range(kFirst ? count : __ldcg(n_pairs), begin, end);
+    chunk_range(kFirst ? count : __ldcg(n_pairs), chunks, begin, end);
     uint32_t k[kSortItems], p[kSortItems];
     bool valid[kSortItems];
     auto load = [&](uint32_t i0) {
@@ -698,23 +715,30 @@ __global__ void __launch_bounds__(kSortThreads) digit_scatter_kernel(const I *__
     };
     int items = begin < end ? load(begin) : 0; /* on their way while the counts are added up */
     {
-        const uint32_t d = threadIdx.x & mask, parts = kSortThreads >> bits;
-        uint32_t all = 0, before = 0;
-#pragma unroll 16
-        for(uint32_t c = threadIdx.x >> bits; c < gridDim.x; c += parts) {
-            const uint32_t v = __ldcg(counts + (c * bins + d));
-            all += v;
-            before += c < blockIdx.x ? v : 0u;
+        /* four digits a thread, up to 32 chunks side by side: a load for each five of 148 chunks where one digit a thread
+         * took 37 (the sort of 1M positions by 14 bits: 38 us, then 33) */
+        const uint32_t quads = (bins + 3) / 4, q = threadIdx.x % quads, lanes = kSortThreads / quads;
+        const uint32_t parts = lanes < 32 ? lanes : 32, part = threadIdx.x / quads;
+        uint4 all4 = make_uint4(0, 0, 0, 0), before4 = all4;
+        if(part < parts) {
+#pragma unroll 5
+            for(uint32_t c = part; c < chunks; c += parts) {
+                const uint4 v = __ldcg(reinterpret_cast<const uint4 *>(counts) + (c * quads + q));
+                const uint32_t m = c < blockIdx.x ? ~0u : 0u;
+                all4 = make_uint4(all4.x + v.x, all4.y + v.y, all4.z + v.z, all4.w + v.w);
+                before4 = make_uint4(before4.x + (v.x & m), before4.y + (v.y & m), before4.z + (v.z & m), before4.w + (v.w & m));
+            }
         }
-        uint32_t *s_all = &s.hist[0][0], *s_before = s_all + kSortThreads; /* of kSortThreads each */
-        s_all[threadIdx.x] = all;
-        s_before[threadIdx.x] = before;
+        uint4 *s_all = reinterpret_cast<uint4 *>(s.pair), *s_before = s_all + kSortThreads; /* of kSortThreads each */
+        s_all[threadIdx.x] = all4;
+        s_before[threadIdx.x] = before4;
         __syncthreads();
-        all = before = 0;
+        uint32_t all = 0, before = 0;
         if(threadIdx.x < bins)
-            for(uint32_t q = 0; q < parts; ++q) {
-                all += s_all[(q << bits) + d];
-                before += s_before[(q << bits) + d];
+#pragma unroll 8
+            for(uint32_t p = 0; p < parts; ++p) {
+                all += reinterpret_cast<const uint32_t *>(s_all + p * quads)[threadIdx.x];
+                before += reinterpret_cast<const uint32_t *>(s_before + p * quads)[threadIdx.x];
             }
         uint32_t n;
         const uint32_t smaller = block_inclusive_scan(all, s.warp, &n) - all;
@@ -995,7 +1019,7 @@ __global__ void __launch_bounds__(kOwnThreads, 2) own_table_kernel(const GT *__r
     for(uint32_t j = threadIdx.x; j < size; j += kOwnThreads) table[j] = 0.0f;
     const unsigned char *bytes = reinterpret_cast<const unsigned char *>(grad);
     uint32_t begin, end;
-    chunk_range(count, begin, end);
+    chunk_range(count, gridDim.x, begin, end);
     for(uint32_t i0 = begin; i0 < end; i0 += kOwnTile) {
         const int items = end - i0 >= kOwnTile ? kOwnItems : (int)((end - i0 + kOwnThreads - 1) / kOwnThreads);
         uint32_t k[kOwnItems], p[kOwnItems];
@@ -1166,7 +1190,8 @@ Plan make_plan(uint64_t count, uint64_t rows, uint64_t dim, uint64_t vec)
             p.bits[i] = (bits + p.passes - 1 - i) / (p.passes - i);
             bits -= p.bits[i];
         }
-        const uint64_t chunks = (count + kTile - 1) / kTile;
+        /* an element a thread before a second CTA idles: 10659 positions in 11 chunks, not in two */
+        const uint64_t chunks = (count + kSortThreads - 1) / kSortThreads;
         p.chunks = (uint32_t)(chunks < (uint64_t)kChunks ? chunks : kChunks);
         p.o_counts = o;
         o += align256(sizeof(uint32_t) * p.chunks * kMaxBins);
@@ -1186,23 +1211,23 @@ Plan make_plan(uint64_t count, uint64_t rows, uint64_t dim, uint64_t vec)
 
 template <typename I, bool kFirst>
 cudaError_t launch_pass(const I *index, const uint2 *pairs, uint32_t count, uint32_t *n_sorted, const Use &use, int shift,
-                        int bits, uint32_t chunks, uint32_t *counts, uint2 *out, const Table &table, uint32_t dim,
-                        cudaStream_t stream)
+                        int bits, uint32_t chunks, uint32_t *counts, uint2 *out, Zeros zeros, cudaStream_t stream)
 {
     constexpr size_t smem = sizeof(SortShared<kSortThreads, kSortItems>);
     cudaError_t e = gsx_allow_smem<digit_scatter_kernel<I, kFirst>>(smem);
     if(e != cudaSuccess) return e;
     if(kFirst)
-        digit_count_kernel<I, true><<<chunks, kSortThreads, 0, stream>>>(index, pairs, count, n_sorted, use, shift, bits,
-                                                                         counts, table, dim);
+        digit_count_kernel<I, true><<<chunks + zeros.ctas, kSortThreads, 0, stream>>>(index, pairs, count, n_sorted, use, shift,
+                                                                                      bits, chunks, counts, zeros);
     else
-        e = gsx_launch_pdl(digit_count_kernel<I, false>, dim3(chunks), dim3(kSortThreads), 0, stream, index, pairs, count,
-                           n_sorted, use, shift, bits, counts, table, dim);
+        e = gsx_launch_pdl(digit_count_kernel<I, false>, dim3(chunks + zeros.ctas), dim3(kSortThreads), 0, stream, index, pairs,
+                           count, n_sorted, use, shift, bits, chunks, counts, zeros);
     Use quiet = use; /* indices are reported once, by the count */
     quiet.bad = nullptr;
+    zeros.first += zeros.ctas;
     if(e == cudaSuccess)
-        e = gsx_launch_pdl(digit_scatter_kernel<I, kFirst>, dim3(chunks), dim3(kSortThreads), smem, stream, index, pairs, count,
-                           n_sorted, quiet, shift, bits, counts, out);
+        e = gsx_launch_pdl(digit_scatter_kernel<I, kFirst>, dim3(chunks + zeros.ctas), dim3(kSortThreads), smem, stream, index,
+                           pairs, count, n_sorted, quiet, shift, bits, chunks, counts, out, zeros);
     return e;
 }
 
@@ -1229,12 +1254,20 @@ cudaError_t launch_sort(const Plan &plan, unsigned char *ws, const void *index_,
         return e;
     }
     uint32_t *counts = reinterpret_cast<uint32_t *>(ws + plan.o_counts);
+    Zeros zeros = { table, dim, 0, 0, 0 };
+    if(!table.accumulate) { /* 64 KB a CTA, an equal part of them in each of the kernels */
+        const uint32_t kernels = 2u * (uint32_t)plan.passes;
+        const uint64_t ctas = (table.rows * dim * table.bytes + 65535) / 65536 / kernels + 1;
+        zeros.ctas = (uint32_t)(ctas < (1u << 24) ? ctas : 1u << 24);
+        zeros.parts = zeros.ctas * kernels;
+    }
     for(int p = 0, shift = 0; p < plan.passes; shift += plan.bits[p], ++p) {
         uint2 *to = pairs[p & 1];
         const cudaError_t e = p == 0 ? launch_pass<I, true>(index, nullptr, count, n_sorted, use, shift, plan.bits[p],
-                                                            plan.chunks, counts, to, table, dim, stream)
+                                                            plan.chunks, counts, to, zeros, stream)
                                      : launch_pass<I, false>(index, pairs[(p - 1) & 1], count, n_sorted, use, shift, plan.bits[p],
-                                                             plan.chunks, counts, to, table, dim, stream);
+                                                             plan.chunks, counts, to, zeros, stream);
+        zeros.first += 2 * zeros.ctas;
         if(e != cudaSuccess) return e;
         *out_pairs = to;
     }
