@@ -81,16 +81,43 @@ __device__ __forceinline__ void add_rows(float (&acc)[VW], const T *__restrict__
  * (r / RG) mod clusters, thread row r mod RG.  A thread keeps U rows in flight; the RG threads of a column are joined in
  * shared memory, the CTAs in distributed shared memory, each in a fixed order.  SPREAD, for rows that no 4-byte access
  * fits: a thread's VW columns lie CT apart, so that the lanes' single elements stay side by side. */
+/* VW consecutive floats in accesses of up to 16 bytes */
+template <int VW>
+__device__ __forceinline__ void load_floats(float (&x)[VW], const float *from)
+{
+    constexpr int P = VW < 4 ? VW : 4;
+#pragma unroll
+    for(int q = 0; q < VW / P; ++q) {
+        const Pack<float, P> y = reinterpret_cast<const Pack<float, P> *>(from)[q];
+#pragma unroll
+        for(int v = 0; v < P; ++v) x[q * P + v] = y.v[v];
+    }
+}
+
+template <int VW>
+__device__ __forceinline__ void store_floats(float *to, const float (&x)[VW])
+{
+    constexpr int P = VW < 4 ? VW : 4;
+#pragma unroll
+    for(int q = 0; q < VW / P; ++q) {
+        Pack<float, P> y;
+#pragma unroll
+        for(int v = 0; v < P; ++v) y.v[v] = x[q * P + v];
+        reinterpret_cast<Pack<float, P> *>(to)[q] = y;
+    }
+}
+
 template <typename T, int VW, int RG, bool SPREAD>
 __global__ void __launch_bounds__(kThreads, kAccumulateCtas) accumulate_kernel(const float *score, uint64_t score_stride,
                                                               const T *__restrict__ weights, uint64_t group_stride,
                                                               uint64_t row_stride, uint32_t groups, uint32_t rows,
                                                               uint32_t length, const int32_t *__restrict__ lengths,
                                                               const int32_t *__restrict__ row_lengths, float decay,
-                                                              float *out, uint64_t out_stride)
+                                                              float *out, uint64_t out_stride, bool wide_scores)
 {
     constexpr int CT = kThreads / RG;
     constexpr int U = 8;
+    constexpr bool kEarly = RG == 1; /* few rows: their scores are loaded before them */
     __shared__ float s_part[RG * CT * VW];
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t splits = cluster.num_blocks(), split = cluster.block_rank();
@@ -100,7 +127,11 @@ __global__ void __launch_bounds__(kThreads, kAccumulateCtas) accumulate_kernel(c
     for(uint32_t g = blockIdx.y; g < groups; g += gridDim.y) {
         const uint32_t n = length_of(lengths, g, length);
         const uint32_t nr = length_of(row_lengths, g, rows);
-        float acc[VW] = {};
+        float acc[VW] = {}, before[VW] = {};
+        const float *in = score + (uint64_t)g * score_stride;
+        float *to = out + (uint64_t)g * out_stride;
+        const bool wide = !SPREAD && wide_scores && j < n && n - j >= VW;
+        if(kEarly && wide && split == 0 && decay != 0.0f) load_floats<VW>(before, in + j);
         if(j < n) {
             uint32_t apart[VW]; /* columns that are not in use are read in the place of the last */
 #pragma unroll
@@ -147,8 +178,14 @@ __global__ void __launch_bounds__(kThreads, kAccumulateCtas) accumulate_kernel(c
             cluster.sync();
         }
         if(split != 0 || rg != 0) continue;
-        const float *in = score + (uint64_t)g * score_stride;
-        float *to = out + (uint64_t)g * out_stride;
+        if(wide) { /* 8 x 3M f16: 14 us, with scores one at a time 23 */
+            if(!kEarly && decay != 0.0f) load_floats<VW>(before, in + j);
+            if(decay != 0.0f)
+#pragma unroll
+                for(int v = 0; v < VW; ++v) acc[v] = fmaf(decay, before[v], acc[v]);
+            store_floats<VW>(to + j, acc);
+            continue;
+        }
 #pragma unroll
         for(int v = 0; v < VW; ++v) {
             const uint32_t c = SPREAD ? j + v * CT : j + v;
@@ -158,17 +195,98 @@ __global__ void __launch_bounds__(kThreads, kAccumulateCtas) accumulate_kernel(c
     }
 }
 
-template <typename T, int VW, int RG, bool SPREAD>
-cudaError_t launch_accumulate_rg(const float *score, uint64_t score_stride, const T *weights, uint64_t group_stride,
-                                 uint64_t row_stride, uint32_t groups, uint32_t rows, uint32_t length,
-                                 const int32_t *lengths, const int32_t *row_lengths, float decay, float *out,
-                                 uint64_t out_stride, cudaStream_t stream)
+/* Many rows that start at any element.  Rows a multiple of VW apart start at the same place of a 16-byte block, so with VW
+ * thread rows every thread's rows do: it reads whole blocks, shift elements left of the CTA's columns, and the shift is
+ * taken out where the thread rows are joined.  Of the CT * VW columns that the threads read, a CTA owns VW fewer.  A block
+ * that reaches over the first or the last element of the weights is read by element.  8 x 2048 x 8191 bf16: 44 us, with
+ * two-byte loads 73; with few rows the join costs more than it saves (8 x 3M f16 odd: 52 us, by element 25). */
+template <typename T>
+__global__ void __launch_bounds__(kThreads, kAccumulateCtas) accumulate_shifted_kernel(
+    const float *score, uint64_t score_stride, const T *__restrict__ weights, uint64_t group_stride, uint64_t row_stride,
+    uint32_t groups, uint32_t rows, uint32_t length, const int32_t *__restrict__ lengths,
+    const int32_t *__restrict__ row_lengths, float decay, float *out, uint64_t out_stride)
 {
-    constexpr uint32_t cols = kThreads / RG * VW;
+    constexpr int VW = 16 / sizeof(T), RG = VW, CT = kThreads / RG, U = 8, OWN = (CT - 1) * VW;
+    __shared__ __align__(16) float s_part[RG][CT * VW];
+    __shared__ float s_sum[OWN];
+    __shared__ uint32_t s_shift[RG];
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t splits = cluster.num_blocks(), split = cluster.block_rank();
+    const int ct = threadIdx.x % CT, rg = threadIdx.x / CT;
+    const uint32_t step = RG * splits, c0 = blockIdx.x / splits * (uint32_t)OWN, row0 = split * RG + (uint32_t)rg;
+    for(uint32_t g = blockIdx.y; g < groups; g += gridDim.y) {
+        const uint32_t n = length_of(lengths, g, length);
+        const uint32_t nr = length_of(row_lengths, g, rows);
+        const T *w = weights + (uint64_t)g * group_stride + (uint64_t)row0 * row_stride + c0;
+        const uint32_t shift = (uint32_t)((uintptr_t)w % 16) / (uint32_t)sizeof(T);
+        const int64_t col = (int64_t)c0 + ct * VW - (int64_t)shift; /* of the thread's block: its first column, may be below 0 */
+        w = w + ct * VW - shift;
+        float acc[VW] = {};
+        if(col < (int64_t)n) {
+            const uint64_t hop = (uint64_t)step * row_stride;
+            int left = nr > row0 ? (int)((nr - row0 + step - 1) / step) : 0;
+            auto by_element = [&]() {
+#pragma unroll
+                for(int v = 0; v < VW; ++v)
+                    if(col + v >= 0 && col + v < (int64_t)n) acc[v] += to_f32(w[v]);
+                w += hop;
+                --left;
+            };
+            if(left > 0 && col < 0 && g == 0 && row0 == 0) by_element();
+            const bool last = left > 0 && col + VW > (int64_t)length && g == groups - 1 && nr == rows && (rows - 1 - row0) % step == 0;
+            left -= last;
+            constexpr uint32_t apart[VW] = {};
+            for(; left >= U; left -= U, w += U * hop) add_rows<T, VW, U, false>(acc, w, hop, apart);
+            if(left >= 4) {
+                add_rows<T, VW, 4, false>(acc, w, hop, apart);
+                left -= 4;
+                w += 4 * hop;
+            }
+            if(left >= 2) {
+                add_rows<T, VW, 2, false>(acc, w, hop, apart);
+                left -= 2;
+                w += 2 * hop;
+            }
+            if(left > 0) {
+                add_rows<T, VW, 1, false>(acc, w, hop, apart);
+                w += hop;
+            }
+            if(last) by_element();
+        }
+        __syncthreads();
+        store_floats<VW>(&s_part[rg][ct * VW], acc);
+        if(ct == 0) s_shift[rg] = shift;
+        __syncthreads();
+        const uint32_t t = threadIdx.x;
+        float sum = 0.0f;
+        if(t < (uint32_t)OWN)
+#pragma unroll
+            for(int k = 0; k < RG; ++k) sum += s_part[k][t + s_shift[k]];
+        if(splits > 1) {
+            if(t < (uint32_t)OWN) s_sum[t] = sum;
+            cluster.sync();
+            if(split == 0 && t < (uint32_t)OWN)
+                for(uint32_t k = 1; k < splits; ++k) sum += cluster.map_shared_rank(s_sum, k)[t];
+            cluster.sync();
+        }
+        if(split != 0 || t >= (uint32_t)OWN) continue;
+        const float *in = score + (uint64_t)g * score_stride;
+        float *to = out + (uint64_t)g * out_stride;
+        const uint32_t c = c0 + t;
+        if(c < n) to[c] = decay == 0.0f ? sum : fmaf(decay, in[c], sum);
+        else if(c < length && to != in) to[c] = in[c];
+    }
+}
+
+/* `cols` columns and `row_threads` rows at a time a CTA */
+template <typename Kernel, typename... Args>
+cudaError_t launch_split(Kernel kernel, uint32_t cols, uint32_t row_threads, uint32_t groups, uint32_t rows, uint32_t length,
+                         cudaStream_t stream, Args... args)
+{
     const uint32_t blocks = (length + cols - 1) / cols, gy = groups < 65535u ? groups : 65535u;
     /* split the rows further while the GPU is not full and a split keeps at least two rows a thread */
     uint32_t splits = 1;
-    while(splits < 8 && (uint64_t)blocks * gy * splits * 2 <= 148 * kAccumulateCtas && rows >= splits * 2 * RG * 2) splits *= 2;
+    while(splits < 8 && (uint64_t)blocks * gy * splits * 2 <= 148 * kAccumulateCtas && rows >= splits * 2 * row_threads * 2) splits *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks * splits, gy);
     cfg.blockDim = dim3(kThreads);
@@ -180,8 +298,20 @@ cudaError_t launch_accumulate_rg(const float *score, uint64_t score_stride, cons
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, accumulate_kernel<T, VW, RG, SPREAD>, score, score_stride, weights, group_stride, row_stride,
-                              groups, rows, length, lengths, row_lengths, decay, out, out_stride);
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <typename T, int VW, int RG, bool SPREAD>
+cudaError_t launch_accumulate_rg(const float *score, uint64_t score_stride, const T *weights, uint64_t group_stride,
+                                 uint64_t row_stride, uint32_t groups, uint32_t rows, uint32_t length,
+                                 const int32_t *lengths, const int32_t *row_lengths, float decay, float *out,
+                                 uint64_t out_stride, cudaStream_t stream)
+{
+    /* scores and out in packs where all of a group's start at 16 bytes */
+    const bool wide = (((uintptr_t)score | (uintptr_t)out | (groups > 1 ? (score_stride | out_stride) * 4 : 0)) & 15) == 0;
+    return launch_split(accumulate_kernel<T, VW, RG, SPREAD>, kThreads / RG * VW, RG, groups, rows, length, stream, score,
+                        score_stride, weights, group_stride, row_stride, groups, rows, length, lengths, row_lengths, decay,
+                        out, out_stride, wide);
 }
 
 /* `unit`: the widest access in bytes (up to 16) that every row's start and the length are multiples of */
@@ -199,7 +329,14 @@ cudaError_t launch_accumulate(uint64_t unit, const float *score, uint64_t score_
     const bool many = rows >= 32;
     if(unit == 16) return many ? run(launch_accumulate_rg<T, W, 8, false>) : run(launch_accumulate_rg<T, W, 1, false>);
     if(unit == 8) return many ? run(launch_accumulate_rg<T, W / 2, 4, false>) : run(launch_accumulate_rg<T, W / 2, 1, false>);
-    if(unit == 4 && sizeof(T) == 2) return many ? run(launch_accumulate_rg<T, 2, 2, false>) : run(launch_accumulate_rg<T, 2, 1, false>);
+    /* the shifted form reads whole blocks between the first and the last element: rows of at least a block, none inside another */
+    const bool apart = length >= (uint32_t)W && (groups == 1 || (group_stride >= length && (group_stride >= (uint64_t)(rows - 1) * row_stride + length ||
+                                                                                      row_stride >= (uint64_t)(groups - 1) * group_stride + length)));
+    if(many && apart)
+        return launch_split(accumulate_shifted_kernel<T>, kThreads - W, W, groups, rows, length, stream, score, score_stride,
+                            static_cast<const T *>(weights), group_stride, row_stride, groups, rows, length, lengths, row_lengths,
+                            decay, out, out_stride);
+    if(unit == 4 && sizeof(T) == 2 && !many) return run(launch_accumulate_rg<T, 2, 1, false>);
     if(many) return run(launch_accumulate_rg<T, 4, 4, true>);
     /* four columns a thread where that still fills the GPU, else one */
     if((uint64_t)groups * ((length + kThreads * 4 - 1) / (kThreads * 4)) >= 148 * kAccumulateCtas) return run(launch_accumulate_rg<T, 4, 1, true>);

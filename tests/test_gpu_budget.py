@@ -83,6 +83,49 @@ def test_accumulate_strided_and_unaligned(cuda_device):
     assert out is one
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("groups,rows,length", [(1, 32, 8), (3, 33, 7), (2, 40, 9), (5, 71, 247), (2, 64, 249), (1, 600, 1003), (2, 300, 251),
+                                                (2, 37, 2050), (40, 35, 501)])
+def test_accumulate_many_rows_that_start_anywhere(cuda_device, groups, rows, length, dtype):
+    """Odd lengths, starts at every element of a 16-byte block, rows next to one another or apart, groups inside rows,
+    and lengths that end inside a block; what lies outside the weights is NaN."""
+    g = _gen(rows + length)
+    score = torch.rand(groups, length, generator=g, device="cuda")
+    lengths = torch.randint(0, length + 1, (groups,), generator=g, device="cuda", dtype=torch.int32)
+    row_lengths = torch.randint(0, rows + 1, (groups,), generator=g, device="cuda", dtype=torch.int32)
+    for start in (0, 1, 3, 6):
+        for pad in (0, 1, 5):
+            for inside in (False, True):
+                shape = (rows, groups, length + pad) if inside else (groups, rows, length + pad)
+                count = shape[0] * shape[1] * shape[2]
+                buf = torch.full((start + count + 9,), float("nan"), device="cuda", dtype=dtype)
+                w = buf[start:start + count].view(shape)[..., :length]
+                w = w.transpose(0, 1) if inside else w
+                w.copy_(torch.rand(groups, rows, length, generator=g, device="cuda"))
+                out = gb.budget_accumulate(score, w, out=torch.empty_like(score), decay=0.5)
+                _check_accumulate(out, score, w, 0.5)
+                out = gb.budget_accumulate(score, w, out=torch.empty_like(score), decay=0.5, lengths=lengths, row_lengths=row_lengths)
+                _check_accumulate(out, score, w, 0.5, lengths, row_lengths)
+    alike = w[:1, :, :].expand(groups, rows, length)  # the same weights for all groups
+    out = gb.budget_accumulate(score, alike, out=torch.empty_like(score), decay=0.5)
+    _check_accumulate(out, score, alike, 0.5)
+
+
+def test_accumulate_scores_at_every_alignment(cuda_device):
+    g = _gen(9)
+    for dtype in (F32, F16):
+        for rows in (3, 40):
+            w = torch.rand(3, rows, 64, generator=g, device="cuda").to(dtype)
+            for a, b, step in [(0, 0, 64), (1, 0, 64), (0, 2, 64), (4, 4, 68), (0, 0, 65), (8, 3, 72)]:
+                score = torch.rand(300, generator=g, device="cuda")[a:a + 3 * step].view(3, step)[:, :64]
+                out = torch.full((300,), 7.0, device="cuda")
+                to = out[b:b + 3 * step].view(3, step)[:, :64]
+                gb.budget_accumulate(score, w, out=to, decay=0.25)
+                _check_accumulate(to, score, w, 0.25)
+                to.fill_(7.0)
+                assert bool((out == 7.0).all())
+
+
 def test_accumulate_offsets_behind_32_bits(cuda_device):
     """Weights of more than 2^32 elements (8.6 GB): the last group's rows are read from their own place."""
     G, R, L = 3, 1500, 1_000_000
