@@ -8,8 +8,8 @@
  *
  * Gradient.  grad_table[v] = scale * sum of grad_out[n] over the n with index[n] = v, summed in the order of n, grouped
  * by row.  No floating-point atomics: the same inputs give the same bits.
- *   sort    a stable sort of (row, position) by the row's bits, in digits of at most 8.  Up to kSmallCount positions: one
- *           CTA, in shared memory, while other CTAs write the table's zeros.  More: per digit the counts of 148 chunks,
+ *   sort    a stable sort of (row, position) by the row's bits, in digits of at most 8.  Up to small_count positions: one
+ *           CTA, in shared memory, while other CTAs write the table's zeros.  More: per digit the counts of up to 148 chunks,
  *           then a scatter in which every CTA adds up the chunks' counts itself and ranks its chunk in tiles.  Positions
  *           whose index is the padding row or out of range are dropped in the first pass.
  *   sums    every CTA takes as many sorted positions as the others, whatever their rows: rows of any popularity cost the
@@ -35,8 +35,16 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kSmallThreads = 1024;
-constexpr int kSmallItems = 8;
-constexpr int kSmallCount = kSmallThreads * kSmallItems; /* positions that one CTA sorts */
+/* Positions a thread that one CTA sorts.  Of 4000 and 8100 positions in 4650 rows the whole gradient takes 20 and 28 us so,
+ * 25 and 26 with the longer sort; a sort of all digits in one cluster of CTAs took 23 and 24.  Beside the zeros of a large
+ * table the one CTA costs nothing: 8191 positions and 268 MB take 57 us, with the longer sort, whose four launches end
+ * with their zeros, 67; 67 MB take 29 and 27. */
+constexpr int kSmallItems = 5, kBesideItems = 8;
+constexpr uint64_t kBesideTable = 1u << 25; /* elements */
+constexpr uint64_t small_count(uint64_t rows, uint64_t dim)
+{
+    return (uint64_t)kSmallThreads * (rows * dim > kBesideTable ? kBesideItems : kSmallItems);
+}
 constexpr int kSortThreads = 1024;
 constexpr int kSortItems = 8;
 constexpr int kTile = kSortThreads * kSortItems; /* pairs that a CTA of the longer sort ranks at once */
@@ -532,29 +540,29 @@ __device__ __forceinline__ uint32_t sort_tile(SortShared<THREADS, ITEMS> &s, con
 }
 
 /* all of a small sort in one CTA */
-template <typename I>
+template <typename I, int ITEMS>
 __global__ void __launch_bounds__(kSmallThreads) small_sort_kernel(const I *__restrict__ index, uint32_t count,
                                                                    const Use use, uint2 *__restrict__ pairs,
                                                                    uint32_t *__restrict__ n_sorted)
 {
     extern __shared__ __align__(16) unsigned char smem[];
-    auto &s = *reinterpret_cast<SortShared<kSmallThreads, kSmallItems> *>(smem);
+    auto &s = *reinterpret_cast<SortShared<kSmallThreads, ITEMS> *>(smem);
     gsx_pdl_trigger(); /* the zeros are written meanwhile */
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int items = (int)((count + kSmallThreads - 1) / kSmallThreads);
     const uint32_t wbase = (uint32_t)warp * 32u * (uint32_t)items + (uint32_t)lane;
-    uint32_t k[kSmallItems], p[kSmallItems], used = 0;
-    bool valid[kSmallItems];
-    I raw[kSmallItems];
+    uint32_t k[ITEMS], p[ITEMS], used = 0;
+    bool valid[ITEMS];
+    I raw[ITEMS];
 #pragma unroll
-    for(int it = 0; it < kSmallItems; ++it) {
+    for(int it = 0; it < ITEMS; ++it) {
         p[it] = wbase + (uint32_t)it * 32u;
         valid[it] = it < items && p[it] < count;
         raw[it] = count > 0 ? __ldg(index + (valid[it] ? p[it] : 0u)) : (I)0;
     }
     bool outside = false;
 #pragma unroll
-    for(int it = 0; it < kSmallItems; ++it) {
+    for(int it = 0; it < ITEMS; ++it) {
         valid[it] &= takes_part(valid[it] ? raw[it] : (I)0, use, outside);
         k[it] = valid[it] ? (uint32_t)raw[it] : 0u;
         used += valid[it];
@@ -570,7 +578,7 @@ __global__ void __launch_bounds__(kSmallThreads) small_sort_kernel(const I *__re
         sort_tile(s, k, p, valid, items, shift, width);
         shift += width;
 #pragma unroll
-        for(int it = 0; it < kSmallItems; ++it) {
+        for(int it = 0; it < ITEMS; ++it) {
             const uint32_t i = wbase + (uint32_t)it * 32u;
             valid[it] = it < items && i < n;
             if(it < items) {
@@ -582,7 +590,7 @@ __global__ void __launch_bounds__(kSmallThreads) small_sort_kernel(const I *__re
         __syncthreads();
     }
 #pragma unroll
-    for(int it = 0; it < kSmallItems; ++it)
+    for(int it = 0; it < ITEMS; ++it)
         if(valid[it]) pairs[wbase + (uint32_t)it * 32u] = make_uint2(k[it], p[it]);
 }
 
@@ -1182,7 +1190,7 @@ Plan make_plan(uint64_t count, uint64_t rows, uint64_t dim, uint64_t vec)
         p.bytes = o + sizeof(float) * p.own * rows * dim;
         return p;
     }
-    if(count > (uint64_t)kSmallCount) {
+    if(count > small_count(rows, dim)) {
         int bits = 1;
         while(bits < 32 && (rows - 1) >> bits) ++bits;
         p.passes = (bits + kMaxBits - 1) / kMaxBits;
@@ -1190,7 +1198,7 @@ Plan make_plan(uint64_t count, uint64_t rows, uint64_t dim, uint64_t vec)
             p.bits[i] = (bits + p.passes - 1 - i) / (p.passes - i);
             bits -= p.bits[i];
         }
-        /* an element a thread before a second CTA idles: 10659 positions in 11 chunks, not in two */
+        /* an element a thread first, then more of them: 10659 positions in 11 chunks, not in two */
         const uint64_t chunks = (count + kSortThreads - 1) / kSortThreads;
         p.chunks = (uint32_t)(chunks < (uint64_t)kChunks ? chunks : kChunks);
         p.o_counts = o;
@@ -1231,6 +1239,16 @@ cudaError_t launch_pass(const I *index, const uint2 *pairs, uint32_t count, uint
     return e;
 }
 
+template <typename I, int ITEMS>
+cudaError_t launch_small_sort(const I *index, uint32_t count, const Use &use, uint2 *pairs, uint32_t *n_sorted, cudaStream_t stream)
+{
+    constexpr size_t smem = sizeof(SortShared<kSmallThreads, ITEMS>);
+    const cudaError_t e = gsx_allow_smem<small_sort_kernel<I, ITEMS>>(smem);
+    if(e != cudaSuccess) return e;
+    small_sort_kernel<I, ITEMS><<<1, kSmallThreads, smem, stream>>>(index, count, use, pairs, n_sorted);
+    return cudaSuccess;
+}
+
 /* sorted pairs end up in *out_pairs; the table's rows are zero afterwards (unless it accumulates) */
 template <typename I>
 cudaError_t launch_sort(const Plan &plan, unsigned char *ws, const void *index_, uint32_t count, const Use &use,
@@ -1241,11 +1259,10 @@ cudaError_t launch_sort(const Plan &plan, unsigned char *ws, const void *index_,
     uint2 *pairs[2] = { reinterpret_cast<uint2 *>(ws + plan.o_pairs[0]), reinterpret_cast<uint2 *>(ws + plan.o_pairs[1]) };
     if(plan.passes == 0) {
         *out_pairs = pairs[0];
-        constexpr size_t smem = sizeof(SortShared<kSmallThreads, kSmallItems>);
-        cudaError_t e = gsx_allow_smem<small_sort_kernel<I>>(smem);
-        if(e != cudaSuccess) return e;
-        small_sort_kernel<I><<<1, kSmallThreads, smem, stream>>>(index, count, use, pairs[0], n_sorted);
-        if(!table.accumulate) {
+        cudaError_t e = count <= (uint32_t)(kSmallThreads * kSmallItems)
+                            ? launch_small_sort<I, kSmallItems>(index, count, use, pairs[0], n_sorted, stream)
+                            : launch_small_sort<I, kBesideItems>(index, count, use, pairs[0], n_sorted, stream);
+        if(e == cudaSuccess && !table.accumulate) {
             /* 16 KB of zeros a CTA: many short CTAs write 15% faster than one wave of long ones (6.9 against 6.0 TB/s) */
             const uint64_t ctas = (table.rows * dim * table.bytes + 16383) / 16384;
             e = gsx_launch_pdl(zero_kernel, dim3((unsigned)(ctas < (1u << 30) ? ctas : 1u << 30)), dim3(kThreads), 0, stream,

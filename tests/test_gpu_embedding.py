@@ -126,7 +126,7 @@ def _check_gradient(got, grad, index, rows, scale, before=None, drop=None):
         assert bool((got[(n == 0)[:, 0]] == 0).all())
 
 
-GRADIENT_SIZES = [(0, 5, 3), (1, 1, 1), (5, 1, 4), (100, 256, 8), (8192, 300, 7), (8193, 300, 7), (9000, 1, 3),
+GRADIENT_SIZES = [(0, 5, 3), (1, 1, 1), (5, 1, 4), (100, 256, 8), (8192, 300, 7), (8193, 300, 7), (5120, 70_000, 7), (5121, 70_000, 7), (148 * 1024 + 1, 300, 7), (30_000, 40_000, 130), (8192, 40_000, 900), (8193, 40_000, 900), (9000, 1, 3),
                   (20_000, 4096, 3), (20_000, 4097, 4), (50_000, 70_000, 2), (33_333, 5000, 45), (300, 1000, 2048),
                   (12_000, 3, 260), (2000, 50, 33), (200_001, 100, 1), (300_000, 1000, 2), (700_000, 4096, 3),
                   (150_000, 777, 4), (60_000, 1, 3), (700_001, 1000, 3), (1_300_000, 4096, 4),
