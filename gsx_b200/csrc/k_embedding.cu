@@ -463,22 +463,27 @@ __device__ __forceinline__ uint32_t block_inclusive_scan(uint32_t v, uint32_t *s
 
 /* A tile of (row, position) pairs that a CTA ranks by one digit of at most 8 bits. */
 constexpr int kHistRow = kMaxBins + 1; /* one more: elements that take no part */
-template <int THREADS, int ITEMS>
+template <int THREADS, int ITEMS, typename P = uint2>
 struct SortShared {
-    uint2 pair[THREADS * ITEMS];
     uint32_t hist[THREADS / 32][kHistRow];
     uint32_t before[kHistRow]; /* of a digit: the tile's pairs with smaller ones */
     uint32_t warp[32];
+    alignas(16) P pair[THREADS * ITEMS]; /* the last: a launch may leave room for the tile that it uses */
 };
 
+/* a pair in eight bytes, or in four: a position in a tile of at most 2^kPlaceBits */
+constexpr int kPlaceBits = 12;
+__device__ __forceinline__ void set_pair(uint2 &to, uint32_t key, uint32_t pos) { to = make_uint2(key, pos); }
+__device__ __forceinline__ void set_pair(uint32_t &to, uint32_t key, uint32_t pos) { to = key << kPlaceBits | pos; }
+
 /* Ranks the tile's pairs (warp w holds elements 32 * items * w + 32 * it + lane) by digit, stable in element
- * order, and leaves them in s.pair in that order, those with valid[it] false (their key is 0) behind the others.
+ * order, and leaves them in s.pair in that order, without those with valid[it] false (their key is 0).
  * Returns, for threads below the number of digits, how many pairs have that digit.  Lanes with equal digits find one
  * another by one ballot per digit bit: __match_any_sync takes a step per distinct value on this GPU (a tile of 8192
  * ranked in 12 us with it, in 4 us with ballots).  No step is under a condition of the element: elements that take
  * no part have a digit of their own (with branches a tile took 2.5 times as many instructions). */
-template <int THREADS, int ITEMS>
-__device__ __forceinline__ uint32_t sort_tile(SortShared<THREADS, ITEMS> &s, const uint32_t (&key)[ITEMS],
+template <int THREADS, int ITEMS, typename P>
+__device__ __forceinline__ uint32_t sort_tile(SortShared<THREADS, ITEMS, P> &s, const uint32_t (&key)[ITEMS],
                                               const uint32_t (&pos)[ITEMS], const bool (&valid)[ITEMS], int items, int shift,
                                               int bits)
 {
@@ -490,6 +495,7 @@ __device__ __forceinline__ uint32_t sort_tile(SortShared<THREADS, ITEMS> &s, con
     __syncthreads();
     uint32_t *wh = s.hist[warp];
     uint32_t rank[ITEMS], digit[ITEMS];
+    /* the ballots of all items first: they do not wait for one another, the counts do */
 #pragma unroll
     for(int it = 0; it < ITEMS; ++it) {
         if(it < items) {
@@ -504,10 +510,16 @@ __device__ __forceinline__ uint32_t sort_tile(SortShared<THREADS, ITEMS> &s, con
                 }
             }
             digit[it] = valid[it] ? d : bins;
+            rank[it] = (uint32_t)__popc(peers & ((1u << lane) - 1u)) | (uint32_t)__popc(peers) << 16; /* and the peers */
+        }
+    }
+#pragma unroll
+    for(int it = 0; it < ITEMS; ++it) {
+        if(it < items) {
             const uint32_t before = wh[digit[it]];
-            rank[it] = before + (uint32_t)__popc(peers & ((1u << lane) - 1u));
             __syncwarp();
-            wh[digit[it]] = before + (uint32_t)__popc(peers); /* the same from every lane of the digit */
+            wh[digit[it]] = before + (rank[it] >> 16); /* the same from every lane of the digit */
+            rank[it] = before + (rank[it] & 0xffffu);
             __syncwarp();
         }
     }
@@ -534,7 +546,7 @@ __device__ __forceinline__ uint32_t sort_tile(SortShared<THREADS, ITEMS> &s, con
     __syncthreads();
 #pragma unroll
     for(int it = 0; it < ITEMS; ++it)
-        if(it < items) s.pair[s.before[digit[it]] + wh[digit[it]] + rank[it]] = make_uint2(key[it], pos[it]);
+        if(it < items && valid[it]) set_pair(s.pair[s.before[digit[it]] + wh[digit[it]] + rank[it]], key[it], pos[it]);
     __syncthreads();
     return count;
 }
@@ -1004,91 +1016,141 @@ __global__ void __launch_bounds__(kThreads) row_join_kernel(const Runs a, const 
  * 8 bits of the row, and thread t adds up the positions of the rows that end in t, in order.  The CTAs' tables are then
  * added up in the order of the chunks.  Lists of more than kOwnLong positions are walked by a warp, 32 at a time. */
 constexpr int kOwnThreads = 256;
-constexpr int kOwnItems = 16;
+constexpr int kOwnItems = 16; /* positions a thread of a tile, at most */
 constexpr uint32_t kOwnTile = kOwnThreads * kOwnItems;
+static_assert(kOwnTile <= 1u << kPlaceBits, "a place of a tile fits a pair");
 constexpr uint64_t kOwnDim = 4, kOwnRows = 128;
-constexpr size_t kOwnTable = 68 * 1024; /* two CTAs an SM */
+constexpr size_t kOwnTable = 68 * 1024;
+static_assert(kOwnTable / 4 <= 1u << (32 - kPlaceBits), "a row fits a pair");
+constexpr size_t kOwnMemory = 113 * 1024; /* of a CTA: two an SM */
 constexpr uint32_t kOwnLong = 64;
-constexpr int kOwnCols = 4; /* columns of a walk */
 static_assert(kOwnThreads == kMaxBins, "thread t owns digit t");
+using OwnShared = SortShared<kOwnThreads, kOwnItems, uint32_t>;
 
-template <typename GT, typename I>
+/* positions of a tile: as many as fit beside the table, with their pairs and gradients, in tiles of equal length */
+uint32_t own_tile(uint32_t len, uint32_t rows, uint32_t dim, size_t gb)
+{
+    const size_t fixed = sizeof(OwnShared) - sizeof(uint32_t) * kOwnTile + 4 * (size_t)rows * dim;
+    const size_t fit = (kOwnMemory - fixed) / (sizeof(uint32_t) + dim * gb) / 32 * 32;
+    const uint32_t most = fit < kOwnTile ? (uint32_t)fit : kOwnTile, tiles = (len + most - 1) / most;
+    return ((len + tiles - 1) / tiles + 31) / 32 * 32;
+}
+
+/* whole multiples of 32 positions a chunk, so that tiles of dense rows start at 16 bytes */
+__host__ __device__ constexpr uint32_t own_length(uint32_t count, uint32_t chunks)
+{
+    return ((count + chunks - 1) / chunks + 31u) / 32u * 32u;
+}
+
+template <typename GT, typename I, int DIM>
 __global__ void __launch_bounds__(kOwnThreads, 2) own_table_kernel(const GT *__restrict__ grad, uint32_t stride_bytes,
                                                                    const I *__restrict__ index, uint32_t count, const Use use,
-                                                                   uint32_t dim, float *__restrict__ partial)
+                                                                   uint32_t tile, float *__restrict__ partial)
 {
-    using Shared = SortShared<kOwnThreads, kOwnItems>;
     extern __shared__ __align__(16) unsigned char smem[];
-    Shared &s = *reinterpret_cast<Shared *>(smem);
-    float *table = reinterpret_cast<float *>(smem + sizeof(Shared));
-    __shared__ uint32_t s_count[kOwnThreads];
+    OwnShared &s = *reinterpret_cast<OwnShared *>(smem);
+    const uint32_t size = use.rows * DIM;
+    GT *s_grad = reinterpret_cast<GT *>(smem + (sizeof(OwnShared) - sizeof(uint32_t) * (kOwnTile - tile)));
+    float *table = reinterpret_cast<float *>(s_grad + tile * DIM);
+    uint32_t *s_count = s.hist[0]; /* of a digit: its pairs; the histograms are done with by then */
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t size = use.rows * dim;
-    for(uint32_t j = threadIdx.x; j < size; j += kOwnThreads) table[j] = 0.0f;
     const unsigned char *bytes = reinterpret_cast<const unsigned char *>(grad);
-    uint32_t begin, end;
-    chunk_range(count, gridDim.x, begin, end);
-    for(uint32_t i0 = begin; i0 < end; i0 += kOwnTile) {
-        const int items = end - i0 >= kOwnTile ? kOwnItems : (int)((end - i0 + kOwnThreads - 1) / kOwnThreads);
+    const bool dense = stride_bytes == DIM * sizeof(GT) && (uintptr_t)grad % 16 == 0;
+    const uint32_t len = own_length(count, gridDim.x);
+    const uint32_t begin = len * blockIdx.x < count ? len * blockIdx.x : count, end = count - begin < len ? count : begin + len;
+    I raw[kOwnItems]; /* the indices of the next tile */
+    auto fetch = [&](uint32_t i0) {
+        const uint32_t here = end - i0 < tile ? end - i0 : tile, items = (here + kOwnThreads - 1) / kOwnThreads;
+#pragma unroll
+        for(uint32_t it = 0; it < kOwnItems; ++it) {
+            const uint32_t i = i0 + (uint32_t)warp * 32u * items + it * 32u + (uint32_t)lane;
+            raw[it] = __ldg(index + (it < items && i < end ? i : end - 1));
+        }
+    };
+    if(begin < end) fetch(begin);
+    for(uint32_t j = threadIdx.x; j < size; j += kOwnThreads) table[j] = 0.0f;
+    for(uint32_t i0 = begin; i0 < end; i0 += tile) {
+        const uint32_t here = end - i0 < tile ? end - i0 : tile;
+        const int items = (int)((here + kOwnThreads - 1) / kOwnThreads);
+        /* the tile's gradients, on their way while it is ranked, and the next one's as far as the L2 */
+        if(dense) {
+            const unsigned char *from = bytes + (uint64_t)i0 * (DIM * sizeof(GT));
+            unsigned char *to = reinterpret_cast<unsigned char *>(s_grad);
+            const uint32_t all = here * DIM * (uint32_t)sizeof(GT), whole = all / 16 * 16;
+#pragma unroll 4
+            for(uint32_t o = threadIdx.x * 16; o < whole; o += kOwnThreads * 16)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to + o)), "l"(from + o)
+                             : "memory");
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            const uint32_t o = whole + threadIdx.x * (uint32_t)sizeof(GT);
+            if(o < all) *reinterpret_cast<GT *>(to + o) = *reinterpret_cast<const GT *>(from + o);
+            const uint32_t rest = end - i0 - here, next = (rest < tile ? rest : tile) * DIM * (uint32_t)sizeof(GT) / 16 * 16;
+            if(threadIdx.x == 0 && next > 0)
+                asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from + all), "r"(next) : "memory");
+        } else {
+            for(uint32_t j = threadIdx.x; j < here * DIM; j += kOwnThreads)
+                s_grad[j] = reinterpret_cast<const GT *>(bytes + (uint64_t)(i0 + j / DIM) * stride_bytes)[j % DIM];
+        }
         uint32_t k[kOwnItems], p[kOwnItems];
-        bool valid[kOwnItems];
-        load_elements<I, true, kOwnItems>(index, nullptr, i0 + (uint32_t)(warp * 32 * items + lane), 32, items, end, use, k, p, valid);
-        s_count[threadIdx.x] = sort_tile(s, k, p, valid, items, 0, kMaxBits);
+        bool valid[kOwnItems], outside = false;
+#pragma unroll
+        for(int it = 0; it < kOwnItems; ++it) {
+            p[it] = (uint32_t)(warp * 32 * items + it * 32 + lane);
+            const bool in = it < items && p[it] < here;
+            valid[it] = takes_part(raw[it], use, outside) && in; /* those behind the end repeat the last index */
+            k[it] = valid[it] ? (uint32_t)raw[it] : 0u;
+        }
+        if(outside && use.bad != nullptr) atomicExch(use.bad, 1u);
+        const uint32_t n = sort_tile(s, k, p, valid, items, 0, kMaxBits);
+        s_count[threadIdx.x] = n;
+        if(i0 + here < end) fetch(i0 + here);
+        asm volatile("cp.async.wait_all;" ::: "memory");
         __syncthreads();
-        for(uint32_t c0 = 0; c0 < dim; c0 += kOwnCols) {
-            const uint32_t cols = dim - c0 < (uint32_t)kOwnCols ? dim - c0 : kOwnCols;
-            const GT *from[kOwnCols]; /* columns that are not there are read in the place of the first */
+        auto split = [&](uint32_t pair, float(&x)[DIM]) { /* its row in the table */
+            const GT *g = s_grad + (pair & ((1u << kPlaceBits) - 1u)) * DIM;
 #pragma unroll
-            for(int c = 0; c < kOwnCols; ++c) from[c] = reinterpret_cast<const GT *>(bytes) + c0 + ((uint32_t)c < cols ? c : 0);
-            auto load = [&](GT(&x)[kOwnCols], uint32_t pos) {
+            for(int c = 0; c < DIM; ++c) x[c] = to_f32(g[c]);
+            return table + (pair >> kPlaceBits) * DIM;
+        };
+        const uint32_t first = s.before[threadIdx.x];
+        if(n <= kOwnLong)
+            for(uint32_t j = 0; j < n; j += 4) {
+                float *to[4];
+                float x[4][DIM];
 #pragma unroll
-                for(int c = 0; c < kOwnCols; ++c)
-                    x[c] = *reinterpret_cast<const GT *>(reinterpret_cast<const unsigned char *>(from[c]) + (uint64_t)pos * stride_bytes);
-            };
-            const uint32_t first = s.before[threadIdx.x], n = s_count[threadIdx.x];
-            if(n <= kOwnLong)
-                for(uint32_t j = 0; j < n; j += 4) {
-                    uint2 kp[4];
-                    GT x[4][kOwnCols];
+                for(uint32_t u = 0; u < 4; ++u) to[u] = split(s.pair[first + (j + u < n ? j + u : n - 1)], x[u]);
 #pragma unroll
-                    for(uint32_t u = 0; u < 4; ++u) kp[u] = s.pair[first + (j + u < n ? j + u : n - 1)];
+                for(uint32_t u = 0; u < 4; ++u)
+                    if(j + u < n)
 #pragma unroll
-                    for(uint32_t u = 0; u < 4; ++u) load(x[u], kp[u].y);
+                        for(int c = 0; c < DIM; ++c) to[u][c] += x[u][c];
+            }
+        /* the long lists, dealt to the warps: the sums of a step's distinct rows one after another */
+        unsigned lists = __ballot_sync(0xffffffffu, s_count[lane * (kOwnThreads / 32) + warp] > kOwnLong);
+        for(; lists != 0u; lists &= lists - 1u) {
+            const int t = (__ffs(lists) - 1) * (kOwnThreads / 32) + warp;
+            const uint32_t m = s_count[t], at = s.before[t];
+            for(uint32_t j = 0; j < m; j += 32) {
+                const bool in = j + lane < m;
+                float x[DIM];
+                float *to = split(s.pair[at + (in ? j + lane : m - 1)], x);
+                const uint32_t place = (uint32_t)(to - table);
+                unsigned rest = __ballot_sync(0xffffffffu, in);
+                while(rest != 0u) {
+                    const uint32_t one = __shfl_sync(0xffffffffu, place, __ffs(rest) - 1);
+                    const bool mine = in && place == one;
+                    float sum = 0.0f; /* lane c: of column c */
 #pragma unroll
-                    for(uint32_t u = 0; u < 4; ++u)
-                        if(j + u < n) {
-                            float *to = table + kp[u].x * dim + c0;
+                    for(int c = 0; c < DIM; ++c) {
+                        float v = mine ? x[c] : 0.0f;
 #pragma unroll
-                            for(int c = 0; c < kOwnCols; ++c)
-                                if((uint32_t)c < cols) to[c] += to_f32(x[u][c]);
-                        }
-                }
-            /* the long lists, dealt to the warps: the sums of a step's distinct rows one after another */
-            for(int t = warp; t < kOwnThreads; t += kOwnThreads / 32) {
-                const uint32_t m = s_count[t], at = s.before[t];
-                if(m <= kOwnLong) continue;
-                for(uint32_t j = 0; j < m; j += 32) {
-                    const bool in = j + lane < m;
-                    const uint2 kp = s.pair[at + (in ? j + lane : m - 1)];
-                    GT x[kOwnCols];
-                    load(x, kp.y);
-                    unsigned rest = __ballot_sync(0xffffffffu, in);
-                    while(rest != 0u) {
-                        const uint32_t row = __shfl_sync(0xffffffffu, kp.x, __ffs(rest) - 1);
-                        const bool mine = in && kp.x == row;
-                        float v[kOwnCols];
-#pragma unroll
-                        for(int c = 0; c < kOwnCols; ++c) {
-                            v[c] = mine ? to_f32(x[c]) : 0.0f;
-#pragma unroll
-                            for(int o = 16; o > 0; o >>= 1) v[c] += __shfl_xor_sync(0xffffffffu, v[c], o);
-                        }
-                        if((uint32_t)lane < cols)
-                            table[row * dim + c0 + lane] += lane == 0 ? v[0] : lane == 1 ? v[1] : lane == 2 ? v[2] : v[3];
-                        rest &= ~__ballot_sync(0xffffffffu, mine);
+                        for(int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+                        sum = lane == c ? v : sum;
                     }
-                    __syncwarp();
+                    if(lane < DIM) table[one + lane] += sum;
+                    rest &= ~__ballot_sync(0xffffffffu, mine);
                 }
+                __syncwarp();
             }
         }
         __syncthreads();
@@ -1127,7 +1189,7 @@ __global__ void __launch_bounds__(kThreads) own_join_kernel(const float *partial
 uint32_t own_chunks(uint64_t count, uint64_t rows, uint64_t dim)
 {
     if(dim > kOwnDim || rows < kOwnRows || rows * dim * 4 > kOwnTable) return 0;
-    uint64_t chunks = count / kOwnTile, most = count / (2 * rows);
+    uint64_t chunks = count / kOwnTile, most = count / rows;
     if(chunks > most) chunks = most;
     if(chunks < 148) return 0;
     return (uint32_t)(chunks < 296 ? chunks : 296);
@@ -1327,12 +1389,23 @@ template <typename GT, typename TT, typename I>
 cudaError_t launch_own(const void *grad, uint64_t stride, const void *index, uint32_t count, const Use &use, const Plan &plan,
                        float *partial, const Table &table, uint32_t dim, cudaStream_t stream)
 {
-    constexpr size_t shared = sizeof(SortShared<kOwnThreads, kOwnItems>);
-    const cudaError_t e = gsx_allow_smem<own_table_kernel<GT, I>>(shared + kOwnTable);
-    if(e != cudaSuccess) return e;
     const uint32_t size = (uint32_t)table.rows * dim;
-    own_table_kernel<GT, I><<<plan.own, kOwnThreads, shared + size * 4, stream>>>(
-        static_cast<const GT *>(grad), (uint32_t)(stride * sizeof(GT)), static_cast<const I *>(index), count, use, dim, partial);
+    const uint32_t tile = own_tile(own_length(count, plan.own), (uint32_t)table.rows, dim, sizeof(GT));
+    auto launch = [&](auto kernel, cudaError_t e) {
+        if(e != cudaSuccess) return e;
+        const size_t smem = sizeof(OwnShared) - sizeof(uint32_t) * (kOwnTile - tile) + (size_t)tile * dim * sizeof(GT) + 4 * (size_t)size;
+        kernel<<<plan.own, kOwnThreads, smem, stream>>>(static_cast<const GT *>(grad), (uint32_t)(stride * sizeof(GT)),
+                                                        static_cast<const I *>(index), count, use, tile, partial);
+        return cudaSuccess;
+    };
+    cudaError_t e;
+    switch(dim) {
+    case 1: e = launch(own_table_kernel<GT, I, 1>, gsx_allow_smem<own_table_kernel<GT, I, 1>>(kOwnMemory)); break;
+    case 2: e = launch(own_table_kernel<GT, I, 2>, gsx_allow_smem<own_table_kernel<GT, I, 2>>(kOwnMemory)); break;
+    case 3: e = launch(own_table_kernel<GT, I, 3>, gsx_allow_smem<own_table_kernel<GT, I, 3>>(kOwnMemory)); break;
+    default: e = launch(own_table_kernel<GT, I, 4>, gsx_allow_smem<own_table_kernel<GT, I, 4>>(kOwnMemory)); break;
+    }
+    if(e != cudaSuccess) return e;
     return gsx_launch_pdl(own_join_kernel<TT>, dim3((size + 31) / 32), dim3(kThreads), 0, stream, (const float *)partial, size,
                           plan.own, dim, table);
 }
