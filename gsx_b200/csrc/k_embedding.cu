@@ -15,12 +15,12 @@
  *   sums    every CTA takes as many sorted positions as the others, whatever their rows: rows of any popularity cost the
  *           same (a warp for each row took 3 to 4 times as long on skewed indices).  Groups of lanes walk runs of
  *           positions with the gradients of the next ones in flight; rows that cross runs or CTAs are joined in order.
- *   small tables of up to four columns with many positions skip the sort as a whole (own_table_kernel).
+ *   small tables of short rows skip the sort: CTAs with tables of sums in shared memory (own_table_kernel).
  * The kernels of a call are launched so that each starts while the one before ends (gsx_launch_pdl).
  *
  * Sums are held in 32 bits.  No chain of additions is longer than a run (128 positions), plus one term for every group
- * of a CTA (64) and an eighth of the CTAs that a row crosses; in the tables in shared memory a chain has the chunk's
- * positions of the row, plus one term for every 37 chunks and eight of those.
+ * of a CTA (64) and an eighth of the CTAs that a row crosses; in the tables in shared memory a chain has the
+ * row's positions of a chunk (at most a 296th of all, or 512), plus one term for every 37 chunks and eight of those.
  */
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -1010,16 +1010,22 @@ __global__ void __launch_bounds__(kThreads) row_join_kernel(const Runs a, const 
 }
 
 /* ------------------------------------------------------------------------------------------ */
-/* Small tables of short rows (a codebook of colours) and many positions: the positions need not be sorted as a whole.
- * 3M x 3 f32 into 4096 rows: 60 us, bound by latency (two CTAs an SM, 0.31 of the issue slots; the data alone takes 7).
- * A CTA keeps a table of sums in shared memory and walks a chunk of the positions in tiles: it ranks a tile by the low
- * 8 bits of the row, and thread t adds up the positions of the rows that end in t, in order.  The CTAs' tables are then
- * added up in the order of the chunks.  Lists of more than kOwnLong positions are walked by a warp, 32 at a time. */
+/* Small tables of short rows (a codebook of colours): the positions need not be sorted as a whole.  A CTA keeps a table of
+ * sums in shared memory and walks a chunk of the positions in tiles.  It ranks a tile by the low 8 bits of the row while the
+ * tile's gradients come into shared memory beside it, then the sums are added in that order: every row has one owner in
+ * the CTA, so the order is fixed.  The CTAs' tables are then added up in the order of the chunks.
+ *
+ * 3M x 3 f32 into 4096 rows: 41 us, bound by the instructions and shared-memory accesses of ranking and walking (16 warps an
+ * SM, as two tables fill its memory); the data alone takes 7.  Of the 64 us that it took before, a fifth went into loads
+ * that all CTAs waited for at the same time: the next tile's indices now go to registers and its gradients to the L2
+ * while this one is walked.  Gradients read by the walk itself, in sorted order, cost the same as staging them, but had
+ * no room for that. */
 constexpr int kOwnThreads = 256;
 constexpr int kOwnItems = 16; /* positions a thread of a tile, at most */
 constexpr uint32_t kOwnTile = kOwnThreads * kOwnItems;
 static_assert(kOwnTile <= 1u << kPlaceBits, "a place of a tile fits a pair");
-constexpr uint64_t kOwnDim = 4, kOwnRows = 128;
+constexpr uint64_t kOwnLeast = 512; /* positions of a chunk */
+constexpr uint32_t kOwnFewest = 512; /* of a tile */
 constexpr size_t kOwnTable = 68 * 1024;
 static_assert(kOwnTable / 4 <= 1u << (32 - kPlaceBits), "a row fits a pair");
 constexpr size_t kOwnMemory = 113 * 1024; /* of a CTA: two an SM */
@@ -1027,12 +1033,18 @@ constexpr uint32_t kOwnLong = 64;
 static_assert(kOwnThreads == kMaxBins, "thread t owns digit t");
 using OwnShared = SortShared<kOwnThreads, kOwnItems, uint32_t>;
 
-/* positions of a tile: as many as fit beside the table, with their pairs and gradients, in tiles of equal length */
+/* the most positions of a tile beside the table, with their pairs and gradients of gb bytes an element */
+uint32_t own_fit(uint64_t rows, uint64_t dim, uint64_t gb)
+{
+    const uint64_t fixed = sizeof(OwnShared) - sizeof(uint32_t) * kOwnTile + 4 * rows * dim;
+    const uint64_t fit = (kOwnMemory - fixed) / (sizeof(uint32_t) + dim * gb) / 32 * 32;
+    return fit < kOwnTile ? (uint32_t)fit : kOwnTile;
+}
+
+/* tiles of equal length */
 uint32_t own_tile(uint32_t len, uint32_t rows, uint32_t dim, size_t gb)
 {
-    const size_t fixed = sizeof(OwnShared) - sizeof(uint32_t) * kOwnTile + 4 * (size_t)rows * dim;
-    const size_t fit = (kOwnMemory - fixed) / (sizeof(uint32_t) + dim * gb) / 32 * 32;
-    const uint32_t most = fit < kOwnTile ? (uint32_t)fit : kOwnTile, tiles = (len + most - 1) / most;
+    const uint32_t most = own_fit(rows, dim, gb), tiles = (len + most - 1) / most;
     return ((len + tiles - 1) / tiles + 31) / 32 * 32;
 }
 
@@ -1042,20 +1054,138 @@ __host__ __device__ constexpr uint32_t own_length(uint32_t count, uint32_t chunk
     return ((count + chunks - 1) / chunks + 31u) / 32u * 32u;
 }
 
+/* Rows of DIM elements: thread t adds up the n pairs of digit t.  Lists of more than kOwnLong go to a warp, 32 at a time. */
+template <typename GT, int DIM>
+__device__ __forceinline__ void walk_lists(const OwnShared &s, const uint32_t *s_count, uint32_t n, uint32_t rows, const GT *s_grad,
+                                           float *table)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    auto split = [&](uint32_t pair, float(&x)[DIM]) { /* its row in the table */
+        const GT *g = s_grad + (pair & ((1u << kPlaceBits) - 1u)) * DIM;
+#pragma unroll
+        for(int c = 0; c < DIM; ++c) x[c] = to_f32(g[c]);
+        return table + (pair >> kPlaceBits) * DIM;
+    };
+    const uint32_t first = s.before[threadIdx.x];
+    if(n <= kOwnLong)
+        for(uint32_t j = 0; j < n; j += 4) {
+            float *to[4];
+            float x[4][DIM];
+#pragma unroll
+            for(uint32_t u = 0; u < 4; ++u) to[u] = split(s.pair[first + (j + u < n ? j + u : n - 1)], x[u]);
+#pragma unroll
+            for(uint32_t u = 0; u < 4; ++u)
+                if(j + u < n)
+#pragma unroll
+                    for(int c = 0; c < DIM; ++c) to[u][c] += x[u][c];
+        }
+    unsigned lists = __ballot_sync(0xffffffffu, s_count[lane * (kOwnThreads / 32) + warp] > kOwnLong);
+    for(; lists != 0u; lists &= lists - 1u) {
+        const int t = (__ffs(lists) - 1) * (kOwnThreads / 32) + warp;
+        const uint32_t m = s_count[t], at = s.before[t];
+        if(rows <= kMaxBins) { /* the list is one row's: the lanes add up theirs first */
+            float sum[DIM] = {}, one = 0.0f;
+#pragma unroll 4
+            for(uint32_t j = lane; j < m; j += 32) {
+                float x[DIM];
+                split(s.pair[at + j], x);
+#pragma unroll
+                for(int c = 0; c < DIM; ++c) sum[c] += x[c];
+            }
+#pragma unroll
+            for(int c = 0; c < DIM; ++c) {
+#pragma unroll
+                for(int o = 16; o > 0; o >>= 1) sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], o);
+                one = lane == c ? sum[c] : one;
+            }
+            if(lane < DIM) table[t * DIM + lane] += one;
+            continue;
+        }
+        /* the sums of a step's distinct rows one after another */
+        for(uint32_t j = 0; j < m; j += 32) {
+            const bool in = j + lane < m;
+            float x[DIM];
+            float *to = split(s.pair[at + (in ? j + lane : m - 1)], x);
+            const uint32_t place = (uint32_t)(to - table);
+            unsigned rest = __ballot_sync(0xffffffffu, in);
+            while(rest != 0u) {
+                const uint32_t one = __shfl_sync(0xffffffffu, place, __ffs(rest) - 1);
+                const bool mine = in && place == one;
+                float sum = 0.0f; /* lane c: of column c */
+#pragma unroll
+                for(int c = 0; c < DIM; ++c) {
+                    float v = mine ? x[c] : 0.0f;
+#pragma unroll
+                    for(int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+                    sum = lane == c ? v : sum;
+                }
+                if(lane < DIM) table[one + lane] += sum;
+                rest &= ~__ballot_sync(0xffffffffu, mine);
+            }
+            __syncwarp();
+        }
+    }
+}
+
+/* Longer rows: groups of lanes side by side on the columns.  A group owns the digits whose pairs start in its equal share of
+ * the tile (300k x 24 into 500 rows: 29 us; a thread for a digit's pairs, four columns at a time, took 61) and walks them as
+ * they lie, storing a sum whenever the row changes. */
+template <typename GT>
+__device__ __forceinline__ void walk_columns(const OwnShared &s, const GT *s_grad, uint32_t dim, float *table)
+{
+    const int clog = dim > 16 ? 5 : dim > 8 ? 4 : 3;
+    const uint32_t groups = kOwnThreads >> clog, group = threadIdx.x >> clog;
+    const uint32_t share = (s.before[kMaxBins] + groups - 1) / groups;
+    auto start = [&](uint32_t place) { /* of the first digit whose pairs start there or behind */
+        uint32_t lo = 0, hi = kMaxBins;
+        while(lo < hi) {
+            const uint32_t mid = (lo + hi) / 2;
+            if(s.before[mid] < place) lo = mid + 1;
+            else hi = mid;
+        }
+        return s.before[lo];
+    };
+    const uint32_t from = start(group * share), to = start((group + 1) * share);
+    for(uint32_t c = threadIdx.x & ((1u << clog) - 1u); c < dim; c += 1u << clog) {
+        uint32_t row = 0xffffffffu;
+        float sum = 0.0f;
+        for(uint32_t j = from; j < to; j += 8) {
+            uint32_t pair[8];
+            float x[8];
+#pragma unroll
+            for(uint32_t u = 0; u < 8; ++u) pair[u] = s.pair[j + u < to ? j + u : to - 1];
+#pragma unroll
+            for(uint32_t u = 0; u < 8; ++u) x[u] = to_f32(s_grad[(pair[u] & ((1u << kPlaceBits) - 1u)) * dim + c]);
+#pragma unroll
+            for(uint32_t u = 0; u < 8; ++u) {
+                if(j + u >= to) break;
+                if(pair[u] >> kPlaceBits != row) {
+                    if(row != 0xffffffffu) table[row * dim + c] += sum;
+                    row = pair[u] >> kPlaceBits;
+                    sum = 0.0f;
+                }
+                sum += x[u];
+            }
+        }
+        if(row != 0xffffffffu) table[row * dim + c] += sum;
+    }
+}
+
 template <typename GT, typename I, int DIM>
 __global__ void __launch_bounds__(kOwnThreads, 2) own_table_kernel(const GT *__restrict__ grad, uint32_t stride_bytes,
                                                                    const I *__restrict__ index, uint32_t count, const Use use,
-                                                                   uint32_t tile, float *__restrict__ partial)
+                                                                   uint32_t tile, uint32_t any_dim, float *__restrict__ partial)
 {
+    const uint32_t dim = DIM > 0 ? DIM : any_dim;
     extern __shared__ __align__(16) unsigned char smem[];
     OwnShared &s = *reinterpret_cast<OwnShared *>(smem);
-    const uint32_t size = use.rows * DIM;
+    const uint32_t size = use.rows * dim;
     GT *s_grad = reinterpret_cast<GT *>(smem + (sizeof(OwnShared) - sizeof(uint32_t) * (kOwnTile - tile)));
-    float *table = reinterpret_cast<float *>(s_grad + tile * DIM);
+    float *table = reinterpret_cast<float *>(s_grad + tile * dim);
     uint32_t *s_count = s.hist[0]; /* of a digit: its pairs; the histograms are done with by then */
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const unsigned char *bytes = reinterpret_cast<const unsigned char *>(grad);
-    const bool dense = stride_bytes == DIM * sizeof(GT) && (uintptr_t)grad % 16 == 0;
+    const bool dense = stride_bytes == dim * sizeof(GT) && (uintptr_t)grad % 16 == 0;
     const uint32_t len = own_length(count, gridDim.x);
     const uint32_t begin = len * blockIdx.x < count ? len * blockIdx.x : count, end = count - begin < len ? count : begin + len;
     I raw[kOwnItems]; /* the indices of the next tile */
@@ -1074,9 +1204,9 @@ __global__ void __launch_bounds__(kOwnThreads, 2) own_table_kernel(const GT *__r
         const int items = (int)((here + kOwnThreads - 1) / kOwnThreads);
         /* the tile's gradients, on their way while it is ranked, and the next one's as far as the L2 */
         if(dense) {
-            const unsigned char *from = bytes + (uint64_t)i0 * (DIM * sizeof(GT));
+            const unsigned char *from = bytes + (uint64_t)i0 * (dim * sizeof(GT));
             unsigned char *to = reinterpret_cast<unsigned char *>(s_grad);
-            const uint32_t all = here * DIM * (uint32_t)sizeof(GT), whole = all / 16 * 16;
+            const uint32_t all = here * dim * (uint32_t)sizeof(GT), whole = all / 16 * 16;
 #pragma unroll 4
             for(uint32_t o = threadIdx.x * 16; o < whole; o += kOwnThreads * 16)
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to + o)), "l"(from + o)
@@ -1084,12 +1214,12 @@ __global__ void __launch_bounds__(kOwnThreads, 2) own_table_kernel(const GT *__r
             asm volatile("cp.async.commit_group;" ::: "memory");
             const uint32_t o = whole + threadIdx.x * (uint32_t)sizeof(GT);
             if(o < all) *reinterpret_cast<GT *>(to + o) = *reinterpret_cast<const GT *>(from + o);
-            const uint32_t rest = end - i0 - here, next = (rest < tile ? rest : tile) * DIM * (uint32_t)sizeof(GT) / 16 * 16;
+            const uint32_t rest = end - i0 - here, next = (rest < tile ? rest : tile) * dim * (uint32_t)sizeof(GT) / 16 * 16;
             if(threadIdx.x == 0 && next > 0)
                 asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from + all), "r"(next) : "memory");
         } else {
-            for(uint32_t j = threadIdx.x; j < here * DIM; j += kOwnThreads)
-                s_grad[j] = reinterpret_cast<const GT *>(bytes + (uint64_t)(i0 + j / DIM) * stride_bytes)[j % DIM];
+            for(uint32_t j = threadIdx.x; j < here * dim; j += kOwnThreads)
+                s_grad[j] = reinterpret_cast<const GT *>(bytes + (uint64_t)(i0 + j / dim) * stride_bytes)[j % dim];
         }
         uint32_t k[kOwnItems], p[kOwnItems];
         bool valid[kOwnItems], outside = false;
@@ -1106,53 +1236,8 @@ __global__ void __launch_bounds__(kOwnThreads, 2) own_table_kernel(const GT *__r
         if(i0 + here < end) fetch(i0 + here);
         asm volatile("cp.async.wait_all;" ::: "memory");
         __syncthreads();
-        auto split = [&](uint32_t pair, float(&x)[DIM]) { /* its row in the table */
-            const GT *g = s_grad + (pair & ((1u << kPlaceBits) - 1u)) * DIM;
-#pragma unroll
-            for(int c = 0; c < DIM; ++c) x[c] = to_f32(g[c]);
-            return table + (pair >> kPlaceBits) * DIM;
-        };
-        const uint32_t first = s.before[threadIdx.x];
-        if(n <= kOwnLong)
-            for(uint32_t j = 0; j < n; j += 4) {
-                float *to[4];
-                float x[4][DIM];
-#pragma unroll
-                for(uint32_t u = 0; u < 4; ++u) to[u] = split(s.pair[first + (j + u < n ? j + u : n - 1)], x[u]);
-#pragma unroll
-                for(uint32_t u = 0; u < 4; ++u)
-                    if(j + u < n)
-#pragma unroll
-                        for(int c = 0; c < DIM; ++c) to[u][c] += x[u][c];
-            }
-        /* the long lists, dealt to the warps: the sums of a step's distinct rows one after another */
-        unsigned lists = __ballot_sync(0xffffffffu, s_count[lane * (kOwnThreads / 32) + warp] > kOwnLong);
-        for(; lists != 0u; lists &= lists - 1u) {
-            const int t = (__ffs(lists) - 1) * (kOwnThreads / 32) + warp;
-            const uint32_t m = s_count[t], at = s.before[t];
-            for(uint32_t j = 0; j < m; j += 32) {
-                const bool in = j + lane < m;
-                float x[DIM];
-                float *to = split(s.pair[at + (in ? j + lane : m - 1)], x);
-                const uint32_t place = (uint32_t)(to - table);
-                unsigned rest = __ballot_sync(0xffffffffu, in);
-                while(rest != 0u) {
-                    const uint32_t one = __shfl_sync(0xffffffffu, place, __ffs(rest) - 1);
-                    const bool mine = in && place == one;
-                    float sum = 0.0f; /* lane c: of column c */
-#pragma unroll
-                    for(int c = 0; c < DIM; ++c) {
-                        float v = mine ? x[c] : 0.0f;
-#pragma unroll
-                        for(int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-                        sum = lane == c ? v : sum;
-                    }
-                    if(lane < DIM) table[one + lane] += sum;
-                    rest &= ~__ballot_sync(0xffffffffu, mine);
-                }
-                __syncwarp();
-            }
-        }
+        if constexpr(DIM > 0) walk_lists<GT, DIM>(s, s_count, n, use.rows, s_grad, table);
+        else walk_columns(s, s_grad, dim, table);
         __syncthreads();
     }
     __syncthreads();
@@ -1182,16 +1267,14 @@ __global__ void __launch_bounds__(kThreads) own_join_kernel(const float *partial
     store_sums<TT, 1>(table, j / dim, j % dim, sum);
 }
 
-/* Chunks of a call that takes this path, or 0: the table fits, and there are enough positions for half the GPU's CTAs
- * with tables that cost no more to write and read than the gradients.  Measured against the sort of all positions
- * (us, here / there): 3M x 3 into 4096 rows 63 / 105, into 256 59 / 79, into 64 79 / 71 (few long lists); 2M x 4 into
- * 512 rows 49 / 72; 2M x 9 into 1000 rows 91 / 89, 2M x 16 276 / 94 (a walk of the lists for every four columns). */
+/* Chunks of a call that takes this path, or 0: the table fits and leaves room for a tile that is worth its fixed steps.
+ * Measured against the sort of all positions (us, here / there): 3M x 3 into 4096 rows 41 / 104, into 1 row 36 / 75;
+ * 300k x 3 into 4096 14 / 35; 1000 x 3 into 4096 8 / 14; 2.5M x 15 into 1000 122 / 140; 20000 x 24 into 500 14 / 23.  Rows
+ * whose tiles would be shorter: 300k x 45 into 300 50 / 40.  1024 positions a chunk: 1000 x 15 into 1000 17 us, with 512 10. */
 uint32_t own_chunks(uint64_t count, uint64_t rows, uint64_t dim)
 {
-    if(dim > kOwnDim || rows < kOwnRows || rows * dim * 4 > kOwnTable) return 0;
-    uint64_t chunks = count / kOwnTile, most = count / rows;
-    if(chunks > most) chunks = most;
-    if(chunks < 148) return 0;
+    if(rows * dim * 4 > kOwnTable || own_fit(rows, dim, 4) < kOwnFewest) return 0;
+    const uint64_t chunks = (count + kOwnLeast - 1) / kOwnLeast;
     return (uint32_t)(chunks < 296 ? chunks : 296);
 }
 
@@ -1395,7 +1478,7 @@ cudaError_t launch_own(const void *grad, uint64_t stride, const void *index, uin
         if(e != cudaSuccess) return e;
         const size_t smem = sizeof(OwnShared) - sizeof(uint32_t) * (kOwnTile - tile) + (size_t)tile * dim * sizeof(GT) + 4 * (size_t)size;
         kernel<<<plan.own, kOwnThreads, smem, stream>>>(static_cast<const GT *>(grad), (uint32_t)(stride * sizeof(GT)),
-                                                        static_cast<const I *>(index), count, use, tile, partial);
+                                                        static_cast<const I *>(index), count, use, tile, dim, partial);
         return cudaSuccess;
     };
     cudaError_t e;
@@ -1403,7 +1486,8 @@ cudaError_t launch_own(const void *grad, uint64_t stride, const void *index, uin
     case 1: e = launch(own_table_kernel<GT, I, 1>, gsx_allow_smem<own_table_kernel<GT, I, 1>>(kOwnMemory)); break;
     case 2: e = launch(own_table_kernel<GT, I, 2>, gsx_allow_smem<own_table_kernel<GT, I, 2>>(kOwnMemory)); break;
     case 3: e = launch(own_table_kernel<GT, I, 3>, gsx_allow_smem<own_table_kernel<GT, I, 3>>(kOwnMemory)); break;
-    default: e = launch(own_table_kernel<GT, I, 4>, gsx_allow_smem<own_table_kernel<GT, I, 4>>(kOwnMemory)); break;
+    case 4: e = launch(own_table_kernel<GT, I, 4>, gsx_allow_smem<own_table_kernel<GT, I, 4>>(kOwnMemory)); break;
+    default: e = launch(own_table_kernel<GT, I, 0>, gsx_allow_smem<own_table_kernel<GT, I, 0>>(kOwnMemory)); break;
     }
     if(e != cudaSuccess) return e;
     return gsx_launch_pdl(own_join_kernel<TT>, dim3((size + 31) / 32), dim3(kThreads), 0, stream, (const float *)partial, size,

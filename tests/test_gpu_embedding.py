@@ -250,6 +250,33 @@ def test_gradients_that_are_not_finite_stay_in_their_rows(cuda_device):
         assert bool(finite.all())
 
 
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("dim", [1, 2, 3, 4, 5, 8, 9, 16, 17, 24, 33])
+@pytest.mark.parametrize("count,rows", [(1, 1), (511, 3), (513, 300), (5000, 256), (5001, 257), (40_000, 500), (400_000, 40)])
+def test_gradients_of_small_tables(cuda_device, count, rows, dim, dtype):
+    """Tables that fit in shared memory: rows of every length, few rows (long lists) and many, popular rows, rows apart,
+    a start at any element, padding and indices out of range."""
+    g = _gen(count + dim)
+    for pad, start in ((0, 0), (3, 1)):
+        buf = torch.randn(count * (dim + pad) + start, generator=g, device="cuda").to(dtype)
+        grad = buf[start:].view(count, dim + pad)[:, :dim]
+        index = (torch.rand(count, generator=g, device="cuda").pow(2 + pad) * rows).int().clamp_(max=rows - 1)
+        if count > 600:
+            index[5] = -1
+            index[600] = rows
+        used = (index >= 0) & (index < rows)
+        want = torch.zeros(rows, dim, dtype=torch.float64, device="cuda")
+        want.index_add_(0, index[used].long(), grad[used].double())
+        size = torch.zeros_like(want).index_add_(0, index[used].long(), grad[used].double().abs())
+        n = torch.bincount(index[used].long(), minlength=rows).double()[:, None]
+        flag = torch.zeros(1, dtype=torch.int32, device="cuda")
+        got = gb.embedding_backward(grad, index, torch.empty(rows, dim, device="cuda"), scale=0.75, bad=flag)
+        assert bool(((got.double() - 0.75 * want).abs() <= 1.01 * U * 0.75 * size * (n + 2)).all())
+        assert bool(flag.item()) == (count > 600)
+        again = gb.embedding_backward(grad, index, torch.empty(rows, dim, device="cuda"), scale=0.75)
+        assert torch.equal(got, again)
+
+
 def test_offsets_behind_32_bits(cuda_device):
     """Tables, outputs and gradients of more than 4 GiB: their last rows are read and written at their own place."""
     dim = 1024
