@@ -510,16 +510,10 @@ __device__ __forceinline__ uint32_t sort_tile(SortShared<THREADS, ITEMS, P> &s, 
                 }
             }
             digit[it] = valid[it] ? d : bins;
-            rank[it] = (uint32_t)__popc(peers & ((1u << lane) - 1u)) | (uint32_t)__popc(peers) << 16; /* and the peers */
-        }
-    }
-#pragma unroll
-    for(int it = 0; it < ITEMS; ++it) {
-        if(it < items) {
             const uint32_t before = wh[digit[it]];
+            rank[it] = before + (uint32_t)__popc(peers & ((1u << lane) - 1u));
             __syncwarp();
-            wh[digit[it]] = before + (rank[it] >> 16); /* the same from every lane of the digit */
-            rank[it] = before + (rank[it] & 0xffffu);
+            wh[digit[it]] = before + (uint32_t)__popc(peers);
             __syncwarp();
         }
     }
@@ -546,7 +540,7 @@ __device__ __forceinline__ uint32_t sort_tile(SortShared<THREADS, ITEMS, P> &s, 
     __syncthreads();
 #pragma unroll
     for(int it = 0; it < ITEMS; ++it)
-        if(it < items && valid[it]) set_pair(s.pair[s.before[digit[it]] + wh[digit[it]] + rank[it]], key[it], pos[it]);
+        if(it < items && (sizeof(P) == 8 || valid[it])) set_pair(s.pair[s.before[digit[it]] + wh[digit[it]] + rank[it]], key[it], pos[it]);
     __syncthreads();
     return count;
 }
@@ -1015,7 +1009,7 @@ __global__ void __launch_bounds__(kThreads) row_join_kernel(const Runs a, const 
  * tile's gradients come into shared memory beside it, then the sums are added in that order: every row has one owner in
  * the CTA, so the order is fixed.  The CTAs' tables are then added up in the order of the chunks.
  *
- * 3M x 3 f32 into 4096 rows: 41 us, bound by the instructions and shared-memory accesses of ranking and walking (16 warps an
+ * 3M x 3 f32 into 4096 rows: 40 us, bound by the instructions and shared-memory accesses of ranking and walking (16 warps an
  * SM, as two tables fill its memory); the data alone takes 7.  Of the 64 us that it took before, a fifth went into loads
  * that all CTAs waited for at the same time: the next tile's indices now go to registers and its gradients to the L2
  * while this one is walked.  Gradients read by the walk itself, in sorted order, cost the same as staging them, but had
@@ -1268,7 +1262,7 @@ __global__ void __launch_bounds__(kThreads) own_join_kernel(const float *partial
 }
 
 /* Chunks of a call that takes this path, or 0: the table fits and leaves room for a tile that is worth its fixed steps.
- * Measured against the sort of all positions (us, here / there): 3M x 3 into 4096 rows 41 / 104, into 1 row 36 / 75;
+ * Measured against the sort of all positions (us, here / there): 3M x 3 into 4096 rows 40 / 104, into 1 row 36 / 75;
  * 300k x 3 into 4096 14 / 35; 1000 x 3 into 4096 8 / 14; 2.5M x 15 into 1000 122 / 140; 20000 x 24 into 500 14 / 23.  Rows
  * whose tiles would be shorter: 300k x 45 into 300 50 / 40.  1024 positions a chunk: 1000 x 15 into 1000 17 us, with 512 10. */
 uint32_t own_chunks(uint64_t count, uint64_t rows, uint64_t dim)
