@@ -1019,8 +1019,7 @@ constexpr int kOwnItems = 16; /* positions a thread of a tile, at most */
 constexpr uint32_t kOwnTile = kOwnThreads * kOwnItems;
 static_assert(kOwnTile <= 1u << kPlaceBits, "a place of a tile fits a pair");
 constexpr uint64_t kOwnLeast = 512; /* positions of a chunk */
-constexpr uint32_t kOwnFewest = 512; /* of a tile */
-constexpr size_t kOwnTable = 68 * 1024;
+constexpr size_t kOwnTable = 96 * 1024;
 static_assert(kOwnTable / 4 <= 1u << (32 - kPlaceBits), "a row fits a pair");
 constexpr size_t kOwnMemory = 113 * 1024; /* of a CTA: two an SM */
 constexpr uint32_t kOwnLong = 64;
@@ -1264,10 +1263,12 @@ __global__ void __launch_bounds__(kThreads) own_join_kernel(const float *partial
 /* Chunks of a call that takes this path, or 0: the table fits and leaves room for a tile that is worth its fixed steps.
  * Measured against the sort of all positions (us, here / there): 3M x 3 into 4096 rows 40 / 104, into 1 row 36 / 75;
  * 300k x 3 into 4096 14 / 35; 1000 x 3 into 4096 8 / 14; 2.5M x 15 into 1000 122 / 140; 20000 x 24 into 500 14 / 23.  Rows
- * whose tiles would be shorter: 300k x 45 into 300 50 / 40.  1024 positions a chunk: 1000 x 15 into 1000 17 us, with 512 10. */
+ * whose tiles would be shorter than 512: 300k x 45 into 300 50 / 40, 2.5M x 24 into 800 231 / 163; but with few columns and
+ * positions 20000 x 24 into 800 17 / 22, 100k x 15 into 1278 20 / 27.  1024 positions a chunk: 1000 x 15 into 1000 17 us,
+ * with 512 10. */
 uint32_t own_chunks(uint64_t count, uint64_t rows, uint64_t dim)
 {
-    if(rows * dim * 4 > kOwnTable || own_fit(rows, dim, 4) < kOwnFewest) return 0;
+    if(rows * dim * 4 > kOwnTable || own_fit(rows, dim, 4) < (count <= 1u << 18 && dim <= 24 ? 256u : 512u)) return 0;
     const uint64_t chunks = (count + kOwnLeast - 1) / kOwnLeast;
     return (uint32_t)(chunks < 296 ? chunks : 296);
 }

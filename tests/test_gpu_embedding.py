@@ -252,7 +252,7 @@ def test_gradients_that_are_not_finite_stay_in_their_rows(cuda_device):
 
 @pytest.mark.parametrize("dtype", [F32, F16])
 @pytest.mark.parametrize("dim", [1, 2, 3, 4, 5, 8, 9, 16, 17, 24, 33])
-@pytest.mark.parametrize("count,rows", [(1, 1), (511, 3), (513, 300), (5000, 256), (5001, 257), (40_000, 500), (400_000, 40)])
+@pytest.mark.parametrize("count,rows", [(1, 1), (511, 3), (513, 300), (5000, 256), (5001, 257), (40_000, 500), (400_000, 40), (6000, 2600)])
 def test_gradients_of_small_tables(cuda_device, count, rows, dim, dtype):
     """Tables that fit in shared memory: rows of every length, few rows (long lists) and many, popular rows, rows apart,
     a start at any element, padding and indices out of range."""
