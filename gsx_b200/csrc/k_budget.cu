@@ -2,7 +2,7 @@
  * Keeping a set of entries (a scene's Gaussians, the rows of key-value caches) within a budget by accumulated weight.
  *
  *   accumulate  out[g, j] = decay * score[g, j] + sum over r of weights[g, r, j].  Reads every weight once; bound by DRAM
- *               (8 x 2048 x 8192 bf16: 42.3 us, 6.3 TB/s; 8 x 3M f32 onto one scene: 22.8 us, 5.3 TB/s).
+ *               (8 x 2048 x 8192 bf16: 41.6 us, 6.5 TB/s; 8 x 3M f32 onto one scene: 19.1 us, 6.3 TB/s).
  *   select      the ordered list of the entries that stay: the `first` first, the `recent` last, and of the others
  *               those with the largest scores (ties to the lowest index).  Bound by latency: each step needs the one
  *               before (32 groups of 32768: 17 us; 3M entries: 49 us in five launches over the whole GPU).
