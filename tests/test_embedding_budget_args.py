@@ -95,12 +95,15 @@ def test_workspace_sizes():
     assert L.gsx_b200_embedding_workspace_bytes(10, 0, 4) == 0
     small = L.gsx_b200_embedding_workspace_bytes(100, 50, 4)
     assert 800 <= small < 1 << 20
-    # (row, position) pairs: once for a sort of one pass (up to 256 rows), twice for more
-    one = L.gsx_b200_embedding_workspace_bytes(500_000, 256, 8)
-    two = L.gsx_b200_embedding_workspace_bytes(500_000, 257, 8)
-    assert 4_000_000 < one < 8_000_000 <= two < 12_000_000
-    # many positions, short rows and a table that fits shared memory: one table of sums for each of 296 chunks
+    # a table that fits shared memory: one table of sums for each of up to 296 chunks
+    assert L.gsx_b200_embedding_workspace_bytes(500_000, 256, 8) == 256 + 296 * 256 * 8 * 4
+    assert L.gsx_b200_embedding_workspace_bytes(500_000, 257, 8) == 256 + 296 * 257 * 8 * 4
     assert L.gsx_b200_embedding_workspace_bytes(3_000_000, 4096, 3) == 256 + 296 * 4096 * 3 * 4
+    assert L.gsx_b200_embedding_workspace_bytes(1000, 10, 4) == 256 + 2 * 10 * 4 * 4
+    # else (row, position) pairs: once for a sort of one pass (up to 256 rows), twice for more
+    one = L.gsx_b200_embedding_workspace_bytes(500_000, 256, 1000)
+    two = L.gsx_b200_embedding_workspace_bytes(500_000, 257, 1000)
+    assert 4_000_000 <= two - one < 4_001_000
     assert L.gsx_b200_budget_workspace_bytes(32, 131_072) == 0
     assert 0 < L.gsx_b200_budget_workspace_bytes(32, 131_073) < 4 << 20
 
