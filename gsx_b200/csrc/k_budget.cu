@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, kAccumulateCtas) accumulate_shifted_
         const uint32_t nr = length_of(row_lengths, g, rows);
         const T *w = weights + (uint64_t)g * group_stride + (uint64_t)row0 * row_stride + c0;
         const uint32_t shift = (uint32_t)((uintptr_t)w % 16) / (uint32_t)sizeof(T);
-        const int64_t col = (int64_t)c0 + ct * VW - (int64_t)shift; /* of the thread's block: its first column, may be below 0 */
+        const int64_t col = (int64_t)c0 + ct * VW - (int64_t)shift; /* the first column of the thread's block */
         w = w + ct * VW - shift;
         float acc[VW] = {};
         if(col < (int64_t)n) {
@@ -329,9 +329,10 @@ cudaError_t launch_accumulate(uint64_t unit, const float *score, uint64_t score_
     const bool many = rows >= 32;
     if(unit == 16) return many ? run(launch_accumulate_rg<T, W, 8, false>) : run(launch_accumulate_rg<T, W, 1, false>);
     if(unit == 8) return many ? run(launch_accumulate_rg<T, W / 2, 4, false>) : run(launch_accumulate_rg<T, W / 2, 1, false>);
-    /* the shifted form reads whole blocks between the first and the last element: rows of at least a block, none inside another */
-    const bool apart = length >= (uint32_t)W && (groups == 1 || (group_stride >= length && (group_stride >= (uint64_t)(rows - 1) * row_stride + length ||
-                                                                                      row_stride >= (uint64_t)(groups - 1) * group_stride + length)));
+    /* the shifted form reads whole blocks between the first and the last element: rows of at least a block, none in another */
+    const uint64_t all_rows = (uint64_t)(rows - 1) * row_stride + length, all_groups = (uint64_t)(groups - 1) * group_stride + length;
+    const bool apart = length >= (uint32_t)W &&
+                       (groups == 1 || (group_stride >= length && (group_stride >= all_rows || row_stride >= all_groups)));
     if(many && apart)
         return launch_split(accumulate_shifted_kernel<T>, kThreads - W, W, groups, rows, length, stream, score, score_stride,
                             static_cast<const T *>(weights), group_stride, row_stride, groups, rows, length, lengths, row_lengths,

@@ -782,7 +782,7 @@ __global__ void __launch_bounds__(kSortThreads) digit_scatter_kernel(const I *__
 /* sums of sorted positions by row
  *
  * 1M x 45 f32 into 16384 rows: 57 us for 243 MB (a row of 180 bytes touches 64-byte pieces that it shares with its
- * neighbours) in random order, 0.52 of the DRAM's peak, bound by the latency of the gathers; 40 more for the sort.
+ * neighbours) in random order, 0.52 of the DRAM's peak, bound by the latency of the gathers; 35 more for the sort.
  *
  * A CTA owns R consecutive sorted positions.  A group of 2^clog lanes, each with NR packs of VW columns, walks a run
  * of C of them in order, with the rows of the next positions in flight, and stores a row whenever the row number
