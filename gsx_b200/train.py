@@ -87,8 +87,9 @@ class Trainer:
 
     def __init__(self, model: GaussianModel, width: int, height: int, lr: dict | None = None, l1_weight=0.8,
                  ssim_weight=0.2, background=(0.0, 0.0, 0.0), group=None, device="cuda:0", exchange="fused", shared: dict | None = None):
-        """shared: {field: SharedRows}; such a field is written from its table before each render and its table is
-        trained in its place (one GPU only: the exchange covers the fields).
+        """shared: {field: SharedRows}; such a field is written from its table and its table is trained in its place (one
+        GPU only: the exchange covers the fields).  model.params holds the table's rows from here on whenever a call
+        has returned; a table set by hand is seen by the next call that renders or evicts.
         exchange (with a group): "fused" = gsx_b200.dp.ShardedAdam (gradient average + sharded Adam +
         parameter all-gather in one NVLink kernel per rank), through the NVSwitch (multimem reduce-load and
         multicast store) from 4 ranks up where every GPU supports it, else over peer loads and stores;
@@ -116,6 +117,12 @@ class Trainer:
             self._setup_fused(model, group, device, lr, exchange)
         if self.sharded is None:
             self.optim = Adam(self._groups())
+        self._expand_shared()
+
+    def _expand_shared(self):
+        """Every shared field's rows from its table."""
+        for f, rows in self.shared.items():
+            rows.expand(self.model.params[f])
 
     def _groups(self):
         """Adam's parameter groups, one per field of the model (a shared field's table in its place)."""
@@ -160,8 +167,7 @@ class Trainer:
     def gradients(self, camera: Camera, target, events=None):
         """Render TRAIN, fused L1+SSIM, render backward: this rank's gradients in model.flat_grad."""
         m = self.model
-        for f, rows in self.shared.items():
-            rows.expand(m.params[f])
+        self._expand_shared()
         self.renderer.render(self.ctx, m.params, camera, self.out, background=self.background,
                              sh_degree=m.sh_degree, forward_type=FORWARD_TRAIN)
         self.loss_sum.zero_()
@@ -181,8 +187,7 @@ class Trainer:
         that colour, taken with all colours grey so that none is clamped, so it follows the backward's rule and counts
         alphas below 1/255 as well; model.grads is overwritten.)"""
         m = self.model
-        for f, rows in self.shared.items():
-            rows.expand(m.params[f])
+        self._expand_shared()
         grey = dict(m.params, sh0=torch.zeros_like(m.params["sh0"]))
         self.renderer.render(self.ctx, grey, camera, self.out, background=self.background, sh_degree=0,
                              forward_type=FORWARD_TRAIN)
@@ -202,8 +207,7 @@ class Trainer:
         if budget >= m.n:
             return score
         keep, kept = budget_select(score, budget, first=first, recent=recent)
-        for f, rows in self.shared.items():  # the tables may have moved since the last render
-            rows.expand(m.params[f])
+        self._expand_shared()  # a table may have been set since the last call
         before, optim = m.params, self.optim
         m._allocate(int(budget), m.flat_param.device)
         out = torch.empty(m.n, dtype=torch.float32, device=score.device)
@@ -239,6 +243,7 @@ class Trainer:
         self.optim.step(force_all=True)
         if events:
             events[1][1].record()
+        self._expand_shared()  # renders outside of the trainer see this step's tables, not the last one's
         return self.loss_sum
 
     def check_exchange(self, camera: Camera, target) -> dict:

@@ -136,3 +136,31 @@ def test_refusals(cuda_device):
             call()
         assert e.value.code == gb.INVALID_ARGUMENT
         assert m.n == 200
+
+
+def _follows(tr, fields):
+    for f in fields:
+        rows, n = tr.shared[f], tr.model.n
+        assert torch.equal(tr.model.params[f].view(n, -1), rows.table[rows.index.long()] * 0.5), f
+
+
+def _image(tr, cam):
+    out = torch.empty(3, H, W, device="cuda")
+    tr.renderer.render(tr.ctx, tr.model.params, cam, out, sh_degree=tr.model.sh_degree, forward_type=gb.FORWARD_INFERENCE)
+    return out
+
+
+@pytest.mark.parametrize("sh_degree,fields", [(0, ("sh0",)), (1, ("sh0", "sh1"))])
+def test_a_shared_field_follows_its_table(cuda_device, sh_degree, fields):
+    """model.params holds the table's rows whenever a call of the trainer has returned, for renders outside of it."""
+    tr, cam, target = _trainer(sh_degree=sh_degree, fields=fields)
+    _follows(tr, fields)
+    for _ in range(2):
+        tr.step(cam, target)
+        _follows(tr, fields)
+    seen = _image(tr, cam)
+    for f in fields:
+        tr.shared[f].expand(tr.model.params[f])
+    assert torch.equal(seen, _image(tr, cam))
+    tr.keep_budget(torch.rand(tr.model.n, device="cuda"), 700)
+    _follows(tr, fields)
