@@ -198,7 +198,8 @@ class Trainer:
 
     def keep_budget(self, score, budget: int, first: int = 0, recent: int = 0):
         """Drop Gaussians until `budget` are left: the `first` first, the `recent` last (just grown) and the largest
-        scores of the others stay, in order, with their Adam moments and row numbers.  Returns their scores."""
+        scores of the others stay, in order, with their Adam moments and row numbers.  The optimizer and its groups stay
+        the same objects, with every setting.  Returns their scores."""
         m = self.model
         if self.group is not None:
             raise GsxError(NOT_SUPPORTED, "keep_budget runs on one GPU")
@@ -208,7 +209,9 @@ class Trainer:
             return score
         keep, kept = budget_select(score, budget, first=first, recent=recent)
         self._expand_shared()  # a table may have been set since the last call
-        before, optim = m.params, self.optim
+        optim = self.optim
+        before = m.params
+        role = {p.data_ptr(): f for f, p in before.items()}
         m._allocate(int(budget), m.flat_param.device)
         out = torch.empty(m.n, dtype=torch.float32, device=score.device)
         gather = [(score, out)] + [(before[f], m.params[f]) for f in m.fields]
@@ -216,13 +219,15 @@ class Trainer:
             index = torch.empty(m.n, dtype=rows.index.dtype, device=rows.index.device)
             gather.append((rows.index, index))
             rows.index = index
-        self.optim = Adam(self._groups())
-        self.optim.steps = list(optim.steps)
-        for i, f in enumerate(m.fields):
-            if f in self.shared:
-                self.optim.m1[i], self.optim.m2[i] = optim.m1[i], optim.m2[i]
-            else:
-                gather += [(optim.m1[i], self.optim.m1[i]), (optim.m2[i], self.optim.m2[i])]
+        for i, g in enumerate(optim.groups):
+            f = role.get(g.parameter.data_ptr())
+            if f is None:  # a shared field's table
+                continue
+            g.parameter, g.gradient = m.params[f], m.grads[f]
+            for moments in (optim.m1, optim.m2):
+                new = torch.empty_like(g.parameter)
+                gather.append((moments[i], new))
+                moments[i] = new
         budget_gather(gather, keep, kept)
         return out
 

@@ -1,5 +1,7 @@
 """Shared rows and the budget where the trainer uses them: lookup before the render, the table's gradient after its
 backward, Adam on the table; blend weights accumulated over views, eviction to a budget, training on."""
+import dataclasses
+
 import numpy as np
 import pytest
 import torch
@@ -164,3 +166,51 @@ def test_a_shared_field_follows_its_table(cuda_device, sh_degree, fields):
     assert torch.equal(seen, _image(tr, cam))
     tr.keep_budget(torch.rand(tr.model.n, device="cuda"), 700)
     _follows(tr, fields)
+
+
+def test_an_eviction_keeps_the_optimizer_and_its_settings(cuda_device):
+    tr, cam, target = _trainer(n=900, fields=("sh0",))
+    tr.step(cam, target)
+    optim, groups = tr.optim, list(tr.optim.groups)
+    for i, g in enumerate(groups):
+        g.learning_rate = 1e-4 * (i + 1)
+        g.beta1, g.beta2, g.weight_decay, g.epsilon, g.max_grad = 0.8, 0.99, 0.01, 1e-6, 0.5
+    tr.keep_budget(torch.rand(900, device="cuda"), 300)
+    assert tr.optim is optim and all(a is b for a, b in zip(optim.groups, groups))
+    m = tr.model
+    for i, (f, g) in enumerate(zip(m.fields, groups)):
+        assert g.role == f and g.learning_rate == 1e-4 * (i + 1)
+        assert (g.beta1, g.beta2, g.weight_decay, g.epsilon, g.max_grad) == (0.8, 0.99, 0.01, 1e-6, 0.5)
+        if f != "sh0":
+            assert g.parameter.data_ptr() == m.params[f].data_ptr() and g.gradient.data_ptr() == m.grads[f].data_ptr()
+            assert optim.m1[i].shape == optim.m2[i].shape == m.params[f].shape
+    tr.gradients(cam, target)
+    alone = gb.Adam([dataclasses.replace(g, parameter=g.parameter.clone()) for g in groups])
+    alone.steps = list(optim.steps)
+    for i in range(len(groups)):
+        alone.m1[i].copy_(optim.m1[i])
+        alone.m2[i].copy_(optim.m2[i])
+    alone.step()
+    tr.update()
+    for a, b in zip(alone.groups, groups):
+        assert torch.equal(a.parameter, b.parameter), b.role
+
+
+def test_an_eviction_with_an_optimizer_of_some_fields(cuda_device):
+    """The caller's own Adam, over a few fields in any order: its moments go with their Gaussians."""
+    tr, cam, target = _trainer(n=900, fields=("sh0",))
+    m = tr.model
+    tr.optim = gb.Adam([gb.ParamGroup("opacity", m.params["opacity"], m.grads["opacity"], 1e-2),
+                        gb.ParamGroup("sh0", tr.shared["sh0"].table, tr.shared["sh0"].grad, 1e-2),
+                        gb.ParamGroup("mean3d", m.params["mean3d"], m.grads["mean3d"], 1e-3)])
+    tr.step(cam, target)
+    m1 = [t.clone() for t in tr.optim.m1]
+    old = {f: v.clone() for f, v in m.params.items()}
+    score = torch.arange(900, device="cuda").float()  # the last 300 stay
+    tr.keep_budget(score, 300)
+    for f in m.fields:
+        assert torch.equal(m.params[f], old[f][600:])
+    assert torch.equal(tr.optim.m1[0], m1[0][600:]) and torch.equal(tr.optim.m1[1], m1[1]) and torch.equal(tr.optim.m1[2], m1[2][600:])
+    before = m.params["logscale"].clone()
+    tr.step(cam, target)
+    assert torch.equal(m.params["logscale"], before) and not torch.equal(m.params["mean3d"], old["mean3d"][600:])
