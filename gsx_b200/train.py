@@ -57,6 +57,17 @@ class GaussianModel:
             self.params[f] = self.flat_param[a:a + c].view(shape)
             self.grads[f] = self.flat_grad[a:a + c].view(shape)
 
+    def sized(self, n: int):
+        """A model of n Gaussians with the same fields, all zero."""
+        other = GaussianModel.__new__(GaussianModel)
+        other.sh_degree, other.fields = self.sh_degree, self.fields
+        other._allocate(n, self.flat_param.device)
+        return other
+
+    def become(self, other):
+        """Take over another model's tensors and layout."""
+        vars(self).update(vars(other))
+
     def rebind(self, flat_param, flat_grad):
         """Move the parameters into other flat buffers (e.g. ones mapped into the peer ranks)."""
         flat_param.copy_(self.flat_param)
@@ -199,7 +210,7 @@ class Trainer:
     def keep_budget(self, score, budget: int, first: int = 0, recent: int = 0):
         """Drop Gaussians until `budget` are left: the `first` first, the `recent` last (just grown) and the largest
         scores of the others stay, in order, with their Adam moments and row numbers.  The optimizer and its groups stay
-        the same objects, with every setting.  Returns their scores."""
+        the same objects, with every setting.  Where it fails, nothing has changed.  Returns their scores."""
         m = self.model
         if self.group is not None:
             raise GsxError(NOT_SUPPORTED, "keep_budget runs on one GPU")
@@ -209,26 +220,27 @@ class Trainer:
             return score
         keep, kept = budget_select(score, budget, first=first, recent=recent)
         self._expand_shared()  # a table may have been set since the last call
+        # all of the new state is made and filled beside the old, and takes its place when nothing can fail any more
+        new = m.sized(int(budget))
+        out = torch.empty(new.n, dtype=torch.float32, device=score.device)
+        gather = [(score, out)] + [(m.params[f], new.params[f]) for f in m.fields]
+        index = {f: torch.empty(new.n, dtype=rows.index.dtype, device=rows.index.device) for f, rows in self.shared.items()}
+        gather += [(rows.index, index[f]) for f, rows in self.shared.items()]
         optim = self.optim
-        before = m.params
-        role = {p.data_ptr(): f for f, p in before.items()}
-        m._allocate(int(budget), m.flat_param.device)
-        out = torch.empty(m.n, dtype=torch.float32, device=score.device)
-        gather = [(score, out)] + [(before[f], m.params[f]) for f in m.fields]
-        for rows in self.shared.values():
-            index = torch.empty(m.n, dtype=rows.index.dtype, device=rows.index.device)
-            gather.append((rows.index, index))
-            rows.index = index
-        for i, g in enumerate(optim.groups):
-            f = role.get(g.parameter.data_ptr())
-            if f is None:  # a shared field's table
-                continue
-            g.parameter, g.gradient = m.params[f], m.grads[f]
-            for moments in (optim.m1, optim.m2):
-                new = torch.empty_like(g.parameter)
-                gather.append((moments[i], new))
-                moments[i] = new
+        field = {p.data_ptr(): f for f, p in m.params.items()}
+        field = [field.get(g.parameter.data_ptr()) for g in optim.groups]  # None: a shared field's table
+        moments = [None if f is None else (torch.empty_like(new.params[f]), torch.empty_like(new.params[f])) for f in field]
+        for i, pair in enumerate(moments):
+            if pair is not None:
+                gather += [(optim.m1[i], pair[0]), (optim.m2[i], pair[1])]
         budget_gather(gather, keep, kept)
+        m.become(new)
+        for f, rows in self.shared.items():
+            rows.index = index[f]
+        for i, g in enumerate(optim.groups):
+            if moments[i] is not None:
+                g.parameter, g.gradient = m.params[field[i]], m.grads[field[i]]
+                optim.m1[i], optim.m2[i] = moments[i]
         return out
 
     def update(self, events=None):

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import gsx_b200 as gb
-from gsx_b200 import scenes
+from gsx_b200 import scenes, train
 from gsx_b200.train import GaussianModel, SharedRows, Trainer
 from oracle import pyoracle as po
 
@@ -214,3 +214,28 @@ def test_an_eviction_with_an_optimizer_of_some_fields(cuda_device):
     before = m.params["logscale"].clone()
     tr.step(cam, target)
     assert torch.equal(m.params["logscale"], before) and not torch.equal(m.params["mean3d"], old["mean3d"][600:])
+
+
+@pytest.mark.parametrize("where", ["_allocate", "budget_gather"])
+def test_an_eviction_that_fails_changes_nothing(cuda_device, monkeypatch, where):
+    """Out of memory, or a refused gather: the model, its optimizer and the row numbers stay as they were."""
+    tr, cam, target = _trainer(n=900, fields=("sh0",))
+    tr.step(cam, target)
+    m, rows = tr.model, tr.shared["sh0"]
+    held = [m.flat_param, m.flat_grad, *m.params.values(), *m.grads.values(), *tr.optim.m1, *tr.optim.m2, rows.index, rows.table]
+    copies = [t.clone() for t in held]
+    layout = (m.n, m.numel, dict(m.offsets), dict(m.field_ranges), list(tr.optim.steps))
+
+    def fail(*args, **kw):
+        raise torch.OutOfMemoryError("no memory")
+
+    with monkeypatch.context() as patch:
+        patch.setattr(train.GaussianModel, where, fail) if where == "_allocate" else patch.setattr(train, where, fail)
+        with pytest.raises(torch.OutOfMemoryError):
+            tr.keep_budget(torch.rand(900, device="cuda"), 300)
+    now = [m.flat_param, m.flat_grad, *m.params.values(), *m.grads.values(), *tr.optim.m1, *tr.optim.m2, rows.index, rows.table]
+    assert all(a is b for a, b in zip(held, now)) and all(torch.equal(a, b) for a, b in zip(copies, now))
+    assert layout == (m.n, m.numel, m.offsets, m.field_ranges, tr.optim.steps)
+    tr.step(cam, target)
+    tr.keep_budget(torch.rand(900, device="cuda"), 300)
+    assert m.n == 300 and bool(torch.isfinite(tr.step(cam, target)).all())
