@@ -78,7 +78,8 @@ class GaussianModel:
 class SharedRows:
     """A field whose rows many Gaussians share (a codebook of colours or of higher-order coefficients): the field is
     scale * table[index], the trained parameter is the table ([rows, columns of the field], f32), index is one int32
-    or int64 row number per Gaussian."""
+    or int64 row number per Gaussian.  Each field has rows of its own, whose table overlaps no other's; index may be the
+    same tensor for several."""
 
     def __init__(self, table, index, scale: float = 1.0):
         self.table, self.index, self.scale = table, index, float(scale)
@@ -122,6 +123,12 @@ class Trainer:
         for f, rows in self.shared.items():
             if f not in model.fields or rows.table.dtype != torch.float32 or rows.index.shape != (model.n,):
                 raise GsxError(NOT_SUPPORTED, "shared rows need a field of the model, a float32 table and an index per Gaussian")
+            if not rows.table.is_contiguous():
+                raise GsxError(INVALID_ARGUMENT, f"the table of {f} must be contiguous")
+        # two groups of one Adam launch over the same memory would race, and each backward would overwrite the other's gradient
+        spans = sorted((r.table.data_ptr(), r.table.data_ptr() + r.table.numel() * 4) for r in self.shared.values())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])) or len({id(r) for r in self.shared.values()}) < len(self.shared):
+            raise GsxError(INVALID_ARGUMENT, "shared rows serve one field each, and their tables must not overlap")
         self.sharded = None
         self.exchange = "nccl" if group is not None else None
         if group is not None and exchange in ("fused", "nvls", "peer"):

@@ -239,3 +239,23 @@ def test_an_eviction_that_fails_changes_nothing(cuda_device, monkeypatch, where)
     tr.step(cam, target)
     tr.keep_budget(torch.rand(900, device="cuda"), 300)
     assert m.n == 300 and bool(torch.isfinite(tr.step(cam, target)).all())
+
+
+def test_a_table_serves_one_field(cuda_device):
+    """Two groups of one Adam launch over the same table would race; the row numbers may be shared."""
+    tr, _, _ = _trainer(n=300, fields=())
+    m = tr.model
+    table = torch.randn(20, 3, device="cuda")
+    index = torch.randint(0, 10, (300,), device="cuda")
+    rows = SharedRows(table, index)
+    for other in (rows, SharedRows(table, index), SharedRows(table[10:], index), SharedRows(table[:10].view(10, 3), index.clone())):
+        with pytest.raises(gb.GsxError) as e:
+            Trainer(m, W, H, shared={"sh0": rows, "logscale": other})
+        assert e.value.code == gb.INVALID_ARGUMENT
+    two = Trainer(m, W, H, shared={"sh0": SharedRows(table[:10], index), "logscale": SharedRows(table[10:], index)})
+    two.keep_budget(torch.arange(300, device="cuda").float(), 50)
+    for rows in two.shared.values():
+        assert torch.equal(rows.index, index[250:])
+    with pytest.raises(gb.GsxError) as e:  # Adam walks a table as one array
+        Trainer(two.model, W, H, shared={"sh0": SharedRows(torch.randn(3, 20, device="cuda").t(), index[:50].clone())})
+    assert e.value.code == gb.INVALID_ARGUMENT
