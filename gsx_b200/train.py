@@ -11,7 +11,8 @@ from __future__ import annotations
 import numpy as np
 import torch
 
-from . import FORWARD_TRAIN, INVALID_ARGUMENT, NOT_SUPPORTED, Adam, Camera, GsxError, ParamGroup, RenderContext, Renderer, l1_ssim
+from . import (FORWARD_TRAIN, INVALID_ARGUMENT, NOT_SUPPORTED, OUT_OF_RANGE, Adam, Camera, GsxError, ParamGroup,
+               RenderContext, Renderer, l1_ssim)
 from .budget import budget_accumulate, budget_gather, budget_select
 from .embedding import embedding_backward, embedding_lookup
 
@@ -84,10 +85,18 @@ class SharedRows:
     def __init__(self, table, index, scale: float = 1.0):
         self.table, self.index, self.scale = table, index, float(scale)
         self.grad = torch.empty_like(table)
+        self.bad = torch.zeros(1, dtype=torch.int32, device=table.device)  # set by a row number outside the table
 
     def expand(self, field):
         """Write the field's rows ([N, ..] f32) from the table."""
-        embedding_lookup(self.table, self.index, out=field.view(field.shape[0], -1), scale=self.scale)
+        embedding_lookup(self.table, self.index, out=field.view(field.shape[0], -1), scale=self.scale, bad=self.bad)
+
+    def check(self):
+        """Synchronise and raise if an expand since the last check met a row number outside the table (such a Gaussian
+        keeps its row, and its gradient is dropped)."""
+        if int(self.bad):
+            self.bad.zero_()
+            raise GsxError(OUT_OF_RANGE, "a row number lies outside the table")
 
     def reduce(self, field_grad):
         """The table's gradient from the field's, summed by row."""
@@ -102,6 +111,7 @@ class Trainer:
         """shared: {field: SharedRows}; such a field is written from its table and its table is trained in its place (one
         GPU only: the exchange covers the fields).  model.params holds the table's rows from here on whenever a call
         has returned; a table set by hand is seen by the next call that renders or evicts.
+        Row numbers outside their table are refused here; ones set later show in SharedRows.check.
         exchange (with a group): "fused" = gsx_b200.dp.ShardedAdam (gradient average + sharded Adam +
         parameter all-gather in one NVLink kernel per rank), through the NVSwitch (multimem reduce-load and
         multicast store) from 4 ranks up where every GPU supports it, else over peer loads and stores;
@@ -136,6 +146,11 @@ class Trainer:
         if self.sharded is None:
             self.optim = Adam(self._groups())
         self._expand_shared()
+        for f, rows in self.shared.items():
+            try:
+                rows.check()
+            except GsxError as e:
+                raise GsxError(e.code, f"{f}: {e.message}") from None
 
     def _expand_shared(self):
         """Every shared field's rows from its table."""

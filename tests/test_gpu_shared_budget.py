@@ -259,3 +259,29 @@ def test_a_table_serves_one_field(cuda_device):
     with pytest.raises(gb.GsxError) as e:  # Adam walks a table as one array
         Trainer(two.model, W, H, shared={"sh0": SharedRows(torch.randn(3, 20, device="cuda").t(), index[:50].clone())})
     assert e.value.code == gb.INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_row_numbers_outside_the_table_are_reported(cuda_device, dtype):
+    tr, cam, target = _trainer(n=300, fields=())
+    table = torch.randn(20, 3, device="cuda")
+    fine = torch.randint(0, 20, (300,), device="cuda", dtype=dtype)
+    for number in (20, -1, 2 ** 31 - 1):
+        index = fine.clone()
+        index[7] = number
+        with pytest.raises(gb.GsxError) as e:
+            Trainer(tr.model, W, H, shared={"sh0": SharedRows(table, index)})
+        assert e.value.code == gb.OUT_OF_RANGE and "sh0" in str(e.value)
+    rows = SharedRows(table, fine)
+    tr = Trainer(tr.model, W, H, shared={"sh0": rows})
+    tr.step(cam, target)
+    rows.check()
+    rows.index[299] = 20  # changed while training: reported by the next check, once
+    tr.step(cam, target)
+    with pytest.raises(gb.GsxError) as e:
+        rows.check()
+    assert e.value.code == gb.OUT_OF_RANGE
+    rows.check()
+    rows.index[299] = 0
+    tr.step(cam, target)
+    rows.check()
