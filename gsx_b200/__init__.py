@@ -85,6 +85,7 @@ class RenderContext:
         check(lib().gsx_b200_context_create(device, ctypes.byref(h)))
         self.handle = h
         self._keep = None
+        self.aux = (None,) * 4  # the accumulators that bind_aux has bound
 
     def close(self):
         if self.handle:
@@ -110,9 +111,9 @@ class RenderContext:
     def bind_aux(self, visible_counter=None, max_screen_radius=None, grad_acc=None, absgrad_acc=None):
         """Bind the [N] f32 density-control accumulators (None = unbound) for later TRAIN renders
         (visible_counter, max_screen_radius) and backwards (grad_acc, absgrad_acc)."""
-        self._aux = (visible_counter, max_screen_radius, grad_acc, absgrad_acc)
-        check(lib().gsx_b200_render_bind_aux(self.handle, _ptr(visible_counter), _ptr(max_screen_radius),
-                                             _ptr(grad_acc), _ptr(absgrad_acc)))
+        aux = (visible_counter, max_screen_radius, grad_acc, absgrad_acc)
+        check(lib().gsx_b200_render_bind_aux(self.handle, *(_ptr(t) for t in aux)))
+        self.aux = aux
 
     def set_train_state(self, borrowed: bool):
         """False (default): the TRAIN forward's state is retained and the caller must not change the

@@ -218,21 +218,29 @@ class Trainer:
         """score ([N] f32) = decay * score + the blend weight of every Gaussian in this view: the sum over the pixels of
         alpha times transmittance, with which its colour enters them.  (It is the gradient of the sum of the image by
         that colour, taken with all colours grey so that none is clamped, so it follows the backward's rule and counts
-        alphas below 1/255 as well; model.grads is overwritten.)"""
+        alphas below 1/255 as well; model.grads is overwritten.)  Density statistics bound to the context are left alone."""
         m = self.model
         self._expand_shared()
         grey = dict(m.params, sh0=torch.zeros_like(m.params["sh0"]))
-        self.renderer.render(self.ctx, grey, camera, self.out, background=self.background, sh_degree=0,
-                             forward_type=FORWARD_TRAIN)
-        self.grad_rgb.zero_()
-        self.grad_rgb[0] = 1.0 / SH_C0
-        self.renderer.backward(self.ctx, self.grad_rgb, m.grads)
+        bound = self.ctx.aux  # this is no training view
+        if any(t is not None for t in bound):
+            self.ctx.bind_aux()
+        try:
+            self.renderer.render(self.ctx, grey, camera, self.out, background=self.background, sh_degree=0,
+                                 forward_type=FORWARD_TRAIN)
+            self.grad_rgb.zero_()
+            self.grad_rgb[0] = 1.0 / SH_C0
+            self.renderer.backward(self.ctx, self.grad_rgb, m.grads)
+        finally:
+            if any(t is not None for t in bound):
+                self.ctx.bind_aux(*bound)
         return budget_accumulate(score, m.grads["sh0"][:, 0].contiguous().view(1, -1), decay=decay)
 
     def keep_budget(self, score, budget: int, first: int = 0, recent: int = 0):
         """Drop Gaussians until `budget` are left: the `first` first, the `recent` last (just grown) and the largest
         scores of the others stay, in order, with their Adam moments and row numbers.  The optimizer and its groups stay
-        the same objects, with every setting.  Where it fails, nothing has changed.  Returns their scores."""
+        the same objects, with every setting.  Where it fails, nothing has changed.  Density statistics bound to the context
+        still have a place per Gaussian from before: bind new ones.  Returns the scores that stay."""
         m = self.model
         if self.group is not None:
             raise GsxError(NOT_SUPPORTED, "keep_budget runs on one GPU")

@@ -285,3 +285,16 @@ def test_row_numbers_outside_the_table_are_reported(cuda_device, dtype):
     rows.index[299] = 0
     tr.step(cam, target)
     rows.check()
+
+
+def test_blend_weights_leave_the_density_statistics_alone(cuda_device):
+    """Its render and backward are no training view: statistics that the context has bound see neither, and stay bound."""
+    tr, cam, target = _trainer(n=800, fields=("sh0",))
+    stats = [torch.full((800,), 3.0, device="cuda") for _ in range(4)]
+    tr.ctx.bind_aux(*stats)
+    tr.blend_weights(cam, torch.zeros(800, device="cuda"))
+    assert all(bool((t == 3.0).all()) for t in stats)
+    tr.step(cam, target)
+    assert all(bool((t != 3.0).any()) for t in stats)
+    tr.ctx.bind_aux()
+    tr.blend_weights(cam, torch.zeros(800, device="cuda"))
