@@ -22,6 +22,7 @@
 
 #include "../../include/gsx_b200.h"
 #include "gsx_b200_kernels.cuh"
+#include "gsx_spans.h"
 
 int gsx_internal_fail(int code, const char *msg);
 
@@ -1053,6 +1054,23 @@ extern "C" int gsx_b200_budget_select(const float *score, uint64_t score_stride,
     const uint64_t most = budget < length ? budget : length;
     if(groups > 1 && (score_stride < length || keep_stride < most || (drop != nullptr && drop_stride < length)))
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "strides must cover a group's entries");
+    if(groups > 1 && (score_stride > (1ull << 40) || keep_stride > (1ull << 40) || (drop != nullptr && drop_stride > (1ull << 40))))
+        return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "strides must be at most 2^40 elements");
+    const uint64_t need = gsx_b200_budget_workspace_bytes(groups, length);
+    /* scores and lengths are read again while the lists are written: by other CTAs of a group, and in the long form by every step */
+    const GsxRows written[] = { { keep, 4 * most, { { groups, 4 * keep_stride } } },
+                                { drop, length > budget ? 4 * (length - budget) : 0, { { groups, 4 * drop_stride } } },
+                                { kept, 4 * groups },
+                                { workspace, need } };
+    const GsxRows read[] = { { score, 4 * length, { { groups, 4 * score_stride } } }, { lengths, 4 * groups } };
+    for(int i = 0; i < 4; ++i) {
+        for(const GsxRows &r : read)
+            if(gsx_rows_meet(written[i], r))
+                return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "keep, kept, drop and workspace must not overlap score or lengths");
+        for(int j = 0; j < i; ++j)
+            if(gsx_rows_meet(written[i], written[j]))
+                return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "keep, kept, drop and workspace must not overlap one another");
+    }
     cudaStream_t stream = (cudaStream_t)stream_;
     Select a;
     a.score = score;
@@ -1092,7 +1110,6 @@ extern "C" int gsx_b200_budget_select(const float *score, uint64_t score_stride,
         cfg.numAttrs = 1;
         return launch_status(cudaLaunchKernelEx(&cfg, select_cluster_kernel, a));
     }
-    const uint64_t need = gsx_b200_budget_workspace_bytes(groups, length);
     if(workspace == nullptr || (uintptr_t)workspace % 4 || workspace_bytes < need)
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "workspace must hold gsx_b200_budget_workspace_bytes bytes");
     Long w;

@@ -439,6 +439,8 @@ GSX_B200_API int gsx_b200_embedding_backward(const void *grad_out, int grad_type
  *   budget - first - recent with the largest scores, ties to the lowest index, NaN below every number, -0 equal
  *   to +0.  kept[g] = min(entries in use, budget).  drop (may be NULL) receives the other entries, in increasing
  *   order: those in use less kept[g].  Places of keep and drop behind the lists are left as they were.
+ *   keep, kept, drop and workspace must overlap neither one another nor score and lengths (kept is not lengths
+ *   updated in place: other blocks still read those).
  *   workspace: gsx_b200_budget_workspace_bytes(groups, length) bytes of device memory, 4-byte aligned, of any
  *   content (0 bytes for groups of up to 131072 entries); calls that overlap on the GPU need one each.
  * gsx_b200_budget_gather: for every field and group, row r of dst = row keep[g, r] of src for r < kept[g]; later
