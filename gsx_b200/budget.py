@@ -126,7 +126,8 @@ def budget_gather(fields, keep, kept, bad=None, stream=None):
     """Row r of dst = row keep[.., r] of src for r < kept[..], for every (src, dst) pair of `fields` (up to 32) in
     one launch.  keep is [budget], [heads, budget] or [batch, heads, budget]; src is its leading shape + (length,) +
     any row shape, dst the same with at least `budget` rows; both may be strided in all but the row, so a cache may
-    be a transposed view.  Rows of dst behind kept are left as they were."""
+    be a transposed view.  Rows of dst behind kept are left as they were.  No dst may overlap a src, keep, kept or bad,
+    and no row of a dst another one; several may interleave in one buffer."""
     lead = keep.shape[:-1]
     if keep.dim() < 1 or len(lead) > 2 or keep.dtype != torch.int32 or not keep.is_contiguous():
         raise invalid("keep must be a contiguous int32 tensor of one to three dimensions")

@@ -20,6 +20,7 @@ struct GsxRows {
     bool empty;
     static constexpr uint64_t kMost = 1ull << 62; /* longer steps and extents count as this, so that no sum wraps */
 
+    GsxRows() : at(0), bytes(0), dims(0), empty(true) {}
     GsxRows(const void *p, uint64_t row_bytes, std::initializer_list<Dim> all = {}) : at((int64_t)(uintptr_t)p), bytes(row_bytes), dims(0)
     {
         empty = p == nullptr || row_bytes == 0;

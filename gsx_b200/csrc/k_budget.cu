@@ -1150,6 +1150,10 @@ extern "C" int gsx_b200_budget_gather(const gsx_b200_gather_field *fields, int32
     if((uintptr_t)keep % 4 || (uintptr_t)kept % 4) return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "pointers must be aligned to 4 bytes");
     if(outer * inner > 1 && keep_stride < budget)
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "keep_stride must be at least budget");
+    if(outer * inner > 1 && keep_stride > (1ull << 40)) return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "keep_stride must be at most 2^40 elements");
+    const GsxRows lists[] = { { keep, 4 * budget, { { outer * inner, 4 * keep_stride } } },
+                              { kept, 4 * outer * inner },
+                              { device_out_of_range, 4 } };
     Fields t;
     t.count = 0;
     uint64_t blocks = 0;
@@ -1157,6 +1161,7 @@ extern "C" int gsx_b200_budget_gather(const gsx_b200_gather_field *fields, int32
         const void *p;
         uint64_t bytes;
     } src_span[GSX_B200_GATHER_MAX_FIELDS], dst_span[GSX_B200_GATHER_MAX_FIELDS];
+    GsxRows dst_rows[GSX_B200_GATHER_MAX_FIELDS];
     for(int i = 0; i < field_count; ++i) {
         const gsx_b200_gather_field &in = fields[i];
         if(in.row_bytes == 0) continue;
@@ -1199,10 +1204,19 @@ extern "C" int gsx_b200_budget_gather(const gsx_b200_gather_field *fields, int32
         if(blocks > (uint64_t)INT32_MAX) return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "too many rows in one call");
         src_span[t.count] = { in.src, length == 0 ? 0 : (outer - 1) * f.src_outer + (inner - 1) * f.src_inner + (length - 1) * (uint64_t)f.src_row + f.row_bytes };
         dst_span[t.count] = { in.dst, (outer - 1) * f.dst_outer + (inner - 1) * f.dst_inner + (budget - 1) * (uint64_t)f.dst_row + f.row_bytes };
+        dst_rows[t.count] = GsxRows(in.dst, in.row_bytes, { { outer, f.dst_outer }, { inner, f.dst_inner }, { budget, f.dst_row } });
+        if(!dst_rows[t.count].nested())
+            return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "the rows and groups of a field's dst must not overlap");
+        for(const GsxRows &r : lists)
+            if(gsx_rows_meet(dst_rows[t.count], r))
+                return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "a field's dst must not overlap keep, kept or the flag");
         ++t.count;
     }
     for(int i = 0; i < t.count; ++i)
         for(int j = 0; j < t.count; ++j) {
+            /* keys and values may interleave in one buffer: rows, not spans */
+            if(j < i && gsx_rows_meet(dst_rows[i], dst_rows[j]))
+                return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "a field's dst must not overlap another's");
             if(overlap(src_span[i].p, src_span[i].bytes, dst_span[j].p, dst_span[j].bytes))
                 return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "a field's dst must not overlap any field's src");
         }

@@ -448,7 +448,8 @@ GSX_B200_API int gsx_b200_embedding_backward(const void *grad_out, int grad_type
  *   outer and inner strides (caches of [batch, head, entry] and [batch, entry, head] order alike).  A keep entry
  *   outside [0, length) sets *device_out_of_range to 1 (when non-NULL) and leaves its row untouched.  keep holds
  *   `budget` places a group, of any content behind kept[g], and need not be in order.  No field's dst may overlap any
- *   field's src, or another's dst.
+ *   field's src (by address range), and no row of a dst another row of any dst, keep, kept or the flag; dst may interleave
+ *   in one buffer, each group's rows within the step to the next (or each row's groups).
  */
 #define GSX_B200_GATHER_MAX_FIELDS 32
 typedef struct gsx_b200_gather_field {

@@ -393,3 +393,32 @@ def test_refusals(cuda_device):
     refused(gb.NOT_SUPPORTED, gb.budget_gather, [(src, dst.half())], keep, kept)
     refused(gb.OUT_OF_RANGE, gb.budget_gather, [(src, dst)] * 33, keep, kept)
     refused(bad, gb.budget_gather, [(src, dst)], keep.long(), kept)
+
+
+@pytest.mark.parametrize("kind", ["entry by entry", "head by head", "rows of two sizes"])
+def test_gather_into_one_interleaved_buffer(cuda_device, kind):
+    """Keys and values that share a buffer: their spans overlap, their rows do not."""
+    g = _gen(18)
+    B, H, S, budget = 2, 3, 100, 40
+    if kind == "entry by entry":
+        buf = torch.full((B, budget + 1, 2, H, 64), 7.0, device="cuda")
+        k2, v2 = buf[:, :, 0].transpose(1, 2), buf[:, :, 1].transpose(1, 2)
+    elif kind == "head by head":
+        buf = torch.full((B, H, 2 * budget + 3, 64), 7.0, device="cuda")
+        k2, v2 = buf[:, :, :budget], buf[:, :, budget + 3:]
+    else:
+        buf = torch.full((B, H, budget * 80 + 5), 7.0, device="cuda")
+        k2 = buf.as_strided((B, H, budget, 64), (H * (budget * 80 + 5), budget * 80 + 5, 64, 1), 0)
+        v2 = buf.as_strided((B, H, budget, 16), (H * (budget * 80 + 5), budget * 80 + 5, 16, 1), budget * 64)
+    k = torch.randn(B, H, S, k2.shape[-1], generator=g, device="cuda")
+    v = torch.randn(B, H, S, v2.shape[-1], generator=g, device="cuda")
+    keep, kept = gb.budget_select(torch.rand(B, H, S, generator=g, device="cuda"), budget)
+    gb.budget_gather([(k, k2), (v, v2)], keep, kept)
+    at = keep.long()[..., None]
+    assert torch.equal(k2[:, :, :budget], torch.gather(k, 2, at.expand(-1, -1, -1, k.shape[-1])))
+    assert torch.equal(v2[:, :, :budget], torch.gather(v, 2, at.expand(-1, -1, -1, v.shape[-1])))
+    assert int((buf != 7.0).sum()) == k2[:, :, :budget].numel() + v2[:, :, :budget].numel()
+    for bad in ([(k, k2), (k, k2)], [(k, k2[:, :1].expand(B, H, k2.shape[2], k2.shape[3]))]):
+        with pytest.raises(gb.GsxError) as e:
+            gb.budget_gather(bad, keep, kept)
+        assert e.value.code == gb.INVALID_ARGUMENT

@@ -104,3 +104,32 @@ def test_select_refuses_overlaps(kw):
 @pytest.mark.parametrize("kw", [dict(sstride=2 ** 41), dict(kstride=2 ** 41), dict(drop=5 * MB, dstride=2 ** 41)])
 def test_select_refuses_strides_out_of_range(kw):
     assert _select(**kw) == gb.OUT_OF_RANGE
+
+
+def _gather(*fields, outer=1, inner=1, length=16, budget=8, keep=MB, kstride=8, kept=2 * MB, bad=None):
+    base = dict(src=64 * MB, dst=4 * MB, row_bytes=12, src_row_stride=12, dst_row_stride=12)
+    table = (_capi.GatherField * len(fields))(*[_capi.GatherField(**dict(base, **f)) for f in fields])
+    return _capi.lib().gsx_b200_budget_gather(table, len(fields), outer, inner, length, budget, keep, kstride, kept, bad, None)
+
+
+GATHER = [([{}, {}], {}), ([{}, dict(dst=4 * MB + 92)], {}), ([{}, dict(dst=4 * MB - 92)], {}),
+          ([dict(dst_inner_stride=0)], dict(inner=2)), ([dict(dst_inner_stride=84)], dict(inner=2)),
+          ([dict(dst_outer_stride=0, dst_inner_stride=96)], dict(outer=2, inner=3)),
+          ([dict(dst_outer_stride=200, dst_inner_stride=96)], dict(outer=2, inner=3)),
+          ([dict(dst_row_stride=24, dst_inner_stride=8)], dict(inner=2)),
+          ([dict(dst=MB + 28)], {}), ([dict(dst=MB - 92)], {}), ([dict(dst=2 * MB)], {}), ([dict(dst=2 * MB - 92)], {}),
+          ([dict(dst=5 * MB - 92)], dict(bad=5 * MB)), ([{}], dict(inner=2, keep=4 * MB + 100)),
+          ([dict(dst_row_stride=32), dict(dst=4 * MB + 8, dst_row_stride=32)], {}),
+          ([dict(dst_row_stride=32), dict(dst=4 * MB + 224 + 8, dst_row_stride=24)], {})]
+
+
+@pytest.mark.parametrize("fields,kw", GATHER)
+def test_gather_refuses_overlaps(fields, kw):
+    inner = kw.get("inner", 1)
+    fields = [dict(dict(dst_inner_stride=96) if inner > 1 else {}, **f) for f in fields]
+    assert _gather(*fields, **kw) == gb.INVALID_ARGUMENT
+    assert b"overlap" in _capi.lib().gsx_b200_last_error()
+
+
+def test_gather_refuses_strides_out_of_range():
+    assert _gather(dict(dst_inner_stride=96), inner=2, kstride=2 ** 41) == gb.OUT_OF_RANGE
