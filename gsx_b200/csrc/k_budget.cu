@@ -1016,6 +1016,9 @@ extern "C" int gsx_b200_budget_accumulate(const float *score, uint64_t score_str
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "out must be score itself or not overlap it");
     if(rows > 0 && overlap(out, out_bytes, weights, es * ((groups - 1) * group_stride + (rows - 1) * row_stride + length)))
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "out must not overlap weights");
+    const GsxRows written(out, 4 * length, { { groups, 4 * out_stride } });
+    if(gsx_rows_meet(written, { lengths, 4 * groups }) || gsx_rows_meet(written, { row_lengths, 4 * groups }))
+        return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "out must not overlap lengths or row_lengths");
     cudaStream_t stream = (cudaStream_t)stream_;
     const uint64_t all = (uint64_t)(uintptr_t)weights | length * es | (groups > 1 ? group_stride * es : 0) | (rows > 1 ? row_stride * es : 0);
     uint64_t unit = 16;

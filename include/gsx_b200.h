@@ -433,7 +433,7 @@ GSX_B200_API int gsx_b200_embedding_backward(const void *grad_out, int grad_type
  * gsx_b200_budget_accumulate: out[g, j] = decay * score[g, j] + sum over r < row_lengths[g] (NULL: all `rows`) of
  *   weights[g, r, j] for the entries in use (f32 sums in a fixed order); decay 0 does not read their scores.
  *   Entries behind lengths[g] are copied from score.  out may be score itself, or must not overlap it; it must
- *   not overlap weights.
+ *   not overlap weights, lengths or row_lengths.
  * gsx_b200_budget_select: keep[g, 0 .. kept[g]) receives, in increasing order, the entries that stay: all of them
  *   when the group uses at most `budget`, else the `first` first, the `recent` last, and of the others the
  *   budget - first - recent with the largest scores, ties to the lowest index, NaN below every number, -0 equal

@@ -133,3 +133,15 @@ def test_gather_refuses_overlaps(fields, kw):
 
 def test_gather_refuses_strides_out_of_range():
     assert _gather(dict(dst_inner_stride=96), inner=2, kstride=2 ** 41) == gb.OUT_OF_RANGE
+
+
+def _accumulate(score=MB, weights=64 * MB, groups=3, rows=2, length=16, stride=16, lengths=None, row_lengths=None, out=2 * MB):
+    return _capi.lib().gsx_b200_budget_accumulate(score, stride, weights, 0, 32, 16, groups, rows, length, lengths, row_lengths,
+                                                  1.0, out, stride, None)
+
+
+@pytest.mark.parametrize("kw", [dict(lengths=2 * MB), dict(row_lengths=2 * MB + 188), dict(lengths=2 * MB - 8),
+                                dict(row_lengths=2 * MB + 124, stride=32), dict(out=MB, lengths=MB + 64)])
+def test_accumulate_refuses_an_out_over_the_lengths(kw):
+    assert _accumulate(**kw) == gb.INVALID_ARGUMENT
+    assert b"overlap" in _capi.lib().gsx_b200_last_error()
