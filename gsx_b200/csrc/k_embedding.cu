@@ -1616,6 +1616,13 @@ extern "C" int gsx_b200_embedding_backward(const void *grad_out, int grad_type, 
     if(workspace_bytes < plan.bytes)
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT,
                                  "workspace is smaller than gsx_b200_embedding_workspace_bytes");
+    {
+        const uint64_t tb = float_bytes(table_type), ob = float_bytes(grad_type), ib = index_type == GSX_B200_DATA_I32 ? 4 : 8;
+        if(overlap(workspace, 1, 0, plan.bytes, grad_table, rows, table_stride * tb, dim * tb) ||
+           overlap(workspace, 1, 0, plan.bytes, grad_out, count, grad_stride * ob, dim * ob) ||
+           overlap(workspace, 1, 0, plan.bytes, index, 1, 0, count * ib))
+            return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "workspace must not overlap grad_table, grad_out or index");
+    }
     cudaStream_t stream = (cudaStream_t)stream_;
     unsigned char *ws = static_cast<unsigned char *>(workspace);
     const Use use = { (uint32_t)rows, padding_row < 0 ? UINT32_MAX : (uint32_t)padding_row, device_out_of_range };

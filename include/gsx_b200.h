@@ -410,7 +410,7 @@ GSX_B200_API int gsx_b200_adc_select_keep(uint64_t n, const float *opacity, cons
  * as they are).  The positions are sorted by row first, so every sum runs in the order of n whatever the
  * launch: the same inputs give the same bits.  Sums are f32, rounded once.  scale must be finite.  Indices equal to padding_row (-1: none)
  * take no part.  workspace: gsx_b200_embedding_workspace_bytes(count, rows, dim) bytes of device memory, 16-byte
- * aligned, of any content; calls that overlap on the GPU need one each.
+ * aligned, of any content, that overlaps no other argument; calls that overlap on the GPU need one each.
  */
 GSX_B200_API int gsx_b200_embedding_lookup(const void *table, int table_type, uint64_t rows, uint64_t dim,
                                            uint64_t table_stride, const void *index, int index_type, uint64_t count,

@@ -145,3 +145,17 @@ def _accumulate(score=MB, weights=64 * MB, groups=3, rows=2, length=16, stride=1
 def test_accumulate_refuses_an_out_over_the_lengths(kw):
     assert _accumulate(**kw) == gb.INVALID_ARGUMENT
     assert b"overlap" in _capi.lib().gsx_b200_last_error()
+
+
+def _backward(grad=64 * MB, index=32 * MB, itype=13, count=20, table=MB, rows=4, dim=8, stride=8, ws=8 * MB):
+    L = _capi.lib()
+    return L.gsx_b200_embedding_backward(grad, 0, stride, index, itype, count, 1.0, -1, table, 0, rows, dim, stride, 0, ws,
+                                         L.gsx_b200_embedding_workspace_bytes(count, rows, dim), None, None)
+
+
+@pytest.mark.parametrize("kw", [dict(ws=MB), dict(ws=MB + 112), dict(ws=MB - 256), dict(ws=64 * MB + 624), dict(ws=64 * MB - 16),
+                                dict(ws=32 * MB + 144), dict(ws=32 * MB - 256), dict(ws=MB, rows=5000, count=9000),
+                                dict(ws=32 * MB + 35_984, itype=12, rows=5000, count=9000)])
+def test_backward_refuses_a_workspace_over_its_operands(kw):
+    assert _backward(**kw) == gb.INVALID_ARGUMENT
+    assert b"overlap" in _capi.lib().gsx_b200_last_error()
