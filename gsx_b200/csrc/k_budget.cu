@@ -1150,7 +1150,8 @@ extern "C" int gsx_b200_budget_gather(const gsx_b200_gather_field *fields, int32
         return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "outer * inner, length and budget must be below 2^31");
     if(outer * inner == 0 || budget == 0 || field_count == 0) return GSX_B200_SUCCESS;
     if(keep == nullptr || kept == nullptr) return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "keep and kept must be non-null");
-    if((uintptr_t)keep % 4 || (uintptr_t)kept % 4) return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "pointers must be aligned to 4 bytes");
+    if((uintptr_t)keep % 4 || (uintptr_t)kept % 4 || (uintptr_t)device_out_of_range % 4)
+        return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "pointers must be aligned to 4 bytes");
     if(outer * inner > 1 && keep_stride < budget)
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "keep_stride must be at least budget");
     if(outer * inner > 1 && keep_stride > (1ull << 40)) return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "keep_stride must be at most 2^40 elements");

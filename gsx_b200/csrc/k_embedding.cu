@@ -1543,7 +1543,7 @@ extern "C" int gsx_b200_embedding_lookup(const void *table, int table_type, uint
     if((rows > 0 && table == nullptr) || index == nullptr || out == nullptr)
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "table, index and out must be non-null");
     if((uintptr_t)table % float_bytes(table_type) || (uintptr_t)out % float_bytes(out_type) ||
-       (uintptr_t)index % (index_type == GSX_B200_DATA_I32 ? 4 : 8))
+       (uintptr_t)index % (index_type == GSX_B200_DATA_I32 ? 4 : 8) || (uintptr_t)device_out_of_range % 4)
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "pointers must be aligned to their element type");
     if(table_stride * float_bytes(table_type) > 0xffffffffull)
         return gsx_internal_fail(GSX_B200_OUT_OF_RANGE, "table_stride must be below 4 GiB");
@@ -1590,7 +1590,7 @@ extern "C" int gsx_b200_embedding_backward(const void *grad_out, int grad_type, 
     if(grad_table == nullptr || workspace == nullptr || (count > 0 && (grad_out == nullptr || index == nullptr)))
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "grad_out, index, grad_table and workspace must be non-null");
     if((uintptr_t)grad_out % float_bytes(grad_type) || (uintptr_t)grad_table % float_bytes(table_type) ||
-       (uintptr_t)index % (index_type == GSX_B200_DATA_I32 ? 4 : 8) || (uintptr_t)workspace % 16)
+       (uintptr_t)index % (index_type == GSX_B200_DATA_I32 ? 4 : 8) || (uintptr_t)device_out_of_range % 4 || (uintptr_t)workspace % 16)
         return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT,
                                  "pointers must be aligned to their element type, the workspace to 16 bytes");
     if(!(scale - scale == 0.0f)) return gsx_internal_fail(GSX_B200_INVALID_ARGUMENT, "scale must be finite");

@@ -159,3 +159,13 @@ def _backward(grad=64 * MB, index=32 * MB, itype=13, count=20, table=MB, rows=4,
 def test_backward_refuses_a_workspace_over_its_operands(kw):
     assert _backward(**kw) == gb.INVALID_ARGUMENT
     assert b"overlap" in _capi.lib().gsx_b200_last_error()
+
+
+def test_a_flag_that_is_not_aligned_is_refused():
+    """The kernels exchange it as one 32-bit word."""
+    L = _capi.lib()
+    bad = 128 * MB + 2
+    assert L.gsx_b200_embedding_lookup(MB, 0, 4, 8, 8, 2 * MB, 12, 3, 1.0, 3 * MB, 0, 8, bad, None) == gb.INVALID_ARGUMENT
+    assert L.gsx_b200_embedding_backward(MB, 0, 8, 2 * MB, 12, 3, 1.0, -1, 3 * MB, 0, 4, 8, 8, 0, 8 * MB, 1 << 40, bad,
+                                         None) == gb.INVALID_ARGUMENT
+    assert _gather({}, bad=bad) == gb.INVALID_ARGUMENT
