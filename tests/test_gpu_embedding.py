@@ -384,3 +384,42 @@ def test_refusals(cuda_device):
     refused(gb.INVALID_ARGUMENT, gb.embedding_backward, grad, index, table[:1].expand(10, 4))
     refused(gb.OUT_OF_RANGE, gb.embedding_backward, grad, index, table, padding_row=10)
     refused(gb.NOT_SUPPORTED, gb.embedding_backward, grad.double(), index, table)
+
+
+def _check_whole(got, grad, index, rows, scale=1.0, before=None):
+    """Whole numbers (and a scale that is a power of two): every sum below 2^24 is exact in any order, so the result is
+    the formula's to the bit, however many positions a row has."""
+    use = (index >= 0) & (index < rows)
+    want = torch.zeros(rows, grad.shape[1], dtype=torch.float64, device="cuda").index_add_(0, index[use].long(), grad[use].double())
+    assert float(torch.zeros_like(want).index_add_(0, index[use].long(), grad[use].double().abs()).max()) < 2 ** 24
+    want = want * scale + (0 if before is None else before.double())
+    assert torch.equal(got.double(), want)
+
+
+@pytest.mark.parametrize("grad_type", [F32, BF16])
+@pytest.mark.parametrize("count,rows,dim", GRADIENT_SIZES)
+def test_gradient_sums_of_whole_numbers_are_exact(cuda_device, count, rows, dim, grad_type):
+    """No part of a long row is lost or added twice: the bound of a sum of n rounded terms grows with n and would not see
+    it."""
+    g = _gen(count + rows + 1)
+    grad = torch.randint(-4, 5, (count, dim), generator=g, device="cuda").to(grad_type)
+    index = _index(g, count, rows, torch.int64, 2.0)
+    index[3::101] = -1
+    got = gb.embedding_backward(grad, index, torch.empty(rows, dim, device="cuda"), scale=0.5)
+    _check_whole(got, grad, index, rows, 0.5)
+    before = torch.randint(-9, 10, (rows, dim), generator=g, device="cuda").float()
+    got = gb.embedding_backward(grad, index, before.clone(), scale=-2.0, accumulate=True)
+    _check_whole(got, grad, index, rows, -2.0, before)
+
+
+@pytest.mark.parametrize("start", [0, 1])
+@pytest.mark.parametrize("count", [3000, 40_000, 300_000, 800_000])
+@pytest.mark.parametrize("dim", [3, 64, 300])
+def test_whole_sums_of_one_row_that_has_nearly_all(cuda_device, count, dim, start):
+    g = _gen(15)
+    grad = torch.randint(1, 5, (count * dim + start,), generator=g, device="cuda").float()[start:].view(count, dim)
+    index = torch.full((count,), 4, dtype=torch.int32, device="cuda")
+    index[::97] = _index(g, index[::97].numel(), 9, torch.int32)
+    _check_whole(gb.embedding_backward(grad, index, torch.empty(9, dim, device="cuda")), grad, index, 9)
+    wide = torch.empty(30_000, dim, device="cuda")  # a table of its own size: the sort of all positions
+    _check_whole(gb.embedding_backward(grad, index, wide), grad, index, 30_000)
