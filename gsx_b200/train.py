@@ -8,6 +8,8 @@ contiguous span (no per-field launches, no packing copies).
 """
 from __future__ import annotations
 
+import math
+
 import numpy as np
 import torch
 
@@ -133,8 +135,14 @@ class Trainer:
         for f, rows in self.shared.items():
             if f not in model.fields or rows.table.dtype != torch.float32 or rows.index.shape != (model.n,):
                 raise GsxError(NOT_SUPPORTED, "shared rows need a field of the model, a float32 table and an index per Gaussian")
-            if not rows.table.is_contiguous():
-                raise GsxError(INVALID_ARGUMENT, f"the table of {f} must be contiguous")
+            if rows.table.shape[1:] != (math.prod(FIELD_COLS[f]),):
+                raise GsxError(INVALID_ARGUMENT, f"the table of {f} must be [rows, {math.prod(FIELD_COLS[f])}]")
+            if any(t.device != model.params[f].device or not t.is_contiguous() for t in (rows.table, rows.index)):
+                raise GsxError(INVALID_ARGUMENT, f"the table and the row numbers of {f} must be contiguous and on the model's device")
+            if rows.index.dtype not in (torch.int32, torch.int64):
+                raise GsxError(NOT_SUPPORTED, f"the row numbers of {f} must be int32 or int64")
+            if bool(((rows.index < 0) | (rows.index >= rows.table.shape[0])).any()):
+                raise GsxError(OUT_OF_RANGE, f"a row number of {f} lies outside the table")
         # two groups of one Adam launch over the same memory would race, and each backward would overwrite the other's gradient
         spans = sorted((r.table.data_ptr(), r.table.data_ptr() + r.table.numel() * 4) for r in self.shared.values())
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])) or len({id(r) for r in self.shared.values()}) < len(self.shared):
@@ -146,11 +154,6 @@ class Trainer:
         if self.sharded is None:
             self.optim = Adam(self._groups())
         self._expand_shared()
-        for f, rows in self.shared.items():
-            try:
-                rows.check()
-            except GsxError as e:
-                raise GsxError(e.code, f"{f}: {e.message}") from None
 
     def _expand_shared(self):
         """Every shared field's rows from its table."""

@@ -298,3 +298,20 @@ def test_blend_weights_leave_the_density_statistics_alone(cuda_device):
     assert all(bool((t != 3.0).any()) for t in stats)
     tr.ctx.bind_aux()
     tr.blend_weights(cam, torch.zeros(800, device="cuda"))
+
+
+def test_a_trainer_that_is_refused_leaves_its_model_alone(cuda_device):
+    tr, _, _ = _trainer(n=300, fields=(), sh_degree=1)
+    m = tr.model
+    before = m.flat_param.clone()
+    good = SharedRows(torch.randn(20, 3, device="cuda"), torch.zeros(300, dtype=torch.int32, device="cuda"))
+    table, index = torch.randn(20, 9, device="cuda"), torch.zeros(300, dtype=torch.int64, device="cuda")
+    for code, other in [(gb.INVALID_ARGUMENT, SharedRows(table[:, :8].contiguous(), index)),
+                        (gb.INVALID_ARGUMENT, SharedRows(table[:, 0].contiguous(), index)),
+                        (gb.INVALID_ARGUMENT, SharedRows(table, index.cpu())), (gb.INVALID_ARGUMENT, SharedRows(table.cpu(), index)),
+                        (gb.INVALID_ARGUMENT, SharedRows(table, index.repeat(2)[::2])), (gb.NOT_SUPPORTED, SharedRows(table, index.short())),
+                        (gb.OUT_OF_RANGE, SharedRows(table, index + 20)), (gb.OUT_OF_RANGE, SharedRows(table, index - 1))]:
+        with pytest.raises(gb.GsxError) as e:
+            Trainer(m, W, H, shared={"sh0": good, "sh1": other})
+        assert e.value.code == code, e.value
+        assert torch.equal(m.flat_param, before)
