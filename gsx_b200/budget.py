@@ -72,7 +72,8 @@ def budget_select(score, budget: int, lengths=None, first: int = 0, recent: int 
     """(keep, kept): per group the increasing list of the entries that stay within `budget` (the `first` first,
     the `recent` last, and the largest scores of the others, ties to the lowest index; NaN is below every number)
     and its length min(entries in use, budget).  keep is int32, leading shape + (at least min(budget, length),);
-    drop, where given, int32 of score's shape, receives the others.  Places behind the lists are left as they were.  No output may overlap another or an input."""
+    drop, where given, int32 of score's shape, receives the others.  Places behind the lists are left as they were.
+    No output may overlap another or an input (kept is not lengths updated in place)."""
     groups, length, stride = _score(score)
     lead = score.shape[:-1]
     if (groups | length | budget) >> 31:

@@ -78,10 +78,6 @@ __device__ __forceinline__ void add_rows(float (&acc)[VW], const T *__restrict__
         for(int v = 0; v < VW; ++v) acc[v] += to_f32(x[u].v[v]);
 }
 
-/* A cluster of CTAs owns kThreads / RG * VW columns of one group and deals their rows out: row r goes to CTA
- * (r / RG) mod clusters, thread row r mod RG.  A thread keeps U rows in flight; the RG threads of a column are joined in
- * shared memory, the CTAs in distributed shared memory, each in a fixed order.  SPREAD, for rows that no 4-byte access
- * fits: a thread's VW columns lie CT apart, so that the lanes' single elements stay side by side. */
 /* VW consecutive floats in accesses of up to 16 bytes */
 template <int VW>
 __device__ __forceinline__ void load_floats(float (&x)[VW], const float *from)
@@ -108,6 +104,10 @@ __device__ __forceinline__ void store_floats(float *to, const float (&x)[VW])
     }
 }
 
+/* A cluster of CTAs owns kThreads / RG * VW columns of one group and deals their rows out: row r goes to the cluster's CTA
+ * (r / RG) mod splits, thread row r mod RG.  A thread keeps U rows in flight; the RG threads of a column are joined in
+ * shared memory, the CTAs in distributed shared memory, each in a fixed order.  SPREAD, for rows that no 4-byte access
+ * fits: a thread's VW columns lie CT apart, so that the lanes' single elements stay side by side. */
 template <typename T, int VW, int RG, bool SPREAD>
 __global__ void __launch_bounds__(kThreads, kAccumulateCtas) accumulate_kernel(const float *score, uint64_t score_stride,
                                                               const T *__restrict__ weights, uint64_t group_stride,

@@ -36,8 +36,8 @@ def embedding_lookup(table, index, out=None, scale: float = 1.0, bad=None, strea
 def embedding_backward(grad_out, index, grad_table, scale: float = 1.0, padding_row: int | None = None,
                        accumulate: bool = False, bad=None, stream=None):
     """grad_table[v] = scale * sum of grad_out[n] over index[n] = v, written for every row (added to it when
-    accumulate), in f32 sums whose order does not depend on the launch.  grad_out is index.shape + (dim,),
-    grad_table [rows, dim].  Indices equal to padding_row take no part; out-of-range ones set `bad`."""
+    accumulate), in f32 sums.  Their order depends on the sizes, types, alignment and strides only: the same call
+    gives the same bits.  grad_out is index.shape + (dim,), grad_table [rows, dim].  Indices equal to padding_row take no part; out-of-range ones set `bad`."""
     if grad_table.dim() != 2:
         raise invalid("grad_table must be [rows, dim]")
     rows, dim = grad_table.shape

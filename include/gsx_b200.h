@@ -407,8 +407,9 @@ GSX_B200_API int gsx_b200_adc_select_keep(uint64_t n, const float *opacity, cons
  * gsx_b200_embedding_lookup: out[n] = scale * table[index[n]], computed in f32 and rounded once.
  * gsx_b200_embedding_backward: grad_table[v] = scale * (sum of grad_out[n] over index[n] = v), written for every
  * row (zero where no index names it), or added to it when accumulate != 0 (rows that no index names are then left
- * as they are).  The positions are sorted by row first, so every sum runs in the order of n whatever the
- * launch: the same inputs give the same bits.  Sums are f32, rounded once.  scale must be finite.  Indices equal to padding_row (-1: none)
+ * as they are).  Sums are f32, rounded once, in an order that depends only on count, rows, dim, the types, and the alignment
+ * and strides of grad_out and grad_table (which decide between packs and single elements): the same call gives the same
+ * bits, and an equal one from a start of another alignment may differ in the last ones.  scale must be finite.  Indices equal to padding_row (-1: none)
  * take no part.  workspace: gsx_b200_embedding_workspace_bytes(count, rows, dim) bytes of device memory, 16-byte
  * aligned, of any content, that overlaps no other argument; calls that overlap on the GPU need one each.
  */
